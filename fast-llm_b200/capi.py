@@ -29,7 +29,7 @@ SYMBOLS = [
     "fl_b200_dequant", "fl_b200_matvec", "fl_b200_matvec_assign", "fl_b200_matvec_expert", "fl_b200_matvec_pitched", "fl_b200_matvec_host",
     "fl_b200_attn_decode", "fl_b200_attn_decode_lse", "fl_b200_seqpar_create", "fl_b200_seqpar_destroy",
     "fl_b200_seqpar_comm", "fl_b200_seqpar_set_peers", "fl_b200_seqpar_combine", "fl_b200_attn_verify", "fl_b200_attn_decode_static", "fl_b200_attn_decode_host", "fl_b200_rmsnorm", "fl_b200_add2",
-    "fl_b200_silu_mul", "fl_b200_router_sel", "fl_b200_wmerge", "fl_b200_rope_kv_append", "fl_b200_argmax", "fl_b200_exec_task", "fl_b200_plan_create", "fl_b200_plan_run", "fl_b200_plan_info", "fl_b200_plan_destroy",
+    "fl_b200_silu_mul", "fl_b200_router_sel", "fl_b200_wmerge", "fl_b200_rope_kv_append", "fl_b200_argmax", "fl_b200_paged_plan", "fl_b200_paged_append", "fl_b200_paged_attn", "fl_b200_exec_task", "fl_b200_plan_create", "fl_b200_plan_run", "fl_b200_plan_info", "fl_b200_plan_destroy",
     "fl_b200_decoder_create", "fl_b200_decoder_create_tp", "fl_b200_decoder_comm", "fl_b200_decoder_set_peers",
     "fl_b200_decoder_destroy", "fl_b200_decoder_set_layer_tensor",
     "fl_b200_decoder_set_layer_norms", "fl_b200_decoder_set_layer_moe", "fl_b200_decoder_set_global", "fl_b200_decoder_set_out_norm",

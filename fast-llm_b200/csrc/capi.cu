@@ -90,6 +90,7 @@ int fl_b200_create(int device, fl_b200_ctx **out) {
     CK(cudaMalloc(&c->xq, matmul_tc_nx_scratch_bytes(kNxMaxCols, kNxTgs, 3)));
     CK(cudaMalloc(&c->nx_part, kNxPartFloats * sizeof(float)));
     CK(attn_init());
+    CK(paged_init());
     *out = c;
     return FL_B200_OK;
 }
@@ -102,6 +103,8 @@ void fl_b200_destroy(fl_b200_ctx *c) {
     cudaFree(c->xq); cudaFree(c->nx_part);
     for (void *p : c->retired) cudaFree(p);
     cudaFree(c->attn_tickets);
+    cudaFree(c->paged_part);
+    cudaFree(c->paged_tickets);
     cudaFree(c->argmax_scratch);
     cudaFree(c->small);
     cudaFree(c->status);

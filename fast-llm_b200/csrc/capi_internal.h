@@ -30,6 +30,8 @@ struct fl_b200_ctx {
     // Scratch buffers that were outgrown. A recorded plan (fl_b200_plan) keeps the address it was
     // captured with, so an outgrown buffer stays allocated until the context goes.
     std::vector<void *> retired;
+    float *paged_part = nullptr;         // records of the attention over pages (fixed size, made by the first call)
+    uint32_t *paged_tickets = nullptr;   // zero between launches
     float *argmax_scratch = nullptr;
     void *small = nullptr;
     uint8_t *xq = nullptr;               // converted activations of the multi-column matmul (fixed size, see fl_b200_create)

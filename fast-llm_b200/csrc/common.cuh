@@ -16,6 +16,9 @@ enum : uint32_t {
     ST_OK = 0,
     ST_WAIT_TIMEOUT = 1,   // a bounded mbarrier wait gave up
     ST_PEER_TIMEOUT = 2,   // a bounded wait for another rank's flag gave up
+    ST_PAGED_PAGE = 3,     // a block table or slot names a page outside the pool
+    ST_PAGED_ARGS = 4,     // lengths of a paged call that contradict each other or its bounds
+    ST_PAGED_FULL = 5,     // a plan needs more pages or tokens than there are
 };
 
 __host__ __device__ inline uint32_t blk_elems(int fmt) {

@@ -79,6 +79,7 @@ struct MatvecArgs {
 // 2-D tiled TMA descriptor over a row-major array (rows x dim0 elements, row pitch stride_bytes).
 cudaError_t tensor_map_2d(CUtensorMap *m, uint32_t elem_bytes, const void *base, uint64_t dim0, uint64_t rows,
                           uint64_t stride_bytes, uint32_t box0, uint32_t box_rows, bool swizzle128);
+cudaError_t tensor_map_groups_swz(CUtensorMap *m, const void *base, uint64_t rows, uint32_t cols, uint32_t box_rows);
 cudaError_t tensor_map_lines_swz(CUtensorMap *m, const void *base, uint64_t rows, uint64_t pitch, uint32_t box_lines,
                                  uint32_t box_rows);   // [rows][pitch / 128][128 bytes], 128-byte swizzle (matvec.cu)
 cudaError_t launch_matvec(const MatvecArgs &a, int sms, cudaStream_t stream);
@@ -229,6 +230,7 @@ cudaError_t launch_attn_decode_static(AttnArgs a, int device, cudaStream_t strea
 size_t attn_static_max_records(void);
 uint32_t attn_static_max_tickets(void);
 cudaError_t attn_init(void);
+cudaError_t paged_init(void);   // paged.cu
 uint32_t attn_pick_splits(uint32_t n_kv_head, uint32_t batch, uint32_t kv_len, int sms, bool shared_kv = false);
 uint32_t attn_used_splits(uint32_t n_splits, uint32_t kv_len);   // those of n_splits that hold keys when kv_len keys are cut
 size_t attn_part_floats(uint32_t n_q_head, uint32_t batch, uint32_t n_splits);

@@ -864,6 +864,24 @@ cudaError_t tensor_map_lines_swz(CUtensorMap *m, const void *base, uint64_t rows
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+// Rows of 64 or 128 f16, packed, seen as [groups of 8 rows][cols / 64][8 rows][64] with the 128-byte swizzle: a box of box_rows
+// rows (a multiple of 8) lands in shared memory as its groups one after another, each cols / 64 blocks of 8 lines of 128 bytes.
+cudaError_t tensor_map_groups_swz(CUtensorMap *m, const void *base, uint64_t rows, uint32_t cols, uint32_t box_rows) {
+    if (!g_encode) {
+        const cudaError_t e = matvec_init();
+        if (e != cudaSuccess) return e;
+    }
+    if ((cols != 64 && cols != 128) || rows % 8 || box_rows % 8) return cudaErrorInvalidValue;
+    const cuuint64_t gdim[4] = {64, 8, cols / 64, rows / 8};
+    const cuuint64_t gstride[3] = {cols * 2, 128, (cuuint64_t)cols * 16};
+    const cuuint32_t box[4] = {64, 8, cols / 64, box_rows / 8};
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    const CUresult r = g_encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void *>(base), gdim, gstride, box, estr,
+                                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 cudaError_t launch_matvec(const MatvecArgs &a, int sms, cudaStream_t stream) {
     if (a.n_tensors < 1 || a.n_tensors > 4 || a.cols == 0) return cudaErrorInvalidValue;
     if (matvec_tc_eligible(a)) return launch_matvec_tc(a, sms, stream);

@@ -1,0 +1,60 @@
+// Paged KV cache: launch interface between paged.cu (C ABI, plan, append) and the attention kernels over pages.
+//
+// Layout: K and V are pools of pages, each [n_pages][n_kv_head][page_size][head_dim] f16, so that a page of one KV head is one
+// contiguous piece as in the unpaged cache. Slot p * page_size + r is row r of page p. A sequence's block table names its pages
+// in order: key j lies in slot table[j / page_size] * page_size + j % page_size.
+#pragma once
+#include "../../include/fl_b200.h"
+#include "kernels.h"
+
+namespace flb {
+
+constexpr uint32_t kPagedMaxSeq = 4096;   // sequences of a call: the plan keeps three prefix sums of them in shared memory
+
+// ---- attention over pages -------------------------------------------------------------------------------------------
+// Rows: row r of a sequence with n new tokens is token r / group, query head hkv * group + r % group (group = n_q_head / n_kv_head).
+// Token i of n attends keys 0 .. kv_len - n + i. A block of rows over one KV head walks tiles of keys; the tiles of all blocks lie
+// on one line and every CTA takes an equal, contiguous piece of it, so that ragged batches load all SMs alike. A block that several
+// CTAs share leaves one record per CTA; the CTA that arrives last adds them in order (no CTA waits for another).
+struct PagedAttnArgs {
+    CUtensorMap kmap, vmap;         // tensor_map_groups_swz: one copy per page; the layout of ldmatrix and tcgen05 operands alike
+    const void *q;
+    void *out;
+    float2 *lse;                    // optional
+    const int32_t *table, *q_start, *kv_len;
+    float *part;                    // records
+    uint32_t *tickets;              // zero between launches
+    uint32_t *status;
+    uint64_t q_stride, out_stride;  // elements between tokens
+    uint32_t n_seq, max_blocks, n_tokens, max_new, n_pages, page_shift;
+    uint32_t n_kv, group, half;     // half: activations are f16
+    float scale;
+};
+
+// Few rows per sequence and KV head (mma.sync). kmap and vmap are filled in here.
+cudaError_t paged_few_init(void);
+size_t paged_few_part_bytes(int sms);
+cudaError_t launch_paged_few(PagedAttnArgs a, const void *k, const void *v, uint32_t head_dim, int sms, cudaStream_t stream);
+constexpr uint32_t kPagedTickets = 1024;   // at least the CTAs of a launch
+
+#if defined(__CUDACC__)
+// One sequence of an attention call, checked: n = 0 where its lengths do not fit the call (reported by `report`).
+struct PagedSeq { uint32_t first, n; int32_t past; };   // past = kv_len - n; may be negative (rows without a key)
+__device__ __forceinline__ PagedSeq paged_seq(const PagedAttnArgs &a, uint32_t s, bool &bad) {
+    const int32_t b = a.q_start[s], e = a.q_start[s + 1], len = a.kv_len[s];
+    const uint64_t room = (uint64_t)a.max_blocks << a.page_shift;
+    bad = b < 0 || e < b || (uint32_t)e > a.n_tokens || (uint32_t)(e - b) > a.max_new || len < 0 || (uint64_t)len > room;
+    return bad ? PagedSeq{0, 0, 0} : PagedSeq{(uint32_t)b, (uint32_t)(e - b), len - (e - b)};
+}
+__device__ __forceinline__ uint64_t share_of(uint64_t units, uint32_t grid, uint32_t c) { return units * c / grid; }
+// The CTA whose share holds unit u.
+__device__ __forceinline__ uint32_t owner_of(uint64_t units, uint32_t grid, uint64_t u) { return (uint32_t)(((u + 1) * grid - 1) / units); }
+
+__device__ __forceinline__ float exp2_fast(float x) {   // 2^x to 2^-22 of its value, 0 for -inf
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+#endif
+
+} // namespace flb

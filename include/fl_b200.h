@@ -66,7 +66,8 @@ const char *fl_b200_last_error(void);
 int fl_b200_create(int device, fl_b200_ctx **out);
 void fl_b200_destroy(fl_b200_ctx *ctx);
 int fl_b200_sync(fl_b200_ctx *ctx);
-/* Reads and clears the device status word (0 = no kernel reported a problem). */
+/* Reads and clears the device status word (0 = no kernel reported a problem, 1 a wait of a kernel's own ran out, 2 a peer
+ * time-out, 3 to 5 see the paged KV cache). */
 int fl_b200_device_status(fl_b200_ctx *ctx, uint32_t *status_out);
 int fl_b200_sm_count(fl_b200_ctx *ctx);
 /* Limit, in nanoseconds of the device clock, of the waits of the exchange kernels for another rank's
@@ -202,6 +203,59 @@ int fl_b200_rope_kv_append(fl_b200_ctx *ctx, float *q_dev, const float *k_dev, c
  * (src/model/decoder.cpp:1253-1264). */
 int fl_b200_argmax(fl_b200_ctx *ctx, const float *logits_dev, uint32_t n, int32_t *idx_dev,
                    float *margin_dev);
+
+/* ---- paged KV cache: many sequences of unlike length in one pool of pages (nothing in the reference, whose decoder holds one
+ *      sequence in one cache). Per step fl_b200_paged_plan, per layer fl_b200_paged_append and fl_b200_paged_attn; all three
+ *      work from lengths on the device, allocate nothing (but for the first fl_b200_paged_attn of a context, see there) and can be
+ *      captured into a graph. Calls of one context share scratch: graphs captured from one context's stream
+ *      are not to run at the same time. What a kernel finds wrong on the device goes to the status word
+ *      (fl_b200_device_status): 3 a table or slot names a page outside the pool, 4 lengths that contradict each other or the
+ *      call's bounds, 5 a plan that needs more pages or tokens than there are; nothing is read or written out of bounds. ---- */
+/* K and V of one layer: two pools [n_pages][n_kv_head][page_size][head_dim] f16, 16-byte aligned. head_dim 64 or 128; page_size
+ * 16, 32, 64, 128 or 256; n_pages * n_kv_head * page_size < 2^31. Slot p * page_size + r is row r of page p. */
+typedef struct {
+    uint16_t *k_dev, *v_dev;
+    uint32_t n_pages, page_size, n_kv_head, head_dim;
+} fl_b200_paged_cache;
+/* Activations of the paged calls: f32 as everywhere else in this library, or f16. */
+enum { FL_B200_ACT_F32 = 0, FL_B200_ACT_F16 = 1 };
+/* The plan of a step, from the sequences' lengths: sequence s (of n_seq <= 4096) holds the pages of held[s] tokens, keeps the
+ * first past[s] <= held[s] of them and gets fresh[s] more (a prompt: held = past = 0; a rewound draft: past < held; an ended
+ * request: past = fresh = 0). Row s of the block table ([n_seq][max_blocks]) names its pages in order, and the first
+ * free_count entries of free_list ([n_pages]) the unused ones, the last of them the next to go. Pages that past + fresh tokens do not
+ * need go onto the list in order of (s, block); then the missing ones are taken from its end in the same order and written into
+ * the table behind the ones held. Other entries of table and list stay as they are. Outputs: *free_count_out (may be
+ * free_count_in itself), q_start[n_seq + 1] = first token of each sequence in the step's batch, kv_len[s] = past + fresh (may be held,
+ * past or fresh itself), and per token of the batch its position and its slot; the rest of pos and slot (max_tokens
+ * each) is -1. Where pages or max_tokens do not suffice (status 5) or lengths are impossible (status 4) the plan is empty: q_start 0, every
+ * pos and slot -1, all else unchanged. No page may be listed twice. Other buffers must not overlap. */
+int fl_b200_paged_plan(fl_b200_ctx *ctx, const int32_t *held_dev, const int32_t *past_dev, const int32_t *fresh_dev,
+                       uint32_t n_seq, uint32_t page_size, int32_t *table_dev, uint32_t max_blocks, int32_t *free_list_dev,
+                       uint32_t n_pages, const int32_t *free_count_in_dev, int32_t *free_count_out_dev, int32_t *q_start_dev,
+                       int32_t *kv_len_dev, int32_t *pos_dev, int32_t *slot_dev, uint32_t max_tokens);
+/* fl_b200_rope_kv_append for a ragged batch: plain RoPE on adjacent pairs of the first n_rot (even, <= head_dim; 0: none)
+ * dimensions of every q and k head, pair i of token t by pos[t] * freq_base^(-2i / n_rot), formed in 64 bits (far positions keep their
+ * angle; the unpaged operator multiplies up in 32 bits as the reference does); q goes to q_out (which may be q, with its stride), k and v rounded
+ * to f16 into row slot[t] of the cache. A token with pos -1 is left out altogether, one with slot -1 is not appended. Slots of a call must
+ * differ. q [n_tokens][q_stride] with n_q_head heads from the start of a row (n_q_head 0: no q), k and v [n_tokens][kv_stride]; strides
+ * in elements, rows 16-byte aligned, so that q, k and v can be parts of one projection's rows. */
+int fl_b200_paged_append(fl_b200_ctx *ctx, const fl_b200_paged_cache *cache, int act_type, const void *q_dev, uint32_t n_q_head,
+                         uint32_t q_stride, const void *k_dev, const void *v_dev, uint32_t kv_stride, const int32_t *pos_dev,
+                         const int32_t *slot_dev, uint32_t n_tokens, uint32_t n_rot, float freq_base, void *q_out_dev,
+                         uint32_t q_out_stride);
+/* Causal grouped-query attention of every sequence's new tokens over its pages: fl_b200_attn_decode, fl_b200_attn_verify and prompt chunks in
+ * one call. Sequence s has tokens q_start[s] .. q_start[s + 1] - 1 of the batch and kv_len[s] keys, its new tokens' own
+ * the last of them; token i of n attends keys 0 .. kv_len - n + i. A token without a key gets zeros. n_q_head is a multiple of
+ * n_kv_head (groups of up to 128), q and out [n_tokens][stride] as above, table [n_seq][max_blocks], scale positive. n_tokens: rows of q and
+ * out; max_new: the most new tokens any sequence has. Sequences whose lengths break these bounds are left out (status 4), rows of
+ * out that belong to no sequence stay as they are, keys on a page outside the pool count as zero vectors (status 3). lse_out
+ * (optional): per token and query head (max score, sum of exp(score - max)), (-inf, 0) without a key: what fl_b200_seqpar_combine merges.
+ * f32 activations: q and the probabilities go to the tensor cores as two f16 parts each (22 bits), sums in f32; f16
+ * activations: as one. Scores within 2^-120 .. 2^120. The first call on a context allocates scratch: make it before a capture. */
+int fl_b200_paged_attn(fl_b200_ctx *ctx, const fl_b200_paged_cache *cache, int act_type, const void *q_dev, uint32_t n_q_head,
+                       uint32_t q_stride, const int32_t *table_dev, uint32_t max_blocks, const int32_t *q_start_dev,
+                       const int32_t *kv_len_dev, uint32_t n_seq, uint32_t n_tokens, uint32_t max_new, float scale, void *out_dev,
+                       uint32_t out_stride, float *lse_out_dev);
 
 /* ---- task-level entry: one reference Task on the device ------------------
  * Field-for-field image of fastllm::Task (include/fastllm/fastllm.h:65-97);
