@@ -1,20 +1,20 @@
-// Attention over a paged cache, few rows per sequence and KV head: blocks of 16 rows (token, query head of the group) against
-// tiles of 64 keys on mma.sync.
+// Attention over a paged cache, few rows per sequence and KV head: up to 16 rows (token, query head of the group) against tiles
+// of 64 keys on mma.sync.
 //
 // o_r = sum_j exp(s_rj - m_r) v_j / sum_j exp(s_rj - m_r), s_rj = scale q_r . k_j, with the running maximum and sum of an online
-// softmax in f32. Bound by the HBM bytes of the keys and values: every tile is read once per block of rows.
+// softmax in f32. Bound by the HBM bytes of the keys and values: every tile is read once.
 //
 // CTA = 4 consumer warps + 1 producer warp, two CTAs per SM. The producer's lanes each copy one page's part of a tile (one TMA box
 // of up to 64 rows) into a ring of three stages of 32 KB; warp w takes keys 16 w .. 16 w + 15 of a tile through
-// ldmatrix. The tiles of all blocks of rows lie on one line (sequence, block, KV head, tile) and every CTA takes an equal piece of it.
+// ldmatrix. All tiles lie on one line (sequence, KV head, tile) and every CTA takes an equal piece of it.
 //   scores : A = 16 rows of q as (hi, lo) f16 parts, scaled by a power of two per row so that both parts stay normal numbers; B = K
 //   softmax: lane (g, t) has rows g and g + 8, keys 2t, 2t + 1 of every 8; row maxima over the 4 lanes of a row
 //   context: A = probabilities as (hi, lo) parts: the scores' accumulators have the layout of that operand; B = V (ldmatrix.trans).
 //            A tile's product starts from zero and is added in f32 with rounding, since the tensor cores truncate their running sum
 //            (1.3e-8 of it per instruction: 1e-5 after 800 tiles).
-// A masked value never meets the tensor core as it is, since 0 x NaN is NaN: rows behind a block's last key are cleared in shared
-// memory, and where rows of a block end at different keys, values that are not finite are taken out there and
-// their effect added to the rows that do attend them (see Unfinite).
+// A masked value never meets the tensor core as it is, since 0 x NaN is NaN: rows behind the last key are cleared in shared
+// memory, and among the keys of the new tokens, which not all rows attend, values that are not finite are taken out there and
+// their effect added to the rows that do attend them (see unfinite_of).
 #include "common.cuh"
 #include "paged.h"
 
@@ -32,14 +32,14 @@ template <int D> struct FewSmem {
     uint8_t ring[kStages][2 * kHalfStage];                                // 1024-byte aligned
     float o[kWarps][kRowsB][36];                                          // a quarter (half, D = 64) of the warps' contexts
     float m[kWarps][kRowsB], l[kWarps][kRowsB];
-    uint32_t unfinite[3][D];                                              // see Unfinite
+    uint32_t unfinite[3][D];                                              // see unfinite_of
     uint64_t full[kStages], empty[kStages];
     uint64_t sum[kThreads / 32];
     uint32_t start_seq, any;
     uint64_t start_off, total;
 };
 
-// Values of +inf, -inf and NaN (class 0, 1, 2) among the keys that only part of a block's rows attend: per class and dimension the
+// Values of +inf, -inf and NaN (class 0, 1, 2) among the keys that only part of the rows attend: per class and dimension the
 // first such key. A row that attends keys 0 .. lim is affected by those <= lim.
 __device__ __forceinline__ float unfinite_of(const uint32_t *u, uint32_t dims, uint32_t d, int32_t lim) {
     const int32_t p = (int32_t)u[d], n = (int32_t)u[dims + d], x = (int32_t)u[2 * dims + d];   // (0x7fffffff: none)
@@ -72,24 +72,15 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t 
 __device__ __forceinline__ void bar_consumers() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 __device__ __forceinline__ void arrive(uint64_t *bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory"); }
 
-// Tiles of a block of rows: at least one, so that somebody writes its rows.
-__device__ __forceinline__ uint32_t tiles_of(const PagedSeq &q, uint32_t blk, uint32_t group, uint32_t &rows, int32_t &keys) {
-    rows = min(kRowsB, q.n * group - blk * kRowsB);
-    keys = max(0, q.past + (int32_t)((blk * kRowsB + rows - 1) / group) + 1);
-    return max(1u, ((uint32_t)keys + kTile - 1) / kTile);
-}
-__device__ __forceinline__ uint64_t units_of(const PagedAttnArgs &a, const PagedSeq &q) {
-    uint64_t u = 0;
-    uint32_t rows;
-    int32_t keys;
-    for (uint32_t b = 0; b * kRowsB < q.n * a.group; ++b) u += tiles_of(q, b, a.group, rows, keys);
-    return u * a.n_kv;
-}
+// Rows of a sequence over one KV head, 0 where it is the other kernel's; its tiles: at least one, so that somebody writes its rows.
+__device__ __forceinline__ uint32_t rows_of(const PagedAttnArgs &a, const PagedSeq &q) { return q.n * a.group > a.few_rows ? 0u : q.n * a.group; }
+__device__ __forceinline__ uint32_t tiles_of(const PagedSeq &q) { return max(1u, ((uint32_t)max(0, q.past + (int32_t)q.n) + kTile - 1) / kTile); }
+__device__ __forceinline__ uint64_t units_of(const PagedAttnArgs &a, const PagedSeq &q) { return rows_of(a, q) ? (uint64_t)tiles_of(q) * a.n_kv : 0u; }
 
-// The pieces of a CTA's share: consecutive tiles of one block of rows over one KV head.
+// The pieces of a CTA's share: consecutive tiles of one sequence over one KV head.
 struct Piece {
     PagedSeq q;
-    uint32_t seq, hkv, blk, rows, tiles, t0, t1;   // tiles t0 .. t1 - 1 of `tiles`
+    uint32_t seq, hkv, rows, tiles, t0, t1;        // tiles t0 .. t1 - 1 of `tiles`
     int32_t keys;
     uint64_t base;                                 // unit of its tile 0
 };
@@ -106,25 +97,19 @@ __device__ __forceinline__ bool next_piece(const PagedAttnArgs &a, Walk &w, Piec
         w.fresh = false;
         p.seq = w.seq;
         p.q = paged_seq(a, p.seq, bad);
-        p.blk = 0; p.hkv = 0;
-        p.base = w.seq_base;
-        p.tiles = tiles_of(p.q, 0, a.group, p.rows, p.keys);
-        while (p.base + (uint64_t)p.tiles * a.n_kv <= w.pos) {   // (blocks of this sequence in front of the share)
-            p.base += (uint64_t)p.tiles * a.n_kv;
-            ++p.blk;
-            p.tiles = tiles_of(p.q, p.blk, a.group, p.rows, p.keys);
-        }
-        p.hkv = (uint32_t)((w.pos - p.base) / p.tiles);
-        p.base += (uint64_t)p.hkv * p.tiles;
+        p.rows = rows_of(a, p.q);
+        p.tiles = tiles_of(p.q);
+        p.hkv = (uint32_t)((w.pos - w.seq_base) / p.tiles);
+        p.base = w.seq_base + (uint64_t)p.hkv * p.tiles;
     } else {
         p.base += p.tiles;
         if (++p.hkv == a.n_kv) {
             p.hkv = 0;
-            ++p.blk;
-            while (p.blk * kRowsB >= p.q.n * a.group) { p.q = paged_seq(a, ++p.seq, bad); p.blk = 0; }
-            p.tiles = tiles_of(p.q, p.blk, a.group, p.rows, p.keys);
+            do { p.q = paged_seq(a, ++p.seq, bad); } while ((p.rows = rows_of(a, p.q)) == 0);
+            p.tiles = tiles_of(p.q);
         }
     }
+    p.keys = max(0, p.q.past + (int32_t)p.q.n);
     p.t0 = (uint32_t)(w.pos - p.base);
     p.t1 = (uint32_t)min((uint64_t)p.tiles, w.hi - p.base);
     w.pos += p.t1 - p.t0;
@@ -231,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
     // ---- consumers ----
     bool first = true;
     while (next_piece(a, walk, p)) {
-        // q of this block: rows g and g + 8, dimensions 2t, 2t + 1 of every 8
+        // q: rows g and g + 8, dimensions 2t, 2t + 1 of every 8
         uint32_t qh[D / 16][4], ql[D / 16][4];
         float f[2];        // score -> exponent of 2, per row
         int32_t lim[2];    // last key of a row
@@ -240,7 +225,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
             bool there[2];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                const uint32_t row = g + 8 * r, at = p.blk * kRowsB + row, tok = at / a.group, head = p.hkv * a.group + at - tok * a.group;
+                const uint32_t row = g + 8 * r, tok = row / a.group, head = p.hkv * a.group + row - tok * a.group;
                 there[r] = row < p.rows;
                 lim[r] = there[r] ? p.q.past + (int32_t)tok : -1;
                 const uint64_t src = there[r] ? (p.q.first + tok) * a.q_stride + (uint64_t)head * D : 0;
@@ -273,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
                     split2(x[r][4 * kb + 2], x[r][4 * kb + 3], qh[kb][2 + r], ql[kb][2 + r]);
                 }
         }
-        const int32_t lim_first = p.q.past + (int32_t)(p.blk * kRowsB / a.group);   // last key that all rows attend
+        const int32_t lim_first = p.q.past;   // last key that all rows attend
         float o[D / 8][4];
 #pragma unroll
         for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
@@ -408,7 +393,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
         for (uint32_t w = 0; w < kWarps; ++w) top = fmaxf(top, sm.m[w][row]);
 #pragma unroll
         for (uint32_t w = 0; w < kWarps; ++w) sum = fmaf(sm.l[w][row], sm.m[w][row] == -INFINITY && top != -INFINITY ? 0.f : exp2_fast(top == -INFINITY ? 0.f : sm.m[w][row] - top), sum);
-        const uint32_t at = p.blk * kRowsB + row, tok = at / a.group, head = p.hkv * a.group + at - tok * a.group;
+        const uint32_t tok = row / a.group, head = p.hkv * a.group + row - tok * a.group;
         const int32_t row_lim = p.q.past + (int32_t)tok;
         const uint64_t dst = (p.q.first + tok) * a.out_stride + (uint64_t)head * D;
         auto put = [&](uint64_t to, const float4 &v) {
@@ -477,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
                     s = fmaf(ml.y, w, s);
                     v.x = fmaf(u.x, w, v.x); v.y = fmaf(u.y, w, v.y); v.z = fmaf(u.z, w, v.z); v.w = fmaf(u.w, w, v.w);
                 }
-                const uint32_t at2 = p.blk * kRowsB + rw, tk = at2 / a.group, hd = p.hkv * a.group + at2 - tk * a.group;
+                const uint32_t tk = rw / a.group, hd = p.hkv * a.group + rw - tk * a.group;
                 const float inv = p.q.past + (int32_t)tk < 0 ? 0.f : 1.f / s;
                 put((p.q.first + tk) * a.out_stride + (uint64_t)hd * D + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
                 if (a.lse && d == 0) put_lse(tk, hd, mx, s);

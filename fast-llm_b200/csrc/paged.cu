@@ -301,7 +301,8 @@ int check_rows(const char *who, const char *what, const void *p, uint32_t n_head
 
 cudaError_t paged_init(void) {
     if (const cudaError_t e = cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(3 * (kPagedMaxSeq + 1) * 4))) return e;
-    return paged_few_init();
+    if (const cudaError_t e = paged_few_init()) return e;
+    return paged_tm_init();
 }
 
 } // namespace flb
@@ -399,7 +400,7 @@ int fl_b200_paged_attn(fl_b200_ctx *c, const fl_b200_paged_cache *cache, int act
         if (cap != cudaStreamCaptureStatusNone)
             return set_err(FL_B200_ERR_STATE, "paged_attn: the first call on a context allocates its scratch; make it before a capture");
         void *part = nullptr, *tickets = nullptr;
-        cudaError_t e = cudaMalloc(&part, paged_few_part_bytes(c->sms));
+        cudaError_t e = cudaMalloc(&part, paged_few_part_bytes(c->sms) + paged_tm_part_bytes(c->sms));
         if (e == cudaSuccess) e = cudaMalloc(&tickets, kPagedTickets * sizeof(uint32_t));
         if (e == cudaSuccess) e = cudaMemsetAsync(tickets, 0, kPagedTickets * sizeof(uint32_t), c->stream);
         if (e != cudaSuccess) {
@@ -420,7 +421,12 @@ int fl_b200_paged_attn(fl_b200_ctx *c, const fl_b200_paged_cache *cache, int act
     a.n_pages = cache->n_pages; a.page_shift = shift;
     a.n_kv = n_kv; a.group = n_q / n_kv; a.half = act == FL_B200_ACT_F16 ? 1u : 0u;
     a.scale = scale;
-    return cuda_err(launch_paged_few(a, cache->k_dev, cache->v_dev, dim, c->sms, c->stream), "paged_attn launch");
+    a.part_tm = c->paged_part + paged_few_part_bytes(c->sms) / sizeof(float);
+    const bool many = (uint64_t)max_new * a.group > kFewRows;
+    a.few_rows = many && n_seq == 1 ? 0 : kFewRows;   // (one sequence: one launch)
+    if (a.few_rows)
+        if (int rc = cuda_err(launch_paged_few(a, cache->k_dev, cache->v_dev, dim, c->sms, c->stream), "paged_attn launch")) return rc;
+    return many ? cuda_err(launch_paged_tm(a, cache->k_dev, cache->v_dev, dim, c->sms, c->stream), "paged_attn launch") : FL_B200_OK;
 }
 
 } // extern "C"

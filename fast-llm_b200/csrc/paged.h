@@ -22,20 +22,25 @@ struct PagedAttnArgs {
     void *out;
     float2 *lse;                    // optional
     const int32_t *table, *q_start, *kv_len;
-    float *part;                    // records
+    float *part, *part_tm;          // records
     uint32_t *tickets;              // zero between launches
     uint32_t *status;
     uint64_t q_stride, out_stride;  // elements between tokens
     uint32_t n_seq, max_blocks, n_tokens, max_new, n_pages, page_shift;
     uint32_t n_kv, group, half;     // half: activations are f16
+    uint32_t few_rows;              // sequences of at most so many rows over a KV head are the first kernel's, the others the second's
     float scale;
 };
 
-// Few rows per sequence and KV head (mma.sync). kmap and vmap are filled in here.
+// Sequences of few rows over a KV head (mma.sync: attn_paged.cu) and of many (tcgen05: attn_paged_tm.cu). kmap and vmap are filled in there.
+constexpr uint32_t kFewRows = 16;
 cudaError_t paged_few_init(void);
 size_t paged_few_part_bytes(int sms);
 cudaError_t launch_paged_few(PagedAttnArgs a, const void *k, const void *v, uint32_t head_dim, int sms, cudaStream_t stream);
-constexpr uint32_t kPagedTickets = 1024;   // at least the CTAs of a launch
+cudaError_t paged_tm_init(void);
+size_t paged_tm_part_bytes(int sms);
+cudaError_t launch_paged_tm(PagedAttnArgs a, const void *k, const void *v, uint32_t head_dim, int sms, cudaStream_t stream);
+constexpr uint32_t kPagedTickets = 1024;   // at least twice the SMs
 
 #if defined(__CUDACC__)
 // One sequence of an attention call, checked: n = 0 where its lengths do not fit the call (reported by `report`).
