@@ -5,7 +5,7 @@
 // that a pair of row and key costs 8 D tensor flops instead of 4 D, and nothing else is rounded below 32 bits. f16
 // activations (Parts = 1): q as it is, the probabilities as one f16 (half a step of 2^-11, as the result).
 //
-// Bound by the tensor cores. Roles of a CTA (12 warps, one CTA per SM):
+// Bound by the tensor cores. Roles of a CTA (11 warps, one CTA per SM):
 //   softmax (2 x 4 warps): "lane" l = its 128 rows, thread = row: scores out of tensor memory, maximum, exponentials, probabilities
 //                          back over the scores' columns; at the end of a piece the contexts out
 //   copy    (1 warp)     : K and V tiles into a ring of slots, one TMA box per page (attn_paged.cu)
@@ -16,8 +16,9 @@
 // tiles; a smaller block gives both lanes its rows, every other tile each, and their results are added as two records.
 // Tiles of all blocks lie on one line (sequence, KV head, block, tile); shares, records and tickets as in attn_paged.cu.
 //
-// The tensor cores truncate their running sum, 1.3e-8 of it per instruction; with f32 activations O is therefore
-// brought out and added in f32 every kFlush tiles (128 instructions), into a buffer of the CTA's own that stays in L2.
+// The tensor cores truncate their running sum, 1.3e-8 of it per instruction; with f32 activations a part of 32 columns of O is therefore
+// brought out at every tile, in turn, added in f32 to a buffer of the CTA's own that stays in L2, and starts from zero: no sum in
+// tensor memory is longer than four tiles (64 instructions).
 #include "common.cuh"
 #include "paged.h"
 
@@ -27,10 +28,8 @@ namespace flb {
 
 namespace {
 
-constexpr uint32_t kRowsL = 128, kTile = 128, kFlush = 8;
-constexpr uint32_t kCopyWarp = 8, kTensorWarp = 9, kValueWarp = 10, kThreads = 12 * 32;   // (the last warp completes a warpgroup)
-// Registers: 168 a thread at launch; the softmax warps hold a row of 128 scores. 128 (208 + 208 + 88) = 384 x 168.
-constexpr uint32_t kRegsSoftmax = 208, kRegsOther = 88;
+constexpr uint32_t kRowsL = 128, kTile = 128;
+constexpr uint32_t kCopyWarp = 8, kTensorWarp = 9, kValueWarp = 10, kThreads = 11 * 32;
 constexpr float kShift = 6.f;   // probabilities are 2^(x - ref), ref = maximum - 6 when it is set and kept while they stay below 2^14
 constexpr uint32_t kOCol = 256, kTmemCols = 512;
 
@@ -42,11 +41,34 @@ template <int D, int Parts> struct Tm {
     static constexpr uint32_t kBytes = kHead + kQ + kSlots * kPart;
     static constexpr uint32_t kRecord = kRowsL * (D + 3);           // floats: [D / 4][128 rows][4], then references, sums, maxima
 };
+// A piece as the softmax warps use it, in shared memory (as registers its fields would cost a row of scores theirs).
+struct Job {
+    uint32_t valid, sm, n, t0;          // sm: small block; tiles t0 .. t0 + n - 1
+    uint32_t first, row0, rows, hkv;    // the sequence's first token; the block's rows row0 .. row0 + rows - 1
+    uint32_t whole, slot;               // the block is this CTA's alone; its record's
+    int32_t past;
+};
+struct Walk {
+    uint64_t pos, hi, seq_base;
+    uint32_t seq;
+    bool fresh;
+};
+struct Block { uint32_t rows, tiles; int32_t keys; };
+struct Piece {
+    PagedSeq q;
+    uint32_t seq, hkv, blk, n_blk;
+    Block b;
+    uint32_t t0, t1;
+    uint64_t base;       // unit of its block's tile 0
+};
 struct Head {
-    uint64_t full[8], empty[8], ready[8], s_full[2], p_full[2], o_done[2], q_full, drain;
-    uint64_t total, start_off, sum[kThreads / 32];
-    uint32_t start_seq, tmem, abort_flag, last[2], ticket;
-    uint32_t unfinite[3 * 128];
+    uint64_t full[8], empty[8], ready[8], s_full[2], p_full[2][2], o_done[2], q_full, drain;
+    uint64_t start_off;
+    uint32_t start_seq, tmem, abort_flag, any_unfinite;
+    Job job;
+    Walk walk;
+    Piece piece;
+    union { uint32_t unfinite[3 * 128]; uint64_t sum[kThreads / 32]; };   // (the sums while the share is found)
 };
 static_assert(sizeof(Head) <= 2048, "head");
 
@@ -127,8 +149,138 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+// two f32 at once
+struct F2 { uint64_t v; };
+__device__ __forceinline__ F2 pair(float a, float b) { F2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ void unpair(F2 x, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v)); }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) { F2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v)); return r; }
+__device__ __forceinline__ F2 add2(F2 a, F2 b) { F2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
+
+__device__ __forceinline__ void cut_at(float (&s)[32], int32_t valid) {   // columns behind `valid` are masked
+#pragma unroll
+    for (int c = 0; c < 32; ++c) s[c] = c <= valid ? s[c] : -INFINITY;
+}
+__device__ __forceinline__ float max_of(const float (&s)[32]) {
+    float t[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+    for (int c = 4; c < 32; c += 4)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) t[j] = fmaxf(t[j], s[c + j]);
+    return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+}
+// 32 scores to probabilities, in place in tensor memory (at): 2^(s f + m) as f16, hi parts in the first 16 columns and, with two parts,
+// lo parts in the others; sum += them. The hi part is the value cut off after 10 bits of mantissa, so that
+// the lo part needs no conversion back: both together keep 21 bits.
+template <int Parts> __device__ __forceinline__ void exp_chunk(const float (&s)[32], F2 f, F2 m, F2 (&sum)[2], uint32_t at) {
+    uint32_t ph[16], pl[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        float y0, y1;
+        unpair(fma2(pair(s[2 * j], s[2 * j + 1]), f, m), y0, y1);
+        const float e0 = exp2_fast(y0), e1 = exp2_fast(y1);
+        sum[j & 1] = add2(sum[j & 1], pair(e0, e1));
+        if (Parts == 2) {
+            const float h0 = __uint_as_float(__float_as_uint(e0) & 0xFFFFE000u), h1 = __uint_as_float(__float_as_uint(e1) & 0xFFFFE000u);
+            float l0, l1;
+            unpair(fma2(pair(h0, h1), pair(-1.f, -1.f), pair(e0, e1)), l0, l1);
+            ph[j] = half2_bits(h0, h1);
+            pl[j] = half2_bits(l0, l1);
+        } else {
+            ph[j] = half2_bits(e0, e1);
+        }
+    }
+    store16(at, ph);
+    if (Parts == 2) store16(at + 16, pl);
+}
+
+// The 32 rows of a warp from global memory, as f16 parts into shared memory (K-major, 128-byte swizzle), every row times a power of two that
+// brings its largest value to [2^11, 2^12): 8 lanes a row, 4 rows at a time. src: of the thread's own row; returns what its scores are to be
+// multiplied by (exponents of 2).
+template <int D, int Parts>
+__device__ __forceinline__ float load_q(const PagedAttnArgs &a, uint8_t *dst, uint64_t src, uint32_t row0, uint32_t rows, bool store) {
+    constexpr int V = 4, K = D / 32, kBatch = 4;   // values of a load, loads of a lane and row, groups of 4 rows in flight
+    const uint32_t lane = threadIdx.x & 31u, sub = lane & 7u, group = lane >> 3;
+    float f = 0.f;
+#pragma unroll 1
+    for (uint32_t i0 = 0; i0 < 8; i0 += kBatch) {
+        float x[kBatch][K][V];
+#pragma unroll
+        for (uint32_t i = 0; i < kBatch; ++i) {
+            const uint32_t rr = (i0 + i) + 8 * group;   // (rows 8 apart: their lines of shared memory are permuted alike, in banks of their own)
+            const uint64_t at = __shfl_sync(0xffffffffu, src, rr);
+            const bool there = row0 + rr < rows;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const uint32_t d = (8 * k + sub) * V;
+                if (Parts == 1) {
+                    const uint2 y = there ? __ldg(reinterpret_cast<const uint2 *>((const __half *)a.q + at + d)) : make_uint2(0u, 0u);
+                    const float2 y0 = __half22float2(*reinterpret_cast<const __half2 *>(&y.x)), y1 = __half22float2(*reinterpret_cast<const __half2 *>(&y.y));
+                    x[i][k][0] = y0.x; x[i][k][1] = y0.y; x[i][k][2] = y1.x; x[i][k][3] = y1.y;
+                } else {
+                    const float4 y = there ? __ldg(reinterpret_cast<const float4 *>((const float *)a.q + at + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    x[i][k][0] = y.x; x[i][k][1] = y.y; x[i][k][2] = y.z; x[i][k][3] = y.w;
+                }
+            }
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kBatch; ++i) {
+            const uint32_t rw = (i0 + i) + 8 * group, rr = row0 + rw;
+            float top = 0.f;
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int j = 0; j < V; ++j) top = fmaxf(top, fabsf(x[i][k][j]));
+#pragma unroll
+            for (int o = 4; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const int e = min(100, max(-100, 138 - (int)(__float_as_uint(top) >> 23)));
+            const float up = __uint_as_float((uint32_t)(e + 127) << 23);
+            const float mine = fmaxf(a.scale * 1.44269504088896341f * __uint_as_float((uint32_t)(127 - e) << 23), 1e-37f);
+            // thread t's row is t: group t / 8's at i = t % 8
+            const float got = __shfl_sync(0xffffffffu, mine, lane & 24u);
+            if ((lane & 7u) == i0 + i) f = got;
+            if (store) {
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    const uint32_t d = (8 * k + sub) * V;
+                    uint8_t *to = dst + (d >> 6) * (kRowsL * 128) + (rr >> 3) * 1024 + (rr & 7u) * 128 + (((((d & 63u) >> 3) ^ rr) & 7u) << 4) + (d & 7u) * 2;
+                    const float u0 = x[i][k][0] * up, u1 = x[i][k][1] * up, u2 = x[i][k][2] * up, u3 = x[i][k][3] * up;
+                    const __half2 h0 = __floats2half2_rn(u0, u1), h1 = __floats2half2_rn(u2, u3);
+                    *reinterpret_cast<uint2 *>(to) = make_uint2(*reinterpret_cast<const uint32_t *>(&h0), *reinterpret_cast<const uint32_t *>(&h1));
+                    if (Parts == 2) {
+                        const float2 b0 = __half22float2(h0), b1 = __half22float2(h1);
+                        *reinterpret_cast<uint2 *>(to + Tm<D, Parts>::kPart) = make_uint2(half2_bits(u0 - b0.x, u1 - b0.y), half2_bits(u2 - b1.x, u3 - b1.y));
+                    }
+                }
+            }
+        }
+    }
+    return f;
+}
+
+// Rows of results through shared memory, so that a warp stores whole rows: 16-byte pieces of row r at (piece ^ r).
+template <int D, int Parts> __device__ __forceinline__ void stage_put(uint8_t *stage, uint32_t r, uint32_t c, const float4 &v) {   // values 4 c ..
+    if (Parts == 2) *reinterpret_cast<float4 *>(stage + r * (D * 4) + ((c ^ (r & (D / 4 - 1))) << 4)) = v;
+    else *reinterpret_cast<uint2 *>(stage + r * (D * 2) + (((c >> 1) ^ (r & (D / 8 - 1))) << 4) + (c & 1u) * 8) = make_uint2(half2_bits(v.x, v.y), half2_bits(v.z, v.w));
+}
+template <int D, int Parts> __device__ __forceinline__ void stage_out(const uint8_t *stage, void *out, uint32_t row0, uint32_t rows, uint64_t dst) {   // a warp's 32 rows
+    constexpr uint32_t kRowBytes = D * 2 * Parts, kLanes = kRowBytes / 16;   // lanes of a row
+    const uint32_t lane = threadIdx.x & 31u, c = lane % kLanes;
+    __syncwarp();
+#pragma unroll 4
+    for (uint32_t i = lane / kLanes; i < 32; i += 32 / kLanes) {
+        const uint64_t at = __shfl_sync(0xffffffffu, dst, i);
+        const uint32_t r = row0 + i;
+        if (r < rows) *reinterpret_cast<uint4 *>(static_cast<uint8_t *>(out) + at * (2 * Parts) + c * 16) = *reinterpret_cast<const uint4 *>(stage + r * kRowBytes + ((c ^ (r & (kLanes - 1))) << 4));
+    }
+    __syncwarp();
+}
+
+// (max score, sum of exp(score - max)) of a row from its largest exponent - kShift and the sum relative to 2^from
+__device__ __forceinline__ float2 lse_of(float highest, float from, float sum) {
+    return highest == -INFINITY ? make_float2(highest, sum) : make_float2((highest + kShift) * 0.693147180559945309f, sum * exp2_fast(from - highest - kShift));
+}
+
 // ---- blocks, shares, pieces --------------------------------------------------------------------------------------------
-struct Block { uint32_t rows, tiles; int32_t keys; };
 __device__ __forceinline__ Block block_of(const PagedAttnArgs &a, const PagedSeq &q, uint32_t blk) {
     Block b;
     b.rows = min(2 * kRowsL, q.n * a.group - blk * 2 * kRowsL);
@@ -162,18 +314,6 @@ __device__ __forceinline__ uint64_t head_units(const PagedAttnArgs &a, const Pag
     return u;
 }
 
-struct Piece {
-    PagedSeq q;
-    uint32_t seq, hkv, blk, n_blk;
-    Block b;
-    uint32_t t0, t1;
-    uint64_t base;       // unit of its block's tile 0
-};
-struct Walk {
-    uint64_t pos, hi, seq_base;
-    uint32_t seq;
-    bool fresh;
-};
 // The next piece of a CTA's share, for a whole warp.
 __device__ __forceinline__ bool next_piece(const PagedAttnArgs &a, Walk &w, Piece &p) {
     if (w.pos >= w.hi) return false;
@@ -250,15 +390,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
     if (tid == 0) {
         for (uint32_t s = 0; s < T::kSlots; ++s) { mbar_init(&hd.full[s], 1); mbar_init(&hd.empty[s], 1); mbar_init(&hd.ready[s], 1); }
-        for (int l = 0; l < 2; ++l) { mbar_init(&hd.s_full[l], 1); mbar_init(&hd.p_full[l], 4); mbar_init(&hd.o_done[l], 1); }
+        for (int l = 0; l < 2; ++l) { mbar_init(&hd.s_full[l], 1); mbar_init(&hd.p_full[l][0], 4); mbar_init(&hd.p_full[l][1], 4); mbar_init(&hd.o_done[l], 1); }
         mbar_init(&hd.q_full, 8);
         mbar_init(&hd.drain, 1);
         hd.abort_flag = 0;
-        hd.ticket = 0;
+        hd.any_unfinite = 0;
         fence_barrier_init();
     }
-    for (uint32_t i = tid; i < 3 * D; i += kThreads) hd.unfinite[i] = 0x7fffffffu;
     griddep_wait();
+    if (tid == 0) a.blocks[blockIdx.x].records = 0;
 
     // ---- this CTA's share of the line ----
     uint64_t total = 0;
@@ -302,6 +442,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
             if (lo >= x && lo < x + u) { hd.start_seq = s0 + tid; hd.start_off = x; }
         }
     }
+    __syncthreads();
+    for (uint32_t i = tid; i < 3 * D; i += kThreads) hd.unfinite[i] = 0x7fffffffu;
     if (warp == kTensorWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&hd.tmem)), "r"(kTmemCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -320,8 +462,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
     uint32_t done = 0;      // copies of the pieces in front
     uint32_t pieces_in = 0; // pieces begun
 
-    if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
-    else asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
     if (warp == kCopyWarp) {
         // ---- copies ----
         const uint32_t box = min(1u << a.page_shift, kTile), boxes = kTile / box, bytes = box * D * 2;
@@ -372,31 +512,32 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
         constexpr uint32_t kIdS = idesc_of(kTile, false), kIdO = idesc_of(D, true), kGroup = D * 16;
         uint32_t pv[2] = {0, 0};   // PV products of a lane so far
         auto ring_wait = [&](uint32_t i) { return wait(&hd.full[(done + i) % T::kSlots], ((done + i) / T::kSlots) & 1u); };
+        auto uniform = [](uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); };
         auto scores = [&](uint32_t l, uint32_t ql, uint32_t i) {   // of lane l, q of lane ql, K in copy i
-            const uint32_t d = tmem + l * kTile, qa = smem_u32(q_s) + ql * Parts * T::kPart, ka = smem_u32(ring) + ((done + i) % T::kSlots) * T::kPart;
+            const uint32_t d = uniform(tmem + l * kTile), qa = uniform(smem_u32(q_s) + ql * Parts * T::kPart), ka = uniform(smem_u32(ring) + ((done + i) % T::kSlots) * T::kPart);
             if (elect_one()) {
 #pragma unroll
                 for (int part = Parts - 1; part >= 0; --part)
 #pragma unroll
                     for (int kb = 0; kb < D / 16; ++kb)
-                        mma_ss(d, desc(qa + part * T::kPart + (kb >> 2) * (kRowsL * 128) + (kb & 3) * 32, 0, 1024), desc(ka + (kb >> 2) * 1024 + (kb & 3) * 32, 0, kGroup), kIdS,
+                        mma_ss(d, desc(qa, 0, 1024) + ((part * T::kPart + (kb >> 2) * (kRowsL * 128) + (kb & 3) * 32) >> 4), desc(ka, 0, kGroup) + (((kb >> 2) * 1024 + (kb & 3) * 32) >> 4), kIdS,
                                part != Parts - 1 || kb != 0);
                 commit(&hd.s_full[l]);
             }
             __syncwarp();
         };
-        auto context = [&](uint32_t l, uint32_t i, bool from_zero) {   // O += P V, V in copy i
-            const uint32_t d = tmem + kOCol + l * 128, pa = tmem + l * kTile, va = smem_u32(ring) + ((done + i) % T::kSlots) * T::kPart;
+        // O += P V for keys 64 .. 127 (first), then 0 .. 63 of the tile, V in copy i
+        auto context = [&](uint32_t l, uint32_t i, uint32_t half, bool from_zero) {
+            const uint32_t d = uniform(tmem + kOCol + l * 128), pa = uniform(tmem + l * kTile + half * 64), va = uniform(smem_u32(ring) + ((done + i) % T::kSlots) * T::kPart + half * 8 * kGroup);
             if (elect_one()) {
 #pragma unroll
                 for (int part = Parts - 1; part >= 0; --part)
 #pragma unroll
-                    for (int kk = 0; kk < (int)kTile / 16; ++kk)
-                        mma_ts(d, pa + part * 64 + kk * 8, desc(va + kk * 2 * kGroup, 1024, kGroup), kIdO, !from_zero || part != Parts - 1 || kk != 0);
-                commit(&hd.o_done[l]);
+                    for (int kk = 0; kk < (int)kTile / 32; ++kk)
+                        mma_ts(d, pa + (kk >> 1) * 32 + part * 16 + (kk & 1) * 8, desc(va, 1024, kGroup) + ((kk * 2 * kGroup) >> 4), kIdO, !from_zero || part != Parts - 1 || kk != 0);
+                if (!half) commit(&hd.o_done[l]);
             }
             __syncwarp();
-            ++pv[l];
         };
         auto ready = [&](uint32_t i) { return wait(&hd.ready[(done + i) % T::kSlots], ((done + i) / T::kSlots) & 1u); };
         auto release = [&](uint32_t i) {
@@ -427,9 +568,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
                     if (t >= n) break;
                     const uint32_t vi = v_index(sm, t, n), ki = k_index(sm, next);
                     if (!ring_wait(vi) || !ready(vi)) break;
-                    if (!wait(&hd.p_full[l], pv[l] & 1u)) break;
+                    if (!wait(&hd.p_full[l][1], pv[l] & 1u)) break;
                     fence_after();
-                    context(l, vi, step == 0 || (Parts == 2 && step % kFlush == 0));
+                    context(l, vi, 1, step == 0);
+                    if (!wait(&hd.p_full[l][0], pv[l] & 1u)) break;
+                    fence_after();
+                    context(l, vi, 0, false);
+                    ++pv[l];
                     if (sm || l == 1) release(vi);
                     if (next < n) {
                         // (the next scores overwrite the probabilities)
@@ -476,6 +621,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
                         const uint4 w = *at;
                         const uint32_t z = ((w.x & 0x7C007C00u) + 0x04000400u) | ((w.y & 0x7C007C00u) + 0x04000400u) | ((w.z & 0x7C007C00u) + 0x04000400u) | ((w.w & 0x7C007C00u) + 0x04000400u);
                         if (z & 0x80008000u) {   // an exponent of all ones
+                            hd.any_unfinite = 1u;
                             __half *h = reinterpret_cast<__half *>(at);
                             for (uint32_t e = 0; e < 8; ++e) {
                                 const uint16_t b = __half_as_ushort(h[e]);
@@ -493,7 +639,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
             }
             done += 2 * n;
         }
-    } else if (warp < 8) {
+    } else {
         // ---- softmax: lane l, thread = row ----
         const uint32_t l = warp >> 2, w4 = warp & 3u, r = tid & 127u;
         const uint32_t ts = tmem + (w4 * 32u << 16) + l * kTile, to = tmem + (w4 * 32u << 16) + kOCol + l * 128;
@@ -502,263 +648,250 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
             else asm volatile("bar.sync 2, 128;" ::: "memory");
         };
         auto bar_both = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
-        float *acc_mem = a.part_tm + ((uint64_t)gridDim.x * 4 + blockIdx.x * 2 + l) * T::kRecord;   // this lane's sums (see kFlush)
+        float4 *acc_mem = reinterpret_cast<float4 *>(a.part_tm + ((uint64_t)gridDim.x * 4 + blockIdx.x * 2 + l) * T::kRecord) + r;   // this row's sums
+        auto part_of = [](const float (&x)[4], uint32_t c) { return c == 0 ? x[0] : c == 1 ? x[1] : c == 2 ? x[2] : x[3]; };
         uint32_t s_seen = 0;
-        bool first = true;
-        while (next_piece(a, walk, p)) {
-            const bool sm = small(p);
-            const uint32_t n = p.t1 - p.t0, row0 = p.blk * 2 * kRowsL + (sm ? 0 : l * kRowsL), rows = min(kRowsL, sm ? p.b.rows : p.b.rows - min(p.b.rows, l * kRowsL));
-            // q as f16 parts into shared memory, every row times a power of two that brings its largest value to [2^11, 2^12)
-            float f = 0.f;
-            if (!dead) {
-                uint8_t *qd = q_s + (sm ? 0 : l) * Parts * T::kPart;
-                constexpr int V = D / 32;   // values of a thread
-#pragma unroll 4
-                for (uint32_t i = 0; i < 32; ++i) {
-                    const uint32_t rr = w4 * 32 + i, at = row0 + rr, tok = at / a.group, head = p.hkv * a.group + at - tok * a.group;
-                    float x[V];
-#pragma unroll
-                    for (int j = 0; j < V; ++j) x[j] = 0.f;
-                    if (rr < rows) {
-                        const uint64_t src = (p.q.first + tok) * a.q_stride + (uint64_t)head * D + lane * V;
-                        if (a.half) {
-#pragma unroll
-                            for (int j = 0; j < V; j += 2) {
-                                const float2 y = __half22float2(*reinterpret_cast<const __half2 *>((const __half *)a.q + src + j));
-                                x[j] = y.x; x[j + 1] = y.y;
-                            }
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < V; j += 2) {
-                                const float2 y = *reinterpret_cast<const float2 *>((const float *)a.q + src + j);
-                                x[j] = y.x; x[j + 1] = y.y;
-                            }
-                        }
-                    }
-                    float top = 0.f;
-#pragma unroll
-                    for (int j = 0; j < V; ++j) top = fmaxf(top, fabsf(x[j]));
-                    top = warp_max(top);
-                    const int e = min(100, max(-100, 138 - (int)(__float_as_uint(top) >> 23)));
-                    const float up = __uint_as_float((uint32_t)(e + 127) << 23);
-                    if (lane == i) f = fmaxf(a.scale * 1.44269504088896341f * __uint_as_float((uint32_t)(127 - e) << 23), 1e-37f);
-                    if (!sm || l == 0) {
-                        const uint32_t d0 = lane * V;
-                        uint8_t *dst = qd + (d0 >> 6) * (kRowsL * 128) + (rr >> 3) * 1024 + (rr & 7u) * 128 + (((((d0 & 63u) >> 3) ^ rr) & 7u) << 4) + (d0 & 7u) * 2;
-#pragma unroll
-                        for (int j = 0; j < V; j += 2) {
-                            const float u0 = x[j] * up, u1 = x[j + 1] * up;
-                            const __half2 h = __floats2half2_rn(u0, u1);
-                            *reinterpret_cast<__half2 *>(dst + 2 * j) = h;
-                            if (Parts == 2) {
-                                const float2 b = __half22float2(h);
-                                *reinterpret_cast<uint32_t *>(dst + T::kPart + 2 * j) = half2_bits(u0 - b.x, u1 - b.y);
-                            }
-                        }
+        if (warp == 0) { hd.walk = walk; hd.job.slot = 2; }   // (2: none yet)
+        for (;;) {
+            if (warp == 0) {
+                Walk w = hd.walk;
+                Piece x = hd.piece;
+                const bool valid = next_piece(a, w, x);
+                __syncwarp();
+                if (lane == 0) {
+                    hd.walk = w;
+                    hd.piece = x;
+                    Job &j = hd.job;
+                    j.valid = valid;
+                    if (valid) {
+                        const uint32_t c0 = owner_of(total, ctas, x.base), c1 = owner_of(total, ctas, x.base + x.b.tiles - 1);
+                        j.sm = small(x); j.n = x.t1 - x.t0; j.t0 = x.t0;
+                        j.first = x.q.first; j.row0 = x.blk * 2 * kRowsL; j.rows = x.b.rows; j.hkv = x.hkv; j.past = x.q.past;
+                        j.whole = c0 == c1;
+                        j.slot = j.slot == 2 ? 0 : 1;
+                        if (!j.whole && c0 == blockIdx.x) a.blocks[c0] = PagedTmBlock{c1 - c0 + 1, j.sm, j.slot, j.first, j.row0, j.rows, j.hkv, j.past};
                     }
                 }
             }
+            bar_both();
+            const Job &job = hd.job;
+            if (!job.valid) break;
+            const bool sm = job.sm;
+            const uint32_t t0 = job.t0, row0 = job.row0 + (sm ? 0 : l * kRowsL), rows = min(kRowsL, sm ? job.rows : job.rows - min(job.rows, l * kRowsL));
+            const uint32_t steps = sm ? (job.n + 1 - l) / 2 : job.n;
+            const uint32_t tok = (row0 + r) / a.group, head = job.hkv * a.group + (row0 + r) - tok * a.group;
+            const bool there = r < rows, active = w4 * 32 < rows;
+            const int32_t lim = there ? job.past + (int32_t)tok : 0x7fffffff;   // (what a row that is not there comes to stays in it)
+            float f = 0.f;
+            if (!dead && active) f = load_q<D, Parts>(a, q_s + (sm ? 0 : l) * Parts * T::kPart, (job.first + tok) * a.q_stride + (uint64_t)head * D, w4 * 32, rows, !sm || l == 0);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) arrive(&hd.q_full);
 
-            const uint32_t tok = (row0 + r) / a.group, head = p.hkv * a.group + (row0 + r) - tok * a.group;
-            const bool there = r < rows;
-            const int32_t lim = there ? p.q.past + (int32_t)tok : 0x7fffffff;   // (what a row that is not there comes to stays in it)
-            const bool active = w4 * 32 < rows;
-            const uint32_t steps = sm ? (n + 1 - l) / 2 : n;
-            float ref = -INFINITY, sum = 0.f, acc_ref = -INFINITY, highest = -INFINITY;
+            float ref = -INFINITY, sum = 0.f, highest = -INFINITY;
+            float acc_ref[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};   // references of the sums in memory, per 32 columns
+            uint32_t out_of = 0;                                               // bit c: columns 32 c .. have a sum in memory
             for (uint32_t step = 0; step < steps; ++step) {
-                const int32_t k0 = (int32_t)((p.t0 + (sm ? 2 * step + l : step)) * kTile);
+                const int32_t k0 = (int32_t)((t0 + (sm ? 2 * step + l : step)) * kTile);
+                const uint32_t c4 = step & 3u;   // the columns of O that go out at this step
+                const bool goes = Parts == 2 && active && step && c4 < D / 32, adds = goes && (out_of >> c4 & 1u);
+                if (goes) {
+                    // a part of O to its sum in memory, while the tensor cores form the scores
+                    float4 old[8];
+                    if (adds)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) old[j] = __ldcg(acc_mem + (8 * c4 + j) * kRowsL);
+                    if (!wait(&hd.o_done[l], (s_seen - 1) & 1u)) break;
+                    fence_after();
+                    const float before = part_of(acc_ref, c4), keep = before == -INFINITY ? 0.f : exp2_fast(before - ref);
+                    float o[32];
+                    load32(to + 32 * c4, o);
+                    wait_ld(o);
+                    if (adds)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            o[4 * j] = fmaf(old[j].x, keep, o[4 * j]); o[4 * j + 1] = fmaf(old[j].y, keep, o[4 * j + 1]);
+                            o[4 * j + 2] = fmaf(old[j].z, keep, o[4 * j + 2]); o[4 * j + 3] = fmaf(old[j].w, keep, o[4 * j + 3]);
+                        }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) __stcg(acc_mem + (8 * c4 + j) * kRowsL, make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]));
+                    const uint32_t zero[16] = {};
+                    store16(to + 32 * c4, zero);
+                    store16(to + 32 * c4 + 16, zero);
+                    out_of |= 1u << c4;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) acc_ref[c] = c4 == (uint32_t)c ? ref : acc_ref[c];
+                }
                 if (!wait(&hd.s_full[l], s_seen & 1u)) break;
                 ++s_seen;
                 if (!active) {
-                    if (lane == 0) arrive(&hd.p_full[l]);
+                    __syncwarp();
+                    if (lane == 0) { arrive(&hd.p_full[l][1]); arrive(&hd.p_full[l][0]); }
                     continue;
                 }
                 fence_after();
-                float s[128];
+                // The scores come once for the maximum; their last 64 columns stay for the exponentials, the others come again.
+                const int32_t valid = lim - k0;   // columns 0 .. valid
+                const bool cut = __any_sync(0xffffffffu, valid < (int32_t)kTile - 1);
+                float top = -INFINITY, sa[32], sb[32];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) load32(ts + 32 * c, s + 32 * c);
-                wait_ld(s);
-                if (__any_sync(0xffffffffu, k0 + 127 > lim)) {
-                    const int32_t valid = lim - k0;
-#pragma unroll
-                    for (int c = 0; c < 128; ++c) s[c] = c <= valid ? s[c] : -INFINITY;
+                for (int h = 0; h < 2; ++h) {
+                    load32(ts + 64 * h, sa);
+                    load32(ts + 64 * h + 32, sb);
+                    wait_ld(sa);
+                    wait_ld(sb);
+                    if (cut) {
+                        cut_at(sa, valid - 64 * h);
+                        cut_at(sb, valid - 64 * h - 32);
+                    }
+                    top = fmaxf(top, fmaxf(max_of(sa), max_of(sb)));
                 }
-                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int c = 0; c < 128; c += 8)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) top[j] = fmaxf(top[j], fmaxf(s[c + j], s[c + 4 + j]));
-                const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * f - kShift;   // -inf: no key
+                const float mx = top * f - kShift;   // -inf: no key
                 highest = fmaxf(highest, mx);
-                const bool from_zero = step == 0 || (Parts == 2 && step % kFlush == 0);
-                if (Parts == 2 && step && from_zero) {
-                    // O of the last kFlush tiles to the sums in memory (the product that completed it precedes these scores)
-                    const float keep = acc_ref == -INFINITY ? 0.f : exp2_fast(acc_ref - ref);
+                float rescale = 1.f;
+                if (mx > ref + (step ? 8.f : 0.f)) {   // (-inf + 8 = -inf: the first key of a row sets its reference)
+                    const float al = ref == -INFINITY ? 1.f : exp2_fast(ref - mx);
+                    ref = mx;
+                    sum *= al;
+                    rescale = al;
+                }
+                if (step && __any_sync(0xffffffffu, rescale != 1.f)) {
 #pragma unroll 1
                     for (int c = 0; c < D; c += 32) {
                         float o[32];
                         load32(to + c, o);
-                        float4 *at = reinterpret_cast<float4 *>(acc_mem) + (c / 4) * kRowsL + r;
-                        if (step > kFlush) {
-                            float4 old[8];
+                        wait_ld(o);
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) old[j] = at[j * kRowsL];
-                            wait_ld(o);
+                        for (int h = 0; h < 2; ++h) {
+                            uint32_t w[16];
 #pragma unroll
-                            for (int j = 0; j < 8; ++j)
-                                at[j * kRowsL] = make_float4(fmaf(old[j].x, keep, o[4 * j]), fmaf(old[j].y, keep, o[4 * j + 1]), fmaf(old[j].z, keep, o[4 * j + 2]), fmaf(old[j].w, keep, o[4 * j + 3]));
-                        } else {
-                            wait_ld(o);
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) at[j * kRowsL] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-                        }
-                    }
-                    acc_ref = ref;
-                }
-                {
-                    const float was = ref;
-                    if (from_zero ? mx > ref : mx > ref + 8.f) ref = mx;   // (from zero: nothing in O to bring along)
-                    const float al = was == -INFINITY || ref == was ? 1.f : exp2_fast(was - ref);
-                    sum *= al;
-                    if (!from_zero && __any_sync(0xffffffffu, al != 1.f)) {
-#pragma unroll 1
-                        for (int c = 0; c < D; c += 32) {
-                            float o[32];
-                            load32(to + c, o);
-                            wait_ld(o);
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                uint32_t w[16];
-#pragma unroll
-                                for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(o[16 * h + j] * al);
-                                store16(to + c + 16 * h, w);
-                            }
+                            for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(o[16 * h + j] * rescale);
+                            store16(to + c + 16 * h, w);
                         }
                     }
                 }
                 const float m = ref == -INFINITY ? 0.f : ref;
-                float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t ph[16], pl[16];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const float e0 = exp2_fast(fmaf(s[32 * c + 2 * j], f, -m)), e1 = exp2_fast(fmaf(s[32 * c + 2 * j + 1], f, -m));
-                        part[j & 1] += e0;
-                        part[2 + (j & 1)] += e1;
-                        const __half2 h = __floats2half2_rn(e0, e1);
-                        ph[j] = *reinterpret_cast<const uint32_t *>(&h);
-                        if (Parts == 2) {
-                            const float2 b = __half22float2(h);
-                            pl[j] = half2_bits(e0 - b.x, e1 - b.y);
-                        }
-                    }
-                    store16(ts + 16 * c, ph);
-                    if (Parts == 2) store16(ts + 64 + 16 * c, pl);
-                }
-                sum += (part[0] + part[1]) + (part[2] + part[3]);
+                const F2 f2 = pair(f, f), m2 = pair(-m, -m);
+                F2 part[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+                exp_chunk<Parts>(sa, f2, m2, part, ts + 64);
+                load32(ts, sa);
+                exp_chunk<Parts>(sb, f2, m2, part, ts + 96);
                 wait_st();
                 fence_before();
                 __syncwarp();
-                if (lane == 0) arrive(&hd.p_full[l]);
+                if (lane == 0) arrive(&hd.p_full[l][1]);
+                wait_ld(sa);
+                load32(ts + 32, sb);
+                if (cut) cut_at(sa, valid);
+                exp_chunk<Parts>(sa, f2, m2, part, ts);
+                wait_ld(sb);
+                if (cut) cut_at(sb, valid - 32);
+                exp_chunk<Parts>(sb, f2, m2, part, ts + 32);
+                float p0, p1, p2, p3;
+                unpair(part[0], p0, p1);
+                unpair(part[1], p2, p3);
+                sum += (p0 + p1) + (p2 + p3);
+                wait_st();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) arrive(&hd.p_full[l][0]);
             }
 
             // ---- the piece's results: the rows themselves, or a record ----
-            const uint32_t c0 = owner_of(total, ctas, p.base), c1 = owner_of(total, ctas, p.base + p.b.tiles - 1), records = (c1 - c0 + 1) * (sm ? 2 : 1);
-            const bool whole = records == 1;
-            float *rec = a.part_tm + (uint64_t)((blockIdx.x * 2 + (first ? 0 : 1)) * 2 + l) * T::kRecord;
-            first = false;
-            if (steps && !dead) {
+            if (steps) {
                 // (every PV product of a lane follows one of its scores: as many of both)
                 wait(&hd.o_done[l], (s_seen - 1) & 1u);
                 fence_after();
             }
-            auto put = [&](uint64_t to_out, const float4 &v) {
-                if (a.half) *reinterpret_cast<uint2 *>((__half *)a.out + to_out) = make_uint2(half2_bits(v.x, v.y), half2_bits(v.z, v.w));
-                else *reinterpret_cast<float4 *>((float *)a.out + to_out) = v;
-            };
-            const uint64_t dst = (p.q.first + tok) * a.out_stride + (uint64_t)head * D;
-            auto put_lse = [&](float mx, float from, float to_sum) {
-                a.lse[(uint64_t)(p.q.first + tok) * a.n_kv * a.group + head] =
-                    mx == -INFINITY ? make_float2(mx, to_sum) : make_float2((mx + kShift) * 0.693147180559945309f, to_sum * exp2_fast(from - mx - kShift));
-            };
-            if (steps && !dead && active) {
-                const float keep = acc_ref == -INFINITY ? 0.f : exp2_fast(acc_ref - ref), inv = lim < 0 ? 0.f : 1.f / sum;
-                const bool acc = Parts == 2 && steps > kFlush;
-#pragma unroll 1
-                for (int c = 0; c < D; c += 32) {
-                    float o[32];
-                    load32(to + c, o);
-                    wait_ld(o);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        float4 v = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-                        if (acc) {
-                            const float4 old = reinterpret_cast<const float4 *>(acc_mem)[(c / 4 + j) * kRowsL + r];
-                            v.x = fmaf(old.x, keep, v.x); v.y = fmaf(old.y, keep, v.y); v.z = fmaf(old.z, keep, v.z); v.w = fmaf(old.w, keep, v.w);
-                        }
-                        const uint32_t d = c + 4 * j;
-                        v.x += unfinite_at(hd.unfinite, D, d, lim); v.y += unfinite_at(hd.unfinite, D, d + 1, lim);
-                        v.z += unfinite_at(hd.unfinite, D, d + 2, lim); v.w += unfinite_at(hd.unfinite, D, d + 3, lim);
-                        if (!whole) __stcg(reinterpret_cast<float4 *>(rec) + (c / 4 + j) * kRowsL + r, v);
-                        else if (there) put(dst + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
-                    }
+            // A small block: the second lane hands its sums to the first, in tensor memory, where its scores were
+            float ref2 = -INFINITY, sum2 = 0.f, acc2_ref[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            uint32_t out2 = 0;
+            if (sm) {
+                if (l && active) {
+                    const uint32_t w[16] = {__float_as_uint(ref), __float_as_uint(sum), __float_as_uint(highest), out_of, __float_as_uint(acc_ref[0]), __float_as_uint(acc_ref[1]),
+                                            __float_as_uint(acc_ref[2]), __float_as_uint(acc_ref[3])};
+                    store16(ts, w);
+                    wait_st();
                 }
-                if (whole && there && a.lse) put_lse(highest, ref, sum);
-            }
-            if (!whole) {
-                __stcg(rec + D * kRowsL + r, steps ? ref : -INFINITY);
-                __stcg(rec + (D + 1) * kRowsL + r, steps ? sum : 0.f);
-                __stcg(rec + (D + 2) * kRowsL + r, steps ? highest : -INFINITY);
-                __threadfence();
-                bar_lane();
-                // (a small block that is this CTA's alone has a ticket of its own: the other may already count the CTA's last block)
-                uint32_t *ticket = c0 == c1 ? &hd.ticket : &a.tickets[2 * c0 + (sm ? 0 : l)];
-                if (r == 0) hd.last[l] = !dead && atomicAdd(ticket, 1u) == records - 1 ? 1u : 0u;
-                bar_lane();
-                if (hd.last[l] && there) {
-                    __threadfence();
-                    const bool c0_first = p.base <= share_of(total, ctas, c0);
-                    auto record = [&](uint32_t i) -> const float * {   // in order of CTA, then lane
-                        const uint32_t ci = sm ? i >> 1 : i, li = sm ? i & 1u : l;
-                        return a.part_tm + (uint64_t)(((c0 + ci) * 2 + (ci || c0_first ? 0 : 1)) * 2 + li) * T::kRecord;
-                    };
-                    float mr = -INFINITY, ms = 0.f, top = -INFINITY;
-                    for (uint32_t i = 0; i < records; ++i) mr = fmaxf(mr, __ldcg(record(i) + D * kRowsL + r));
-                    for (uint32_t i = 0; i < records; ++i) {
-                        const float m = __ldcg(record(i) + D * kRowsL + r);
-                        top = fmaxf(top, __ldcg(record(i) + (D + 2) * kRowsL + r));
-                        if (m != -INFINITY) ms = fmaf(__ldcg(record(i) + (D + 1) * kRowsL + r), exp2_fast(m - mr), ms);
-                    }
-                    const float inv = lim < 0 ? 0.f : 1.f / ms;
-                    for (int c = 0; c < D / 4; c += 8) {
-                        float4 v[8];
+                fence_before();
+                bar_both();
+                fence_after();
+                if (!l && active && job.n > 1) {
+                    float w[32];
+                    load32(ts + kTile, w);
+                    wait_ld(w);
+                    ref2 = w[0]; sum2 = w[1]; highest = fmaxf(highest, w[2]); out2 = __float_as_uint(w[3]);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-                        for (uint32_t i = 0; i < records; ++i) {
-                            const float m = __ldcg(record(i) + D * kRowsL + r);
-                            if (m == -INFINITY) continue;
-                            const float w = exp2_fast(m - mr);
+                    for (int c = 0; c < 4; ++c) acc2_ref[c] = w[4 + c];
+                }
+            }
+            if (steps && !dead && active && !(sm && l)) {
+                const bool whole = job.whole, two = sm && job.n > 1;
+                const float both = fmaxf(ref, ref2), w1 = ref == -INFINITY ? 0.f : exp2_fast(ref - both), w2 = ref2 == -INFINITY ? 0.f : exp2_fast(ref2 - both);
+                const float all = fmaf(sum, w1, sum2 * w2), inv = lim < 0 ? 0.f : 1.f / all;
+                float *rec = a.part_tm + (uint64_t)((blockIdx.x * 2 + job.slot) * 2 + l) * T::kRecord;
+                // Rows go out through shared memory, where the lane's q was (a small block's lanes share the first q; the second is free).
+                uint8_t *stage = q_s + (sm ? 1 : l) * Parts * T::kPart;
+                const bool any_unfinite = hd.any_unfinite != 0;
+#pragma unroll 1
+                for (int c = 0; c < D / 32; ++c) {
+                    float o[32];
+                    auto lane_part = [&](uint32_t from, const float4 *mem, uint32_t out, float before, float rf) {   // 32 columns of a lane's contexts
+                        load32(from + 32 * c, o);
+                        const bool acc = Parts == 2 && (out >> c & 1u);
+                        float4 old[8];
+                        if (acc)
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) old[j] = __ldcg(mem + (8 * c + j) * kRowsL);
+                        wait_ld(o);
+                        if (acc) {
+                            const float keep = before == -INFINITY ? 0.f : exp2_fast(before - rf);
 #pragma unroll
                             for (int j = 0; j < 8; ++j) {
-                                const float4 u = __ldcg(reinterpret_cast<const float4 *>(record(i)) + (c + j) * kRowsL + r);
-                                v[j].x = fmaf(u.x, w, v[j].x); v[j].y = fmaf(u.y, w, v[j].y); v[j].z = fmaf(u.z, w, v[j].z); v[j].w = fmaf(u.w, w, v[j].w);
+                                o[4 * j] = fmaf(old[j].x, keep, o[4 * j]); o[4 * j + 1] = fmaf(old[j].y, keep, o[4 * j + 1]);
+                                o[4 * j + 2] = fmaf(old[j].z, keep, o[4 * j + 2]); o[4 * j + 3] = fmaf(old[j].w, keep, o[4 * j + 3]);
                             }
                         }
+                    };
+                    float v[32];
+                    if (two) {
+                        lane_part(to + 128, acc_mem + T::kRecord / 4, out2, part_of(acc2_ref, c), ref2);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) put(dst + 4 * (c + j), make_float4(v[j].x * inv, v[j].y * inv, v[j].z * inv, v[j].w * inv));
+                        for (int j = 0; j < 32; ++j) v[j] = o[j] * w2;
                     }
-                    if (a.lse) put_lse(top, mr, ms);
+                    lane_part(to, acc_mem, out_of, part_of(acc_ref, c), ref);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = two ? fmaf(o[j], w1, v[j]) : o[j];
+                    if (any_unfinite)
+#pragma unroll 1
+                        for (int j = 0; j < 32; ++j) {
+                            const float u = unfinite_at(hd.unfinite, D, 32 * c + j, lim);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) v[i] += i == j ? u : 0.f;
+                        }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        if (!whole) __stcg(reinterpret_cast<float4 *>(rec) + (8 * c + j) * kRowsL + r, make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+                        else stage_put<D, Parts>(stage, r, 8 * c + j, make_float4(v[4 * j] * inv, v[4 * j + 1] * inv, v[4 * j + 2] * inv, v[4 * j + 3] * inv));
+                    }
                 }
-                if (r == 0 && hd.last[l]) *ticket = 0;
+                const float from = two ? both : ref, total_sum = two ? all : sum;
+                if (whole) {
+                    stage_out<D, Parts>(stage, a.out, w4 * 32, rows, (job.first + tok) * a.out_stride + (uint64_t)head * D);
+                    if (there && a.lse) a.lse[(uint64_t)(job.first + tok) * a.n_kv * a.group + head] = lse_of(highest, from, total_sum);
+                } else {
+                    __stcg(rec + D * kRowsL + r, from);
+                    __stcg(rec + (D + 1) * kRowsL + r, total_sum);
+                    __stcg(rec + (D + 2) * kRowsL + r, highest);
+                }
             }
             fence_before();
             bar_both();   // both lanes are done with q, O and the notes
-            for (uint32_t i = tid; i < 3 * D; i += 256) hd.unfinite[i] = 0x7fffffffu;
-            bar_both();
+            if (hd.any_unfinite) {
+                for (uint32_t i = tid; i < 3 * D; i += 256) hd.unfinite[i] = 0x7fffffffu;
+                bar_both();
+                if (tid == 0) hd.any_unfinite = 0;
+            }
         }
     }
     griddep_launch_dependents();
@@ -771,12 +904,64 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
     }
 }
 
+// The rows of the blocks that several CTAs shared: block x is the one that begins in CTA x's share, y 16 of its rows. The records are added in
+// order of their CTAs. A launch of its own, so that all SMs read them (one CTA alone: 38 records of 32 rows 97 us).
+constexpr uint32_t kCombineRows = 16, kCombineThreads = 128;
+template <int D, int Parts>
+__global__ void __launch_bounds__(kCombineThreads) paged_tm_combine_kernel(const __grid_constant__ PagedAttnArgs a) {
+    __shared__ __align__(16) float4 rows_s[kCombineRows][D / 4 + 1];
+    griddep_launch_dependents();
+    griddep_wait();
+    const PagedTmBlock b = a.blocks[blockIdx.x];
+    const uint32_t row0 = blockIdx.y * kCombineRows;
+    if (b.records == 0 || row0 >= b.rows) return;
+    constexpr uint32_t kRecord = Tm<D, Parts>::kRecord, kChunks = D / 4, kPer = kCombineRows * kChunks / kCombineThreads, kStep = kCombineThreads / kCombineRows;
+    const uint32_t rw = threadIdx.x % kCombineRows, c = threadIdx.x / kCombineRows, lane_of = row0 / kRowsL, r = row0 % kRowsL + rw;
+    const uint32_t at = b.row0 + row0 + rw, tok = at / a.group, head = b.hkv * a.group + at - tok * a.group;
+    const bool there = row0 + rw < b.rows;
+    auto record = [&](uint32_t i) { return a.part_tm + (uint64_t)(((blockIdx.x + i) * 2 + (i ? 0 : b.slot)) * 2 + lane_of) * kRecord; };
+    float from = -INFINITY, high = -INFINITY, sum = 0.f;
+#pragma unroll 4
+    for (uint32_t i = 0; i < b.records; ++i) {
+        from = fmaxf(from, __ldcg(record(i) + D * kRowsL + r));
+        high = fmaxf(high, __ldcg(record(i) + (D + 2) * kRowsL + r));
+    }
+    float4 v[kPer];
+#pragma unroll
+    for (uint32_t j = 0; j < kPer; ++j) v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (uint32_t i = 0; i < b.records; ++i) {
+        const float *rec = record(i);
+        const float m = __ldcg(rec + D * kRowsL + r), x = __ldcg(rec + (D + 1) * kRowsL + r), w = m == -INFINITY ? 0.f : exp2_fast(m - from);
+        sum = fmaf(x, w, sum);
+#pragma unroll
+        for (uint32_t j = 0; j < kPer; ++j) {
+            const float4 u = __ldcg(reinterpret_cast<const float4 *>(rec) + (c + j * kStep) * kRowsL + r);
+            v[j].x = fmaf(u.x, w, v[j].x); v[j].y = fmaf(u.y, w, v[j].y); v[j].z = fmaf(u.z, w, v[j].z); v[j].w = fmaf(u.w, w, v[j].w);
+        }
+    }
+    const float inv = b.past + (int32_t)tok < 0 ? 0.f : 1.f / sum;
+#pragma unroll
+    for (uint32_t j = 0; j < kPer; ++j) rows_s[rw][c + j * kStep] = make_float4(v[j].x * inv, v[j].y * inv, v[j].z * inv, v[j].w * inv);
+    if (c == 0 && there && a.lse) a.lse[(uint64_t)(b.first + tok) * a.n_kv * a.group + head] = lse_of(high, from, sum);
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < kCombineRows * kChunks; i += kCombineThreads) {
+        const uint32_t ro = i / kChunks, ch = i % kChunks;
+        if (row0 + ro >= b.rows) break;
+        const uint32_t x = b.row0 + row0 + ro, t = x / a.group, h = b.hkv * a.group + x - t * a.group;
+        const uint64_t dst = (b.first + t) * a.out_stride + (uint64_t)h * D + ch * 4;
+        const float4 y = rows_s[ro][ch];
+        if (Parts == 1) *reinterpret_cast<uint2 *>((__half *)a.out + dst) = make_uint2(half2_bits(y.x, y.y), half2_bits(y.z, y.w));
+        else *reinterpret_cast<float4 *>((float *)a.out + dst) = y;
+    }
+}
+
 template <int D, int Parts> constexpr size_t tm_smem() { return Tm<D, Parts>::kBytes + 1024; }
 static_assert(tm_smem<128, 2>() <= 227 * 1024 && tm_smem<128, 1>() <= 227 * 1024 && tm_smem<64, 2>() <= 227 * 1024, "shared memory");
 
-const struct { void (*k)(const PagedAttnArgs); size_t smem; } kKernels[2][2] = {
-    {{paged_tm_kernel<64, 2>, tm_smem<64, 2>()}, {paged_tm_kernel<64, 1>, tm_smem<64, 1>()}},
-    {{paged_tm_kernel<128, 2>, tm_smem<128, 2>()}, {paged_tm_kernel<128, 1>, tm_smem<128, 1>()}}};
+const struct { void (*k)(const PagedAttnArgs); size_t smem; void (*combine)(const PagedAttnArgs); } kKernels[2][2] = {
+    {{paged_tm_kernel<64, 2>, tm_smem<64, 2>(), paged_tm_combine_kernel<64, 2>}, {paged_tm_kernel<64, 1>, tm_smem<64, 1>(), paged_tm_combine_kernel<64, 1>}},
+    {{paged_tm_kernel<128, 2>, tm_smem<128, 2>(), paged_tm_combine_kernel<128, 2>}, {paged_tm_kernel<128, 1>, tm_smem<128, 1>(), paged_tm_combine_kernel<128, 1>}}};
 
 } // namespace
 
@@ -787,16 +972,17 @@ cudaError_t paged_tm_init(void) {
     return cudaSuccess;
 }
 
-size_t paged_tm_part_bytes(int sms) { return (size_t)6 * sms * Tm<128, 2>::kRecord * sizeof(float); }
+size_t paged_tm_part_bytes(int sms) { return (size_t)6 * sms * Tm<128, 2>::kRecord * sizeof(float) + (size_t)sms * sizeof(PagedTmBlock); }
 
 cudaError_t launch_paged_tm(PagedAttnArgs a, const void *k, const void *v, uint32_t head_dim, int sms, cudaStream_t stream) {
     const uint64_t rows = (uint64_t)a.n_pages * a.n_kv << a.page_shift;
     const uint32_t box = std::min(1u << a.page_shift, kTile);
-    if (2 * (uint32_t)sms > kPagedTickets) return cudaErrorInvalidConfiguration;
+    a.blocks = reinterpret_cast<PagedTmBlock *>(a.part_tm + (size_t)6 * sms * Tm<128, 2>::kRecord);
     if (const cudaError_t e = tensor_map_groups_swz(&a.kmap, k, rows, head_dim, box)) return e;
     if (const cudaError_t e = tensor_map_groups_swz(&a.vmap, v, rows, head_dim, box)) return e;
     const auto &kernel = kKernels[head_dim == 128][a.half];
-    return launch_kernel(kernel.k, dim3((uint32_t)sms), dim3(kThreads), kernel.smem, stream, true, a);
+    if (const cudaError_t e = launch_kernel(kernel.k, dim3((uint32_t)sms), dim3(kThreads), kernel.smem, stream, true, a)) return e;
+    return launch_kernel(kernel.combine, dim3((uint32_t)sms, 2 * kRowsL / kCombineRows), dim3(kCombineThreads), 0, stream, true, a);
 }
 
 } // namespace flb

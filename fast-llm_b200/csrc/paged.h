@@ -16,6 +16,11 @@ constexpr uint32_t kPagedMaxSeq = 4096;   // sequences of a call: the plan keeps
 // Token i of n attends keys 0 .. kv_len - n + i. A block of rows over one KV head walks tiles of keys; the tiles of all blocks lie
 // on one line and every CTA takes an equal, contiguous piece of it, so that ragged batches load all SMs alike. A block that several
 // CTAs share leaves one record per CTA; the CTA that arrives last adds them in order (no CTA waits for another).
+// A block that several CTAs of attn_paged_tm.cu share, noted by the one that begins it.
+struct PagedTmBlock {
+    uint32_t records, sm, slot, first, row0, rows, hkv;   // records: CTAs; 0: none. slot: of the first CTA's record
+    int32_t past;
+};
 struct PagedAttnArgs {
     CUtensorMap kmap, vmap;         // tensor_map_groups_swz: one copy per page; the layout of ldmatrix and tcgen05 operands alike
     const void *q;
@@ -23,6 +28,7 @@ struct PagedAttnArgs {
     float2 *lse;                    // optional
     const int32_t *table, *q_start, *kv_len;
     float *part, *part_tm;          // records
+    PagedTmBlock *blocks;           // one per CTA
     uint32_t *tickets;              // zero between launches
     uint32_t *status;
     uint64_t q_stride, out_stride;  // elements between tokens
