@@ -168,6 +168,22 @@ __device__ __forceinline__ float max_of(const float (&s)[32]) {
         for (int j = 0; j < 4; ++j) t[j] = fmaxf(t[j], s[c + j]);
     return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
 }
+__device__ __forceinline__ void add4(float4 *at, const float4 &v) {
+    asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(at), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+// A row's sums in memory (columns 32 c .. for the bits c of `out`) from one reference to another, which is returned.
+__device__ __noinline__ float move_sums(float4 *mem, uint32_t out, float from, float to) {
+    __threadfence();
+    const float by = from == -INFINITY ? 0.f : exp2_fast(from - to);
+    for (uint32_t c = 0; c < 32; ++c)
+        if (out >> (c / 8) & 1u) {
+            float4 *at = mem + c * kRowsL;
+            const float4 v = __ldcg(at);
+            __stcg(at, make_float4(v.x * by, v.y * by, v.z * by, v.w * by));
+        }
+    __threadfence();
+    return to;
+}
 // 32 scores to probabilities, in place in tensor memory (at): 2^(s f + m) as f16, hi parts in the first 16 columns and, with two parts,
 // lo parts in the others; sum += them. The hi part is the value cut off after 10 bits of mantissa, so that
 // the lo part needs no conversion back: both together keep 21 bits.
@@ -649,7 +665,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
         };
         auto bar_both = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
         float4 *acc_mem = reinterpret_cast<float4 *>(a.part_tm + ((uint64_t)gridDim.x * 4 + blockIdx.x * 2 + l) * T::kRecord) + r;   // this row's sums
-        auto part_of = [](const float (&x)[4], uint32_t c) { return c == 0 ? x[0] : c == 1 ? x[1] : c == 2 ? x[2] : x[3]; };
         uint32_t s_seen = 0;
         if (warp == 0) { hd.walk = walk; hd.job.slot = 2; }   // (2: none yet)
         for (;;) {
@@ -689,38 +704,33 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
             if (lane == 0) arrive(&hd.q_full);
 
             float ref = -INFINITY, sum = 0.f, highest = -INFINITY;
-            float acc_ref[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};   // references of the sums in memory, per 32 columns
+            float acc_ref = -INFINITY;                                         // reference of the sums in memory
             uint32_t out_of = 0;                                               // bit c: columns 32 c .. have a sum in memory
             for (uint32_t step = 0; step < steps; ++step) {
                 const int32_t k0 = (int32_t)((t0 + (sm ? 2 * step + l : step)) * kTile);
                 const uint32_t c4 = step & 3u;   // the columns of O that go out at this step
-                const bool goes = Parts == 2 && active && step && c4 < D / 32, adds = goes && (out_of >> c4 & 1u);
-                if (goes) {
+                if (Parts == 2 && active && step && c4 < D / 32) {
                     // a part of O to its sum in memory, while the tensor cores form the scores
-                    float4 old[8];
-                    if (adds)
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) old[j] = __ldcg(acc_mem + (8 * c4 + j) * kRowsL);
                     if (!wait(&hd.o_done[l], (s_seen - 1) & 1u)) break;
                     fence_after();
-                    const float before = part_of(acc_ref, c4), keep = before == -INFINITY ? 0.f : exp2_fast(before - ref);
                     float o[32];
                     load32(to + 32 * c4, o);
                     wait_ld(o);
-                    if (adds)
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            o[4 * j] = fmaf(old[j].x, keep, o[4 * j]); o[4 * j + 1] = fmaf(old[j].y, keep, o[4 * j + 1]);
-                            o[4 * j + 2] = fmaf(old[j].z, keep, o[4 * j + 2]); o[4 * j + 3] = fmaf(old[j].w, keep, o[4 * j + 3]);
-                        }
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) __stcg(acc_mem + (8 * c4 + j) * kRowsL, make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]));
                     const uint32_t zero[16] = {};
                     store16(to + 32 * c4, zero);
                     store16(to + 32 * c4 + 16, zero);
-                    out_of |= 1u << c4;
+                    if (out_of == 0) acc_ref = ref;
+                    if (ref - acc_ref > 40.f) acc_ref = move_sums(acc_mem, out_of, acc_ref, ref);   // (far below what f32 holds: |O| < 2^47)
+                    const float by = ref == acc_ref ? 1.f : exp2_fast(ref - acc_ref);
+                    float4 *at = acc_mem + 8 * c4 * kRowsL;
+                    const bool adds = out_of >> c4 & 1u;
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) acc_ref[c] = c4 == (uint32_t)c ? ref : acc_ref[c];
+                    for (int j = 0; j < 8; ++j) {
+                        const float4 v = make_float4(o[4 * j] * by, o[4 * j + 1] * by, o[4 * j + 2] * by, o[4 * j + 3] * by);
+                        if (adds) add4(at + j * kRowsL, v);
+                        else __stcg(at + j * kRowsL, v);
+                    }
+                    out_of |= 1u << c4;
                 }
                 if (!wait(&hd.s_full[l], s_seen & 1u)) break;
                 ++s_seen;
@@ -802,14 +812,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
                 // (every PV product of a lane follows one of its scores: as many of both)
                 wait(&hd.o_done[l], (s_seen - 1) & 1u);
                 fence_after();
+                if (Parts == 2) __threadfence();   // (the additions to the sums in memory come before the loads below)
             }
             // A small block: the second lane hands its sums to the first, in tensor memory, where its scores were
-            float ref2 = -INFINITY, sum2 = 0.f, acc2_ref[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            float ref2 = -INFINITY, sum2 = 0.f, acc2_ref = -INFINITY;
             uint32_t out2 = 0;
             if (sm) {
                 if (l && active) {
-                    const uint32_t w[16] = {__float_as_uint(ref), __float_as_uint(sum), __float_as_uint(highest), out_of, __float_as_uint(acc_ref[0]), __float_as_uint(acc_ref[1]),
-                                            __float_as_uint(acc_ref[2]), __float_as_uint(acc_ref[3])};
+                    const uint32_t w[16] = {__float_as_uint(ref), __float_as_uint(sum), __float_as_uint(highest), out_of, __float_as_uint(acc_ref)};
                     store16(ts, w);
                     wait_st();
                 }
@@ -820,9 +830,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
                     float w[32];
                     load32(ts + kTile, w);
                     wait_ld(w);
-                    ref2 = w[0]; sum2 = w[1]; highest = fmaxf(highest, w[2]); out2 = __float_as_uint(w[3]);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) acc2_ref[c] = w[4 + c];
+                    ref2 = w[0]; sum2 = w[1]; highest = fmaxf(highest, w[2]); out2 = __float_as_uint(w[3]); acc2_ref = w[4];
                 }
             }
             if (steps && !dead && active && !(sm && l)) {
@@ -845,7 +853,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
                             for (int j = 0; j < 8; ++j) old[j] = __ldcg(mem + (8 * c + j) * kRowsL);
                         wait_ld(o);
                         if (acc) {
-                            const float keep = before == -INFINITY ? 0.f : exp2_fast(before - rf);
+                            const float keep = before == rf ? 1.f : exp2_fast(before - rf);
 #pragma unroll
                             for (int j = 0; j < 8; ++j) {
                                 o[4 * j] = fmaf(old[j].x, keep, o[4 * j]); o[4 * j + 1] = fmaf(old[j].y, keep, o[4 * j + 1]);
@@ -855,11 +863,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
                     };
                     float v[32];
                     if (two) {
-                        lane_part(to + 128, acc_mem + T::kRecord / 4, out2, part_of(acc2_ref, c), ref2);
+                        lane_part(to + 128, acc_mem + T::kRecord / 4, out2, acc2_ref, ref2);
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v[j] = o[j] * w2;
                     }
-                    lane_part(to, acc_mem, out_of, part_of(acc_ref, c), ref);
+                    lane_part(to, acc_mem, out_of, acc_ref, ref);
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[j] = two ? fmaf(o[j], w1, v[j]) : o[j];
                     if (any_unfinite)
