@@ -184,6 +184,22 @@ __device__ __noinline__ float move_sums(float4 *mem, uint32_t out, float from, f
     __threadfence();
     return to;
 }
+// (out of line, as load_q and finish are: what they need in registers stays out of the loop over the tiles)
+__device__ __noinline__ void scale_o(uint32_t at, uint32_t columns, float by) {
+#pragma unroll 1
+    for (uint32_t c = 0; c < columns; c += 32) {
+        float o[32];
+        load32(at + c, o);
+        wait_ld(o);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            uint32_t w[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(o[16 * h + j] * by);
+            store16(at + c + 16 * h, w);
+        }
+    }
+}
 // 32 scores to probabilities, in place in tensor memory (at): 2^(s f + m) as f16, hi parts in the first 16 columns and, with two parts,
 // lo parts in the others; sum += them. The hi part is the value cut off after 10 bits of mantissa, so that
 // the lo part needs no conversion back: both together keep 21 bits.
@@ -213,7 +229,7 @@ template <int Parts> __device__ __forceinline__ void exp_chunk(const float (&s)[
 // brings its largest value to [2^11, 2^12): 8 lanes a row, 4 rows at a time. src: of the thread's own row; returns what its scores are to be
 // multiplied by (exponents of 2).
 template <int D, int Parts>
-__device__ __forceinline__ float load_q(const PagedAttnArgs &a, uint8_t *dst, uint64_t src, uint32_t row0, uint32_t rows, bool store) {
+__device__ __noinline__ float load_q(const PagedAttnArgs &a, uint8_t *dst, uint64_t src, uint32_t row0, uint32_t rows, bool store) {
     constexpr int V = 4, K = D / 32, kBatch = 4;   // values of a load, loads of a lane and row, groups of 4 rows in flight
     const uint32_t lane = threadIdx.x & 31u, sub = lane & 7u, group = lane >> 3;
     float f = 0.f;
@@ -394,6 +410,104 @@ __device__ __forceinline__ uint32_t copy_at(bool sm, uint32_t i, uint32_t n, boo
 // Whether a tile holds keys that not all rows of the block attend.
 __device__ __forceinline__ bool partly(const PagedAttnArgs &a, const Piece &p, uint32_t tile) {
     return (int32_t)((tile + 1) * kTile) > p.q.past + (int32_t)(p.blk * 2 * kRowsL / a.group) + 1;
+}
+
+__device__ __forceinline__ void bar_both() { asm volatile("bar.sync 1, 256;" ::: "memory"); }   // the softmax warps
+
+struct Sums { float ref, sum, highest, acc_ref; uint32_t out_of; };   // of a row
+// The results of a lane's piece: the rows themselves, or a record. done: the lane has any, and they are in tensor memory.
+template <int D, int Parts>
+__device__ __noinline__ void finish(const PagedAttnArgs &a, Head &hd, uint8_t *q_s, const Sums s, bool done, uint32_t tmem) {
+    using T = Tm<D, Parts>;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, l = warp >> 2, w4 = warp & 3u, r = tid & 127u;
+    const uint32_t ts = tmem + (w4 * 32u << 16) + l * kTile, to = tmem + (w4 * 32u << 16) + kOCol + l * 128;
+    const float4 *acc_mem = reinterpret_cast<const float4 *>(a.part_tm + ((uint64_t)gridDim.x * 4 + blockIdx.x * 2 + l) * T::kRecord) + r;
+    const Job &job = hd.job;
+    const bool sm = job.sm;
+    const uint32_t row0 = job.row0 + (sm ? 0 : l * kRowsL), rows = min(kRowsL, sm ? job.rows : job.rows - min(job.rows, l * kRowsL));
+    const uint32_t tok = (row0 + r) / a.group, head = job.hkv * a.group + (row0 + r) - tok * a.group;
+    const bool there = r < rows, active = w4 * 32 < rows;
+    const int32_t lim = there ? job.past + (int32_t)tok : 0x7fffffff;
+    float ref = s.ref, sum = s.sum, highest = s.highest;
+    // A small block: the second lane hands its sums to the first, in tensor memory, where its scores were
+    float ref2 = -INFINITY, sum2 = 0.f, acc2_ref = -INFINITY;
+    uint32_t out2 = 0;
+    if (sm) {
+        if (l && active) {
+            const uint32_t w[16] = {__float_as_uint(ref), __float_as_uint(sum), __float_as_uint(highest), s.out_of, __float_as_uint(s.acc_ref)};
+            store16(ts, w);
+            wait_st();
+        }
+        fence_before();
+        bar_both();
+        fence_after();
+        if (!l && active && job.n > 1) {
+            float w[32];
+            load32(ts + kTile, w);
+            wait_ld(w);
+            ref2 = w[0]; sum2 = w[1]; highest = fmaxf(highest, w[2]); out2 = __float_as_uint(w[3]); acc2_ref = w[4];
+        }
+    }
+    if (done && active && !(sm && l)) {
+        const bool whole = job.whole, two = sm && job.n > 1;
+        const float both = fmaxf(ref, ref2), w1 = ref == -INFINITY ? 0.f : exp2_fast(ref - both), w2 = ref2 == -INFINITY ? 0.f : exp2_fast(ref2 - both);
+        const float all = fmaf(sum, w1, sum2 * w2), inv = lim < 0 ? 0.f : 1.f / all;
+        float *rec = a.part_tm + (uint64_t)((blockIdx.x * 2 + job.slot) * 2 + l) * T::kRecord;
+        // Rows go out through shared memory, where the lane's q was (a small block's lanes share the first q; the second is free).
+        uint8_t *stage = q_s + (sm ? 1 : l) * Parts * T::kPart;
+        const bool any_unfinite = hd.any_unfinite != 0;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+            float o[32];
+            auto lane_part = [&](uint32_t from, const float4 *mem, uint32_t out, float before, float rf) {   // 32 columns of a lane's contexts
+                load32(from + 32 * c, o);
+                const bool acc = Parts == 2 && (out >> c & 1u);
+                float4 old[8];
+                if (acc)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) old[j] = __ldcg(mem + (8 * c + j) * kRowsL);
+                wait_ld(o);
+                if (acc) {
+                    const float keep = before == rf ? 1.f : exp2_fast(before - rf);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        o[4 * j] = fmaf(old[j].x, keep, o[4 * j]); o[4 * j + 1] = fmaf(old[j].y, keep, o[4 * j + 1]);
+                        o[4 * j + 2] = fmaf(old[j].z, keep, o[4 * j + 2]); o[4 * j + 3] = fmaf(old[j].w, keep, o[4 * j + 3]);
+                    }
+                }
+            };
+            float v[32];
+            if (two) {
+                lane_part(to + 128, acc_mem + T::kRecord / 4, out2, acc2_ref, ref2);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = o[j] * w2;
+            }
+            lane_part(to, acc_mem, s.out_of, s.acc_ref, ref);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = two ? fmaf(o[j], w1, v[j]) : o[j];
+            if (any_unfinite)
+#pragma unroll 1
+                for (int j = 0; j < 32; ++j) {
+                    const float u = unfinite_at(hd.unfinite, D, 32 * c + j, lim);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] += i == j ? u : 0.f;
+                }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (!whole) __stcg(reinterpret_cast<float4 *>(rec) + (8 * c + j) * kRowsL + r, make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+                else stage_put<D, Parts>(stage, r, 8 * c + j, make_float4(v[4 * j] * inv, v[4 * j + 1] * inv, v[4 * j + 2] * inv, v[4 * j + 3] * inv));
+            }
+        }
+        const float from = two ? both : ref, total_sum = two ? all : sum;
+        if (whole) {
+            stage_out<D, Parts>(stage, a.out, w4 * 32, rows, (job.first + tok) * a.out_stride + (uint64_t)head * D);
+            if (there && a.lse) a.lse[(uint64_t)(job.first + tok) * a.n_kv * a.group + head] = lse_of(highest, from, total_sum);
+        } else {
+            __stcg(rec + D * kRowsL + r, from);
+            __stcg(rec + (D + 1) * kRowsL + r, total_sum);
+            __stcg(rec + (D + 2) * kRowsL + r, highest);
+        }
+    }
 }
 
 template <int D, int Parts>
@@ -659,11 +773,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
         // ---- softmax: lane l, thread = row ----
         const uint32_t l = warp >> 2, w4 = warp & 3u, r = tid & 127u;
         const uint32_t ts = tmem + (w4 * 32u << 16) + l * kTile, to = tmem + (w4 * 32u << 16) + kOCol + l * 128;
-        auto bar_lane = [&] {
-            if (l) asm volatile("bar.sync 3, 128;" ::: "memory");
-            else asm volatile("bar.sync 2, 128;" ::: "memory");
-        };
-        auto bar_both = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
         float4 *acc_mem = reinterpret_cast<float4 *>(a.part_tm + ((uint64_t)gridDim.x * 4 + blockIdx.x * 2 + l) * T::kRecord) + r;   // this row's sums
         uint32_t s_seen = 0;
         if (warp == 0) { hd.walk = walk; hd.job.slot = 2; }   // (2: none yet)
@@ -765,21 +874,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
                     sum *= al;
                     rescale = al;
                 }
-                if (step && __any_sync(0xffffffffu, rescale != 1.f)) {
-#pragma unroll 1
-                    for (int c = 0; c < D; c += 32) {
-                        float o[32];
-                        load32(to + c, o);
-                        wait_ld(o);
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            uint32_t w[16];
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(o[16 * h + j] * rescale);
-                            store16(to + c + 16 * h, w);
-                        }
-                    }
-                }
+                if (step && __any_sync(0xffffffffu, rescale != 1.f)) scale_o(to, D, rescale);
                 const float m = ref == -INFINITY ? 0.f : ref;
                 const F2 f2 = pair(f, f), m2 = pair(-m, -m);
                 F2 part[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
@@ -814,85 +909,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
                 fence_after();
                 if (Parts == 2) __threadfence();   // (the additions to the sums in memory come before the loads below)
             }
-            // A small block: the second lane hands its sums to the first, in tensor memory, where its scores were
-            float ref2 = -INFINITY, sum2 = 0.f, acc2_ref = -INFINITY;
-            uint32_t out2 = 0;
-            if (sm) {
-                if (l && active) {
-                    const uint32_t w[16] = {__float_as_uint(ref), __float_as_uint(sum), __float_as_uint(highest), out_of, __float_as_uint(acc_ref)};
-                    store16(ts, w);
-                    wait_st();
-                }
-                fence_before();
-                bar_both();
-                fence_after();
-                if (!l && active && job.n > 1) {
-                    float w[32];
-                    load32(ts + kTile, w);
-                    wait_ld(w);
-                    ref2 = w[0]; sum2 = w[1]; highest = fmaxf(highest, w[2]); out2 = __float_as_uint(w[3]); acc2_ref = w[4];
-                }
-            }
-            if (steps && !dead && active && !(sm && l)) {
-                const bool whole = job.whole, two = sm && job.n > 1;
-                const float both = fmaxf(ref, ref2), w1 = ref == -INFINITY ? 0.f : exp2_fast(ref - both), w2 = ref2 == -INFINITY ? 0.f : exp2_fast(ref2 - both);
-                const float all = fmaf(sum, w1, sum2 * w2), inv = lim < 0 ? 0.f : 1.f / all;
-                float *rec = a.part_tm + (uint64_t)((blockIdx.x * 2 + job.slot) * 2 + l) * T::kRecord;
-                // Rows go out through shared memory, where the lane's q was (a small block's lanes share the first q; the second is free).
-                uint8_t *stage = q_s + (sm ? 1 : l) * Parts * T::kPart;
-                const bool any_unfinite = hd.any_unfinite != 0;
-#pragma unroll 1
-                for (int c = 0; c < D / 32; ++c) {
-                    float o[32];
-                    auto lane_part = [&](uint32_t from, const float4 *mem, uint32_t out, float before, float rf) {   // 32 columns of a lane's contexts
-                        load32(from + 32 * c, o);
-                        const bool acc = Parts == 2 && (out >> c & 1u);
-                        float4 old[8];
-                        if (acc)
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) old[j] = __ldcg(mem + (8 * c + j) * kRowsL);
-                        wait_ld(o);
-                        if (acc) {
-                            const float keep = before == rf ? 1.f : exp2_fast(before - rf);
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                o[4 * j] = fmaf(old[j].x, keep, o[4 * j]); o[4 * j + 1] = fmaf(old[j].y, keep, o[4 * j + 1]);
-                                o[4 * j + 2] = fmaf(old[j].z, keep, o[4 * j + 2]); o[4 * j + 3] = fmaf(old[j].w, keep, o[4 * j + 3]);
-                            }
-                        }
-                    };
-                    float v[32];
-                    if (two) {
-                        lane_part(to + 128, acc_mem + T::kRecord / 4, out2, acc2_ref, ref2);
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = o[j] * w2;
-                    }
-                    lane_part(to, acc_mem, out_of, acc_ref, ref);
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = two ? fmaf(o[j], w1, v[j]) : o[j];
-                    if (any_unfinite)
-#pragma unroll 1
-                        for (int j = 0; j < 32; ++j) {
-                            const float u = unfinite_at(hd.unfinite, D, 32 * c + j, lim);
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) v[i] += i == j ? u : 0.f;
-                        }
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        if (!whole) __stcg(reinterpret_cast<float4 *>(rec) + (8 * c + j) * kRowsL + r, make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
-                        else stage_put<D, Parts>(stage, r, 8 * c + j, make_float4(v[4 * j] * inv, v[4 * j + 1] * inv, v[4 * j + 2] * inv, v[4 * j + 3] * inv));
-                    }
-                }
-                const float from = two ? both : ref, total_sum = two ? all : sum;
-                if (whole) {
-                    stage_out<D, Parts>(stage, a.out, w4 * 32, rows, (job.first + tok) * a.out_stride + (uint64_t)head * D);
-                    if (there && a.lse) a.lse[(uint64_t)(job.first + tok) * a.n_kv * a.group + head] = lse_of(highest, from, total_sum);
-                } else {
-                    __stcg(rec + D * kRowsL + r, from);
-                    __stcg(rec + (D + 1) * kRowsL + r, total_sum);
-                    __stcg(rec + (D + 2) * kRowsL + r, highest);
-                }
-            }
+            finish<D, Parts>(a, hd, q_s, Sums{ref, sum, highest, acc_ref, out_of}, steps != 0 && !dead, tmem);
             fence_before();
             bar_both();   // both lanes are done with q, O and the notes
             if (hd.any_unfinite) {
