@@ -62,7 +62,7 @@ struct Piece {
     uint64_t base;       // unit of its block's tile 0
 };
 struct Head {
-    uint64_t full[8], empty[8], ready[8], s_full[2], p_full[2][2], o_done[2], q_full, drain;
+    uint64_t full[8], empty[8], v_ready[8], s_full[2], p_full[2][2], o_done[2], q_full, drain;
     uint64_t start_off;
     uint32_t start_seq, tmem, abort_flag, any_unfinite;
     Job job;
@@ -160,13 +160,18 @@ __device__ __forceinline__ void cut_at(float (&s)[32], int32_t valid) {   // col
 #pragma unroll
     for (int c = 0; c < 32; ++c) s[c] = c <= valid ? s[c] : -INFINITY;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 __device__ __forceinline__ float max_of(const float (&s)[32]) {
-    float t[4] = {s[0], s[1], s[2], s[3]};
+    float t[4] = {max3(s[0], s[1], s[2]), max3(s[3], s[4], s[5]), max3(s[6], s[7], s[8]), max3(s[9], s[10], s[11])};
 #pragma unroll
-    for (int c = 4; c < 32; c += 4)
+    for (int c = 12; c < 28; c += 8)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) t[j] = fmaxf(t[j], s[c + j]);
-    return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+        for (int j = 0; j < 4; ++j) t[j] = max3(t[j], s[c + 2 * j], s[c + 2 * j + 1]);
+    return max3(max3(t[0], s[28], s[29]), max3(t[1], s[30], s[31]), fmaxf(t[2], t[3]));
 }
 __device__ __forceinline__ void add4(float4 *at, const float4 &v) {
     asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(at), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
@@ -519,7 +524,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
     uint8_t *q_s = base + T::kHead, *ring = q_s + T::kQ;
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
     if (tid == 0) {
-        for (uint32_t s = 0; s < T::kSlots; ++s) { mbar_init(&hd.full[s], 1); mbar_init(&hd.empty[s], 1); mbar_init(&hd.ready[s], 1); }
+        for (uint32_t s = 0; s < T::kSlots; ++s) { mbar_init(&hd.full[s], 1); mbar_init(&hd.empty[s], 1); }
+        for (uint32_t s = 0; s < 8; ++s) mbar_init(&hd.v_ready[s], 1);
         for (int l = 0; l < 2; ++l) { mbar_init(&hd.s_full[l], 1); mbar_init(&hd.p_full[l][0], 4); mbar_init(&hd.p_full[l][1], 4); mbar_init(&hd.o_done[l], 1); }
         mbar_init(&hd.q_full, 8);
         mbar_init(&hd.drain, 1);
@@ -641,38 +647,48 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
         // ---- tensor cores ----
         constexpr uint32_t kIdS = idesc_of(kTile, false), kIdO = idesc_of(D, true), kGroup = D * 16;
         uint32_t pv[2] = {0, 0};   // PV products of a lane so far
-        auto ring_wait = [&](uint32_t i) { return wait(&hd.full[(done + i) % T::kSlots], ((done + i) / T::kSlots) & 1u); };
+        uint32_t v_done = 0;       // V tiles of the pieces in front
+        const uint32_t ring_s = smem_u32(ring);
+        const uint64_t q_desc = desc(smem_u32(q_s), 0, 1024), k_desc = desc(ring_s, 0, kGroup), v_desc = desc(ring_s, 1024, kGroup);
+        // A copy's slot and the parity of its barrier. (Waits for several barriers ask for all of them before they look at an answer: one
+        // round trip to shared memory instead of one each; the tensor cores stand still meanwhile.)
+        auto slot_of = [&](uint32_t i) { return (done + i) % T::kSlots; };
+        auto parity_of = [&](uint32_t i) { return ((done + i) / T::kSlots) & 1u; };
+        auto wait2 = [&](uint64_t *x, uint32_t px, uint64_t *y, uint32_t py) {
+            const bool gx = try_bar(x, px), gy = try_bar(y, py);
+            return __all_sync(0xffffffffu, gx && gy) || (wait(x, px) && wait(y, py));
+        };
         auto uniform = [](uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); };
-        auto scores = [&](uint32_t l, uint32_t ql, uint32_t i) {   // of lane l, q of lane ql, K in copy i
-            const uint32_t d = uniform(tmem + l * kTile), qa = uniform(smem_u32(q_s) + ql * Parts * T::kPart), ka = uniform(smem_u32(ring) + ((done + i) % T::kSlots) * T::kPart);
+        auto scores = [&](uint32_t l, uint32_t ql, uint32_t slot) {   // of lane l, q of lane ql, K in a slot
+            const uint32_t d = tmem + l * kTile;
+            const uint64_t qd = q_desc + (ql * Parts * T::kPart >> 4), kd = k_desc + (slot * T::kPart >> 4);
             if (elect_one()) {
 #pragma unroll
                 for (int part = Parts - 1; part >= 0; --part)
 #pragma unroll
                     for (int kb = 0; kb < D / 16; ++kb)
-                        mma_ss(d, desc(qa, 0, 1024) + ((part * T::kPart + (kb >> 2) * (kRowsL * 128) + (kb & 3) * 32) >> 4), desc(ka, 0, kGroup) + (((kb >> 2) * 1024 + (kb & 3) * 32) >> 4), kIdS,
+                        mma_ss(d, qd + ((part * T::kPart + (kb >> 2) * (kRowsL * 128) + (kb & 3) * 32) >> 4), kd + (((kb >> 2) * 1024 + (kb & 3) * 32) >> 4), kIdS,
                                part != Parts - 1 || kb != 0);
                 commit(&hd.s_full[l]);
             }
             __syncwarp();
         };
-        // O += P V for keys 64 .. 127 (first), then 0 .. 63 of the tile, V in copy i
-        auto context = [&](uint32_t l, uint32_t i, uint32_t half, bool from_zero) {
-            const uint32_t d = uniform(tmem + kOCol + l * 128), pa = uniform(tmem + l * kTile + half * 64), va = uniform(smem_u32(ring) + ((done + i) % T::kSlots) * T::kPart + half * 8 * kGroup);
+        // O += P V for keys 64 .. 127 (first), then 0 .. 63 of the tile, V in a slot
+        auto context = [&](uint32_t l, uint32_t slot, uint32_t half, bool from_zero) {
+            const uint32_t d = tmem + kOCol + l * 128, pa = tmem + l * kTile + half * 64;
+            const uint64_t vd = v_desc + ((slot * T::kPart + half * 8 * kGroup) >> 4);
             if (elect_one()) {
 #pragma unroll
                 for (int part = Parts - 1; part >= 0; --part)
 #pragma unroll
                     for (int kk = 0; kk < (int)kTile / 32; ++kk)
-                        mma_ts(d, pa + (kk >> 1) * 32 + part * 16 + (kk & 1) * 8, desc(va, 1024, kGroup) + ((kk * 2 * kGroup) >> 4), kIdO, !from_zero || part != Parts - 1 || kk != 0);
+                        mma_ts(d, pa + (kk >> 1) * 32 + part * 16 + (kk & 1) * 8, vd + ((kk * 2 * kGroup) >> 4), kIdO, !from_zero || part != Parts - 1 || kk != 0);
                 if (!half) commit(&hd.o_done[l]);
             }
             __syncwarp();
         };
-        auto ready = [&](uint32_t i) { return wait(&hd.ready[(done + i) % T::kSlots], ((done + i) / T::kSlots) & 1u); };
-        auto release = [&](uint32_t i) {
-            ready(i);   // (a slot is not filled again before the value warp has seen it; it is long past)
-            if (elect_one()) commit(&hd.empty[(done + i) % T::kSlots]);
+        auto release = [&](uint32_t slot) {
+            if (elect_one()) commit(&hd.empty[slot]);
             __syncwarp();
         };
         while (!dead && next_piece(a, walk, p)) {
@@ -682,38 +698,42 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
             ++pieces_in;
             fence_after();
             // the first scores
-            if (!ring_wait(0)) break;
-            scores(0, 0, 0);
-            if (sm) release(0);
+            uint32_t slot = uniform(slot_of(0));
+            if (!wait(&hd.full[slot], parity_of(0))) break;
+            scores(0, 0, slot);
+            if (sm) release(slot);
             if (!sm || n > 1) {
-                const uint32_t i = sm ? 1 : 0;
-                if (!ring_wait(i)) break;
-                scores(1, sm ? 0 : 1, i);
-                release(i);
+                if (sm) {
+                    slot = uniform(slot_of(1));
+                    if (!wait(&hd.full[slot], parity_of(1))) break;
+                }
+                scores(1, sm ? 0 : 1, slot);
+                release(slot);
             }
             const uint32_t steps = sm ? (n + 1) / 2 : n;
             for (uint32_t step = 0; step < steps && !dead; ++step)
                 for (uint32_t l = 0; l < 2 && !dead; ++l) {
                     const uint32_t t = sm ? 2 * step + l : step, next = sm ? t + 2 : t + 1;
                     if (t >= n) break;
-                    const uint32_t vi = v_index(sm, t, n), ki = k_index(sm, next);
-                    if (!ring_wait(vi) || !ready(vi)) break;
-                    if (!wait(&hd.p_full[l][1], pv[l] & 1u)) break;
+                    // (what the value warp has seen has landed)
+                    const uint32_t vs = uniform(slot_of(v_index(sm, t, n))), ki = k_index(sm, next), ks = uniform(slot_of(ki)), v_count = v_done + t;
+                    if (!wait2(&hd.p_full[l][1], pv[l] & 1u, &hd.v_ready[v_count & 7u], v_count >> 3 & 1u)) break;
                     fence_after();
-                    context(l, vi, 1, step == 0);
+                    context(l, vs, 1, step == 0);
                     if (!wait(&hd.p_full[l][0], pv[l] & 1u)) break;
                     fence_after();
-                    context(l, vi, 0, false);
+                    context(l, vs, 0, false);
                     ++pv[l];
-                    if (sm || l == 1) release(vi);
+                    if (sm || l == 1) release(vs);
                     if (next < n) {
                         // (the next scores overwrite the probabilities)
-                        if (!ring_wait(ki) || !wait(&hd.o_done[l], (pv[l] - 1) & 1u)) break;
+                        if (!wait2(&hd.full[ks], parity_of(ki), &hd.o_done[l], (pv[l] - 1) & 1u)) break;
                         fence_after();
-                        scores(l, sm ? 0 : l, ki);
-                        if (sm || l == 1) release(ki);
+                        scores(l, sm ? 0 : l, ks);
+                        if (sm || l == 1) release(ks);
                     }
                 }
+            v_done += n;
             done += 2 * n;
         }
         if (dead) {
@@ -724,18 +744,21 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
         }
     } else if (warp == kValueWarp) {
         // ---- values that must not meet the tensor cores ----
+        uint32_t v_seen = 0;
         while (!dead && next_piece(a, walk, p)) {
             const uint32_t n = p.t1 - p.t0;
             const bool sm = small(p);
             if (!wait(&hd.q_full, pieces_in & 1u)) break;   // (the notes of the piece before have been read)
             ++pieces_in;
             const int32_t lim_first = p.q.past + (int32_t)(p.blk * 2 * kRowsL / a.group);
-            for (uint32_t i = 0; i < 2 * n; ++i) {
-                bool v;
-                const uint32_t t = copy_at(sm, i, n, v), slot = (done + i) % T::kSlots;
-                if (!wait(&hd.full[slot], ((done + i) / T::kSlots) & 1u)) break;
-                if (!v || !partly(a, p, p.t0 + t)) {
-                    if (lane == 0) arrive(&hd.ready[slot]);
+            for (uint32_t t = 0; t < n; ++t, ++v_seen) {
+                const uint32_t i = done + v_index(sm, t, n), slot = i % T::kSlots;
+                // (a slot is not filled again before its V tile has been reported; at most five reports are ahead of the tensor warp, the V tiles of a full ring)
+                // (first that the slot was free: a copy before it that has not landed yet would leave the barrier one phase behind, where this
+                // phase's parity reads as complete)
+                if (!wait(&hd.empty[slot], ((i / T::kSlots) & 1u) ^ 1u) || !wait(&hd.full[slot], (i / T::kSlots) & 1u)) break;
+                if (!partly(a, p, p.t0 + t)) {
+                    if (lane == 0) arrive(&hd.v_ready[v_seen & 7u]);
                     continue;
                 }
                 uint8_t *vt = ring + slot * T::kPart;
@@ -765,7 +788,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) arrive(&hd.ready[slot]);
+                if (lane == 0) arrive(&hd.v_ready[v_seen & 7u]);
             }
             done += 2 * n;
         }
