@@ -4,14 +4,16 @@
 // o_r = sum_j exp(s_rj - m_r) v_j / sum_j exp(s_rj - m_r), s_rj = scale q_r . k_j, with the running maximum and sum of an online
 // softmax in f32. Bound by the HBM bytes of the keys and values: every tile is read once.
 //
-// CTA = 4 consumer warps + 1 producer warp, two CTAs per SM. The producer's lanes each copy one page's part of a tile (one TMA box
-// of up to 64 rows) into a ring of three stages of 32 KB; warp w takes keys 16 w .. 16 w + 15 of a tile through
-// ldmatrix. All tiles lie on one line (sequence, KV head, tile) and every CTA takes an equal piece of it.
-//   scores : A = 16 rows of q as (hi, lo) f16 parts, scaled by a power of two per row so that both parts stay normal numbers; B = K
-//   softmax: lane (g, t) has rows g and g + 8, keys 2t, 2t + 1 of every 8; row maxima over the 4 lanes of a row
-//   context: A = probabilities as (hi, lo) parts: the scores' accumulators have the layout of that operand; B = V (ldmatrix.trans).
-//            A tile's product starts from zero and is added in f32 with rounding, since the tensor cores truncate their running sum
-//            (1.3e-8 of it per instruction: 1e-5 after 800 tiles).
+// CTA = 4 warps, two CTAs per SM. Lanes of warp 0 each copy one page's part of a tile (one TMA box of up to 64 rows) into a ring of three
+// stages of 32 KB; warp w takes keys 16 w .. 16 w + 15 of a tile. All tiles lie on one line (sequence, KV head, tile) and every CTA
+// takes an equal piece of it.
+//   scores : A = 16 keys (ldmatrix), B = 4 rows of q as (hi, lo) f16 parts, scaled by a power of two per row so that both parts stay
+//            normal numbers: lane (g, t) has row t and keys g and g + 8
+//   softmax: row maxima over the 8 lanes of a row
+//   context: A = V^T (ldmatrix.trans), B = the probabilities as (hi, lo) parts. A tile's product starts from zero and is added in f32
+//            with rounding, since the tensor cores truncate their running sum (1.3e-8 of it per instruction: 1e-5 after 800 tiles).
+// Keys as rows of A cost 16 instructions per 16 keys and 4 rows; the rows as A cost 64 for any number of them, and a tile then took 1.25 us
+// of mma.sync (4 x 65000 keys 187 us).
 // A masked value never meets the tensor core as it is, since 0 x NaN is NaN: rows behind the last key are cleared in shared
 // memory, and among the keys of the new tokens, which not all rows attend, values that are not finite are taken out there and
 // their effect added to the rows that do attend them (see unfinite_of).
@@ -24,53 +26,8 @@ namespace flb {
 
 namespace {
 
-constexpr uint32_t kRowsB = 16, kTile = 64, kStages = 3, kWarps = 4, kThreads = (kWarps + 1) * 32;
+constexpr uint32_t kRowsB = kFewRows, kBlocks = kRowsB / 4, kTile = 64, kStages = 3, kWarps = 4, kThreads = kWarps * 32;
 constexpr float kShift = 12.f;   // probabilities are 2^(x - m + 12): their lo parts stay normal f16 numbers down to 2^-14 of the largest
-
-template <int D> struct FewSmem {
-    static constexpr uint32_t kHalfStage = kTile * D * 2;                 // K or V of a tile
-    uint8_t ring[kStages][2 * kHalfStage];                                // 1024-byte aligned
-    float o[kWarps][kRowsB][36];                                          // a quarter (half, D = 64) of the warps' contexts
-    float m[kWarps][kRowsB], l[kWarps][kRowsB];
-    uint32_t unfinite[3][D];                                              // see unfinite_of
-    uint64_t full[kStages], empty[kStages];
-    uint64_t sum[kThreads / 32];
-    uint32_t start_seq, any;
-    uint64_t start_off, total;
-};
-
-// Values of +inf, -inf and NaN (class 0, 1, 2) among the keys that only part of the rows attend: per class and dimension the
-// first such key. A row that attends keys 0 .. lim is affected by those <= lim.
-__device__ __forceinline__ float unfinite_of(const uint32_t *u, uint32_t dims, uint32_t d, int32_t lim) {
-    const int32_t p = (int32_t)u[d], n = (int32_t)u[dims + d], x = (int32_t)u[2 * dims + d];   // (0x7fffffff: none)
-    if (x <= lim || (p <= lim && n <= lim)) return __int_as_float(0x7fffffff);
-    return p <= lim ? INFINITY : n <= lim ? -INFINITY : 0.f;
-}
-
-__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-// D(16 x 8, f32) += A(16 x 16) B(16 x 8)
-__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t half2_bits(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-// (a, b) as two f16 pairs, hi + lo
-__device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t &lo) {
-    const __half2 h = __floats2half2_rn(a, b);
-    const float2 f = __half22float2(h);
-    hi = *reinterpret_cast<const uint32_t *>(&h);
-    lo = half2_bits(a - f.x, b - f.y);
-}
-__device__ __forceinline__ void bar_consumers() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
-__device__ __forceinline__ void arrive(uint64_t *bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory"); }
 
 // Rows of a sequence over one KV head, 0 where it is the other kernel's; its tiles: at least one, so that somebody writes its rows.
 __device__ __forceinline__ uint32_t rows_of(const PagedAttnArgs &a, const PagedSeq &q) { return q.n * a.group > a.few_rows ? 0u : q.n * a.group; }
@@ -82,11 +39,10 @@ struct Piece {
     PagedSeq q;
     uint32_t seq, hkv, rows, tiles, t0, t1;        // tiles t0 .. t1 - 1 of `tiles`
     int32_t keys;
-    uint64_t base;                                 // unit of its tile 0
+    uint32_t base;                                 // unit of its tile 0
 };
 struct Walk {
-    uint64_t pos, hi, seq_base;   // seq_base: first unit of sequence `seq`
-    uint32_t seq;
+    uint32_t pos, hi, seq_base, seq;               // seq_base: first unit of sequence `seq`
     bool fresh;
 };
 // The next piece; p keeps the state between calls.
@@ -99,8 +55,8 @@ __device__ __forceinline__ bool next_piece(const PagedAttnArgs &a, Walk &w, Piec
         p.q = paged_seq(a, p.seq, bad);
         p.rows = rows_of(a, p.q);
         p.tiles = tiles_of(p.q);
-        p.hkv = (uint32_t)((w.pos - w.seq_base) / p.tiles);
-        p.base = w.seq_base + (uint64_t)p.hkv * p.tiles;
+        p.hkv = (w.pos - w.seq_base) / p.tiles;
+        p.base = w.seq_base + p.hkv * p.tiles;
     } else {
         p.base += p.tiles;
         if (++p.hkv == a.n_kv) {
@@ -110,10 +66,261 @@ __device__ __forceinline__ bool next_piece(const PagedAttnArgs &a, Walk &w, Piec
         }
     }
     p.keys = max(0, p.q.past + (int32_t)p.q.n);
-    p.t0 = (uint32_t)(w.pos - p.base);
-    p.t1 = (uint32_t)min((uint64_t)p.tiles, w.hi - p.base);
+    p.t0 = w.pos - p.base;
+    p.t1 = min(p.tiles, w.hi - p.base);
     w.pos += p.t1 - p.t0;
     return true;
+}
+
+template <int D> struct FewSmem {
+    static constexpr uint32_t kHalfStage = kTile * D * 2;                 // K or V of a tile
+    uint8_t ring[kStages][2 * kHalfStage];                                // 1024-byte aligned
+    float o[kWarps * kRowsB * 36];                                        // the warps' contexts, a part at a time; then records' maxima and sums
+    float m[kWarps][kRowsB], l[kWarps][kRowsB];
+    uint32_t unfinite[3][D];                                              // see unfinite_of
+    uint64_t full[kStages];
+    uint64_t sum[kWarps];
+    uint32_t start_seq, start_off, any;
+    Walk walk;                                                            // of the copies (warp 0), which run ahead of the tiles in use
+    Piece piece;
+    uint32_t tile, issued;                                                // its next tile; copies begun
+};
+
+// Values of +inf, -inf and NaN (class 0, 1, 2) among the keys that only part of the rows attend: per class and dimension the
+// first such key. A row that attends keys 0 .. lim is affected by those <= lim.
+__device__ __forceinline__ float unfinite_of(const uint32_t *u, uint32_t dims, uint32_t d, int32_t lim) {
+    const int32_t p = (int32_t)u[d], n = (int32_t)u[dims + d], x = (int32_t)u[2 * dims + d];   // (0x7fffffff: none)
+    if (x <= lim || (p <= lim && n <= lim)) return __int_as_float(0x7fffffff);
+    return p <= lim ? INFINITY : n <= lim ? -INFINITY : 0.f;
+}
+
+__device__ __forceinline__ void prefetch_map(const CUtensorMap *m) { asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory"); }
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// D(16 x 8, f32) += A(16 x 16) B(16 x 8)
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// D = A B
+__device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ uint32_t half2_bits(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+// Part 0 or 1 of (a, b) as two f16 pairs hi + lo
+__device__ __forceinline__ uint32_t part2(float a, float b, uint32_t part) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    return part ? half2_bits(a - f.x, b - f.y) : *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ void put(const PagedAttnArgs &a, uint64_t to, const float4 &v) {
+    if (a.half) *reinterpret_cast<uint2 *>((__half *)a.out + to) = make_uint2(half2_bits(v.x, v.y), half2_bits(v.z, v.w));
+    else *reinterpret_cast<float4 *>((float *)a.out + to) = v;
+}
+__device__ __forceinline__ void put_lse(const PagedAttnArgs &a, uint64_t tok, uint32_t head, float mx, float s) {
+    a.lse[tok * a.n_kv * a.group + head] = make_float2(mx * 0.693147180559945309f, s * 0.000244140625f);   // 2^-kShift
+}
+// 2^(m - top); 0 for a maximum of nothing beside one of something
+__device__ __forceinline__ float weight(float m, float top) { return m == -INFINITY && top != -INFINITY ? 0.f : exp2_fast(top == -INFINITY ? 0.f : m - top); }
+
+// Copies the next tile of the share, if there is one, into its slot, which is free (a warp: lane i part i of the tile, one page's or less).
+// The page was looked up a call ahead; returns the next one's. Out of line: its registers are not the loop's.
+template <int D>
+__device__ __noinline__ int32_t copy_tile(const PagedAttnArgs &a, FewSmem<D> &sm, int32_t page) {
+    constexpr uint32_t kKV = FewSmem<D>::kHalfStage;
+    const uint32_t lane = threadIdx.x & 31u, shift = min(a.page_shift, 6u), box = 1u << shift, boxes = kTile >> shift;
+    auto page_at = [&](const Piece &p, uint32_t tile) -> int32_t {   // -1: behind the last key
+        const uint32_t key = tile * kTile + (lane << shift);
+        return lane < boxes && key < (uint32_t)p.keys ? a.table[(uint64_t)p.seq * a.max_blocks + (key >> a.page_shift)] : -1;
+    };
+    uint32_t tile = sm.tile;
+    if (tile == sm.piece.t1) {
+        Walk w = sm.walk;
+        Piece p = sm.piece;
+        const bool more = next_piece(a, w, p);
+        __syncwarp();
+        if (!more) return page;
+        if (lane == 0) { sm.walk = w; sm.piece = p; }
+        tile = p.t0;
+        page = page_at(p, tile);
+        __syncwarp();
+    }
+    const Piece &p = sm.piece;
+    const uint32_t page_groups = (1u << a.page_shift) >> 3, key = tile * kTile + (lane << shift), issued = sm.issued, stage = issued % kStages;
+    uint32_t at = a.n_pages * a.n_kv * page_groups;   // behind the pool: copies from there bring zeros
+    if (lane < boxes && key < (uint32_t)p.keys) {
+        if ((uint32_t)page < a.n_pages) at = ((uint32_t)page * a.n_kv + p.hkv) * page_groups + ((key & ((1u << a.page_shift) - 1u)) >> 3);
+        else atomicCAS(a.status, ST_OK, ST_PAGED_PAGE);
+    }
+    if (lane == 0) mbar_arrive_expect_tx(&sm.full[stage], 2 * kKV);
+    __syncwarp();
+    if (lane < boxes) {
+        const uint32_t dst = smem_u32(sm.ring[stage]) + lane * box * D * 2, bar = smem_u32(&sm.full[stage]);
+        asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %2, %2, %3}], [%4];" ::"r"(dst),
+                     "l"(&a.kmap), "r"(0u), "r"(at), "r"(bar) : "memory");
+        asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %2, %2, %3}], [%4];" ::"r"(dst + kKV),
+                     "l"(&a.vmap), "r"(0u), "r"(at), "r"(bar) : "memory");
+    }
+    if (tile + 1 < p.t1) page = page_at(p, tile + 1);
+    __syncwarp();
+    if (lane == 0) { sm.tile = tile + 1; sm.issued = issued + 1; }
+    __syncwarp();
+    return page;
+}
+
+// The records of a sequence over one KV head, added in order: of CTA c0 the piece at its end (or its first), of the others the one at
+// their start. (max, sum) of as many as there is room for at a time to shared memory, then the contexts, kFlight loads of a thread in
+// flight: the launch's tail is a chain of round trips to L2. Out of line: its registers are not the loop's.
+template <int D>
+__device__ __noinline__ void combine(const PagedAttnArgs &a, FewSmem<D> &sm, const PagedSeq q, uint32_t hkv, uint32_t rows, uint32_t c0, uint32_t pieces, bool c0_first) {
+    constexpr uint32_t kFlight = 10, kRecord = kRowsB * (D + 4);
+    const uint32_t tid = threadIdx.x, items = rows * (D / 4), most = (uint32_t)(sizeof(sm.o) / sizeof(float2)) / rows;
+    const float *base = a.part + (uint64_t)c0 * 2 * kRecord;
+    auto record = [&](uint32_t i) { return base + (2 * i + (i || c0_first ? 0 : 1)) * kRecord; };
+    float2 *ml_s = reinterpret_cast<float2 *>(sm.o);
+    for (uint32_t i0 = 0; i0 < items; i0 += kThreads) {
+        const uint32_t i = i0 + tid, rw = i < items ? i / (D / 4) : rows - 1, d = i % (D / 4) * 4, at = rw * (D + 4) + d;
+        float mx = -INFINITY, s = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (uint32_t k0 = 0; k0 < pieces; k0 += most) {
+            const uint32_t nk = min(most, pieces - k0);
+            if (i0 == 0 || pieces > most) {
+                __syncthreads();
+                for (uint32_t e = tid; e < nk * rows; e += kThreads) ml_s[e] = __ldcg(reinterpret_cast<const float2 *>(record(k0 + e / rows) + e % rows * (D + 4) + D));
+                __syncthreads();
+            }
+            float top = mx;
+            for (uint32_t k = 0; k < nk; ++k) top = fmaxf(top, ml_s[k * rows + rw].x);
+            const float w0 = weight(mx, top);
+            s *= w0; v.x *= w0; v.y *= w0; v.z *= w0; v.w *= w0;
+            mx = top;
+#pragma unroll 1
+            for (uint32_t k = 0; k < nk; k += kFlight) {
+                float4 u[kFlight];
+#pragma unroll
+                for (uint32_t j = 0; j < kFlight; ++j)
+                    if (k + j < nk) u[j] = __ldcg(reinterpret_cast<const float4 *>(record(k0 + k + j) + at));
+#pragma unroll
+                for (uint32_t j = 0; j < kFlight; ++j) {
+                    if (k + j >= nk) break;
+                    const float2 ml = ml_s[(k + j) * rows + rw];
+                    const float w = weight(ml.x, top);
+                    s = fmaf(ml.y, w, s);
+                    v.x = fmaf(u[j].x, w, v.x); v.y = fmaf(u[j].y, w, v.y); v.z = fmaf(u[j].z, w, v.z); v.w = fmaf(u[j].w, w, v.w);
+                }
+            }
+        }
+        if (i >= items) continue;
+        const uint32_t tk = rw / a.group, hd = hkv * a.group + rw - tk * a.group;
+        const float inv = q.past + (int32_t)tk < 0 ? 0.f : 1.f / s;
+        put(a, (q.first + tk) * a.out_stride + (uint64_t)hd * D + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+        if (a.lse && d == 0) put_lse(a, q.first + tk, hd, mx, s);
+    }
+}
+
+// The rows of a piece as the threads hold them: blocks of 4, lane (g, t) row t.
+template <int D> struct Rows {
+    uint32_t q[kBlocks][D / 16][2];        // operand: column g = row g / 2, part g & 1; dimensions 2t, 2t + 1, 2t + 8, 2t + 9 of every 16
+    float o[kBlocks][D / 16][2];           // contexts: dimensions g and g + 8 of every 16
+    float f[kBlocks], m[kBlocks], l[kBlocks];   // score -> exponent of 2; maximum, sum
+    int32_t lim[kBlocks];                  // last key
+};
+
+// A warp's 16 keys (from key k0) against N blocks of rows.
+template <int D, int N>
+__device__ __forceinline__ void tile_step(Rows<D> &w, uint32_t k_s, uint32_t v_s, int32_t k0) {
+    constexpr uint32_t kGroupBytes = 8 * D * 2;
+    const uint32_t lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u, mi = lane >> 3, r8 = lane & 7u;
+    float sc[N][4];
+#pragma unroll
+    for (int kb = 0; kb < D / 16; ++kb) {
+        uint32_t ka[4];
+        ldsm4(k_s + (mi & 1u) * kGroupBytes + (kb >> 2) * 1024 + r8 * 128 + (((2 * (kb & 3) + (mi >> 1)) ^ r8) << 4), ka);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            if (kb == 0) mma_first(sc[n], ka, w.q[n][kb][0], w.q[n][kb][1]);
+            else mma(sc[n], ka, w.q[n][kb][0], w.q[n][kb][1]);
+        }
+    }
+    float al[N];
+    uint32_t pb[N][2];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const float s0 = k0 + (int32_t)g <= w.lim[n] ? sc[n][0] + sc[n][1] : -INFINITY, s1 = k0 + 8 + (int32_t)g <= w.lim[n] ? sc[n][2] + sc[n][3] : -INFINITY;
+        float top = fmaxf(s0, s1);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+        const float mn = fmaxf(w.m[n], top * w.f[n]), ref = (mn == -INFINITY ? 0.f : mn) - kShift;
+        al[n] = exp2_fast(w.m[n] - kShift - ref);
+        w.m[n] = mn;
+        const float p0 = exp2_fast(fmaf(s0, w.f[n], -ref)), p1 = exp2_fast(fmaf(s1, w.f[n], -ref));
+        w.l[n] = fmaf(w.l[n], al[n], p0 + p1);   // (this lane's keys)
+        // operand: column g = row g / 2, part g & 1; keys 2t, 2t + 1, 2t + 8, 2t + 9
+        const uint32_t src = 8 * t + (g >> 1);
+        const float a0 = __shfl_sync(0xffffffffu, p0, src), b0 = __shfl_sync(0xffffffffu, p0, src + 4);
+        const float a1 = __shfl_sync(0xffffffffu, p1, src), b1 = __shfl_sync(0xffffffffu, p1, src + 4);
+        pb[n][0] = part2(a0, b0, g & 1u);
+        pb[n][1] = part2(a1, b1, g & 1u);
+    }
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) {
+        uint32_t va[4];
+        ldsm4t(v_s + (mi >> 1) * kGroupBytes + (dt >> 2) * 1024 + r8 * 128 + (((2 * (dt & 3) + (mi & 1u)) ^ r8) << 4), va);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            float d[4];
+            mma_first(d, va, pb[n][0], pb[n][1]);
+            w.o[n][dt][0] = fmaf(w.o[n][dt][0], al[n], d[0] + d[1]);
+            w.o[n][dt][1] = fmaf(w.o[n][dt][1], al[n], d[2] + d[3]);
+        }
+    }
+}
+
+// q of a piece's rows, the factors of their scores, their last keys.
+template <int D>
+__device__ __forceinline__ void load_rows(const PagedAttnArgs &a, const Piece &p, Rows<D> &w) {
+    const uint32_t lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
+#pragma unroll
+    for (uint32_t n = 0; n < kBlocks; ++n) {
+        if (n * 4 >= p.rows) break;
+        const uint32_t row = n * 4 + (g >> 1), tok = row / a.group, head = p.hkv * a.group + row - tok * a.group;
+        const bool there = row < p.rows;
+        const uint64_t src = there ? (p.q.first + tok) * a.q_stride + (uint64_t)head * D : 0;
+        float2 x[D / 8];
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) {
+            if (a.half) x[j] = __half22float2(*reinterpret_cast<const __half2 *>((const __half *)a.q + src + 8 * j + 2 * t));
+            else x[j] = *reinterpret_cast<const float2 *>((const float *)a.q + src + 8 * j + 2 * t);
+        }
+        float top = 0.f;
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) top = fmaxf(top, fmaxf(fabsf(x[j].x), fabsf(x[j].y)));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // a power of two brings the row's largest value to [2^11, 2^12)
+        const int e = min(100, max(-100, 138 - (int)(__float_as_uint(top) >> 23)));
+        const float up = __uint_as_float((uint32_t)(e + 127) << 23);
+        w.f[n] = __shfl_sync(0xffffffffu, fmaxf(a.scale * 1.44269504088896341f * __uint_as_float((uint32_t)(127 - e) << 23), 1e-37f), 8 * t);
+#pragma unroll
+        for (int kb = 0; kb < D / 16; ++kb)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) w.q[n][kb][j] = part2(x[2 * kb + j].x * up, x[2 * kb + j].y * up, g & 1u);
+        const uint32_t mine = n * 4 + t;
+        w.lim[n] = mine < p.rows ? p.q.past + (int32_t)(mine / a.group) : -1;
+        w.m[n] = -INFINITY;
+        w.l[n] = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt) w.o[n][dt][0] = w.o[n][dt][1] = 0.f;
+    }
 }
 
 template <int D>
@@ -123,154 +330,94 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
     constexpr uint32_t kKV = FewSmem<D>::kHalfStage, kGroupBytes = 8 * D * 2;
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, g = lane >> 2, t = lane & 3u;
     if (tid == 0) {
-        for (uint32_t s = 0; s < kStages; ++s) { mbar_init(&sm.full[s], 1); mbar_init(&sm.empty[s], kWarps); }
+        prefetch_map(&a.kmap);
+        prefetch_map(&a.vmap);
+        for (uint32_t s = 0; s < kStages; ++s) mbar_init(&sm.full[s], 1);
+        sm.issued = 0;
         fence_barrier_init();
     }
     for (uint32_t i = tid; i < 3 * D; i += kThreads) (&sm.unfinite[0][0])[i] = 0x7fffffffu;
+    __syncthreads();
     griddep_wait();
 
-    // ---- this CTA's share of the line ----
+    // ---- this CTA's share of the line: every warp by itself for up to 32 sequences ----
+    Shares sh;
+    uint32_t start_off, start_seq;
     {
-        const uint32_t per = (a.n_seq + kThreads - 1) / kThreads, s0 = min(tid * per, a.n_seq), s1 = min(s0 + per, a.n_seq);
+        const bool one_warp = a.n_seq <= 32;
+        const uint32_t threads = one_warp ? 32 : kThreads, i = one_warp ? lane : tid;
+        const uint32_t per = (a.n_seq + threads - 1) / threads, s0 = min(i * per, a.n_seq), s1 = min(s0 + per, a.n_seq);
         uint64_t mine = 0;
         bool bad = false, any_bad = false;
         for (uint32_t s = s0; s < s1; ++s) {
             mine += units_of(a, paged_seq(a, s, bad));
             any_bad |= bad;
         }
-        if (any_bad && blockIdx.x == 0) atomicCAS(a.status, ST_OK, ST_PAGED_ARGS);
         uint64_t x = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint64_t u = __shfl_up_sync(0xffffffffu, x, o);
             if (lane >= (uint32_t)o) x += u;
         }
-        if (lane == 31) sm.sum[warp] = x;
-        __syncthreads();
-        uint64_t total = 0;
-        for (uint32_t w = 0; w < kThreads / 32; ++w) {
-            if (w < warp) x += sm.sum[w];
-            total += sm.sum[w];
+        uint64_t total = __shfl_sync(0xffffffffu, x, 31);
+        if (!one_warp) {
+            if (lane == 31) sm.sum[warp] = x;
+            __syncthreads();
+            total = 0;
+            for (uint32_t w = 0; w < kWarps; ++w) {
+                if (w < warp) x += sm.sum[w];
+                total += sm.sum[w];
+            }
         }
+        if ((any_bad || total >> 32) && blockIdx.x == 0) atomicCAS(a.status, ST_OK, ST_PAGED_ARGS);
         x -= mine;
-        const uint32_t ctas = (uint32_t)min((uint64_t)gridDim.x, total);
-        if (blockIdx.x >= ctas) return;   // (no share is empty: the CTAs of a block's records are consecutive)
-        const uint64_t lo = share_of(total, ctas, blockIdx.x);
-        if (tid == 0) sm.total = total;
-        if (lo >= x && lo < x + mine) {
-            uint32_t s = s0;
+        sh = shares_of(total >> 32 ? 0u : (uint32_t)total, gridDim.x);
+        if (blockIdx.x >= sh.n) return;
+        const uint32_t lo = share_lo(sh, blockIdx.x);
+        const bool here = lo >= x && lo < x + mine;
+        uint32_t s = s0;
+        if (here)
             for (;; ++s) {
                 const uint64_t u = units_of(a, paged_seq(a, s, bad));
                 if (lo < x + u) break;
                 x += u;
             }
-            sm.start_seq = s;
-            sm.start_off = x;
+        if (one_warp) {
+            const int src = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+            start_seq = __shfl_sync(0xffffffffu, s, src);
+            start_off = __shfl_sync(0xffffffffu, (uint32_t)x, src);
+        } else {
+            if (here) { sm.start_seq = s; sm.start_off = (uint32_t)x; }
+            __syncthreads();
+            start_seq = sm.start_seq;
+            start_off = sm.start_off;
         }
-        __syncthreads();
     }
-    const uint64_t total = sm.total;
-    const uint32_t ctas = (uint32_t)min((uint64_t)gridDim.x, total);
-    Walk walk{share_of(total, ctas, blockIdx.x), share_of(total, ctas, blockIdx.x + 1), sm.start_off, sm.start_seq, true};
+    Walk walk{share_lo(sh, blockIdx.x), share_lo(sh, blockIdx.x + 1), start_off, start_seq, true};
     Piece p;
-    uint32_t stage = 0, parity = 0;   // of the ring
-
-    if (warp == kWarps) {
-        // ---- producer ----
-        const uint32_t box = min(1u << a.page_shift, kTile), boxes = kTile / box, bytes = box * D * 2;
-        const uint32_t page_groups = (1u << a.page_shift) >> 3, outside = a.n_pages * a.n_kv * page_groups;
-        while (next_piece(a, walk, p)) {
-            const int32_t *row = a.table + (uint64_t)p.seq * a.max_blocks;
-            auto page_at = [&](uint32_t tile) -> int32_t {   // the page that this lane's part of the tile lies on; -1: behind the last key
-                const uint32_t key = tile * kTile + lane * box;
-                return lane < boxes && key < (uint32_t)p.keys ? row[key >> a.page_shift] : -1;
-            };
-            int32_t page = page_at(p.t0);
-            for (uint32_t tile = p.t0; tile < p.t1; ++tile) {
-                const uint32_t key = tile * kTile + lane * box;
-                uint32_t at = outside;   // copies from there bring zeros
-                if (lane < boxes && key < (uint32_t)p.keys) {
-                    if ((uint32_t)page < a.n_pages)
-                        at = ((uint32_t)page * a.n_kv + p.hkv) * page_groups + ((key & ((1u << a.page_shift) - 1u)) >> 3);
-                    else
-                        atomicCAS(a.status, ST_OK, ST_PAGED_PAGE);
-                }
-                if (tile + 1 < p.t1) page = page_at(tile + 1);
-                if (!mbar_wait_bounded(&sm.empty[stage], parity ^ 1u, a.status)) return;
-                if (lane == 0) mbar_arrive_expect_tx(&sm.full[stage], 2 * kKV);
-                __syncwarp();
-                if (lane < boxes) {
-                    const uint32_t dst = smem_u32(sm.ring[stage]) + lane * bytes, bar = smem_u32(&sm.full[stage]);
-                    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %2, %2, %3}], [%4];" ::"r"(dst),
-                                 "l"(&a.kmap), "r"(0u), "r"(at), "r"(bar) : "memory");
-                    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %2, %2, %3}], [%4];" ::"r"(dst + kKV),
-                                 "l"(&a.vmap), "r"(0u), "r"(at), "r"(bar) : "memory");
-                }
-                if (++stage == kStages) { stage = 0; parity ^= 1u; }
-            }
-        }
-        griddep_launch_dependents();
-        return;
+    int32_t page = -1;                // of the next copy (this lane's part of it)
+    if (warp == 0) {
+        if (lane == 0) { sm.walk = walk; sm.piece.t1 = 0; sm.tile = 0; }
+        __syncwarp();
+#pragma unroll 1
+        for (uint32_t i = 0; i < kStages; ++i) page = copy_tile<D>(a, sm, page);
     }
 
-    // ---- consumers ----
+    uint32_t stage = 0, parity = 0;   // of the ring
     bool first = true;
     while (next_piece(a, walk, p)) {
-        // q: rows g and g + 8, dimensions 2t, 2t + 1 of every 8
-        uint32_t qh[D / 16][4], ql[D / 16][4];
-        float f[2];        // score -> exponent of 2, per row
-        int32_t lim[2];    // last key of a row
-        {
-            float x[2][D / 4];
-            bool there[2];
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const uint32_t row = g + 8 * r, tok = row / a.group, head = p.hkv * a.group + row - tok * a.group;
-                there[r] = row < p.rows;
-                lim[r] = there[r] ? p.q.past + (int32_t)tok : -1;
-                const uint64_t src = there[r] ? (p.q.first + tok) * a.q_stride + (uint64_t)head * D : 0;
-#pragma unroll
-                for (int j = 0; j < D / 8; ++j) {
-                    float2 v = make_float2(0.f, 0.f);
-                    if (there[r]) {
-                        if (a.half) v = __half22float2(*reinterpret_cast<const __half2 *>((const __half *)a.q + src + 8 * j + 2 * t));
-                        else v = *reinterpret_cast<const float2 *>((const float *)a.q + src + 8 * j + 2 * t);
-                    }
-                    x[r][2 * j] = v.x; x[r][2 * j + 1] = v.y;
-                }
-                float top = 0.f;
-#pragma unroll
-                for (int j = 0; j < D / 4; ++j) top = fmaxf(top, fabsf(x[r][j]));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                // a power of two brings the row's largest value to [2^11, 2^12)
-                const int e = min(100, max(-100, 138 - (int)(__float_as_uint(top) >> 23)));
-                const float up = __uint_as_float((uint32_t)(e + 127) << 23);
-                f[r] = a.scale * 1.44269504088896341f * __uint_as_float((uint32_t)(127 - e) << 23);
-#pragma unroll
-                for (int j = 0; j < D / 4; ++j) x[r][j] *= up;
-            }
-#pragma unroll
-            for (int kb = 0; kb < D / 16; ++kb)
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    split2(x[r][4 * kb], x[r][4 * kb + 1], qh[kb][r], ql[kb][r]);
-                    split2(x[r][4 * kb + 2], x[r][4 * kb + 3], qh[kb][2 + r], ql[kb][2 + r]);
-                }
-        }
+        Rows<D> w;
+        load_rows<D>(a, p, w);
         const int32_t lim_first = p.q.past;   // last key that all rows attend
-        float o[D / 8][4];
-#pragma unroll
-        for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-
+#pragma unroll 1
         for (uint32_t tile = p.t0; tile < p.t1; ++tile) {
-            if (!mbar_wait_bounded(&sm.full[stage], parity, a.status)) return;
+            const bool landed = mbar_wait_bounded(&sm.full[stage], parity, a.status);
             const int32_t k0 = (int32_t)(tile * kTile + warp * 16);
-            if (k0 < p.keys) {
-                const uint32_t kb_s = smem_u32(sm.ring[stage]) + warp * 2 * kGroupBytes, vb_s = kb_s + kKV;
+            if (landed && k0 < p.keys) {
+                const uint32_t k_s = smem_u32(sm.ring[stage]) + warp * 2 * kGroupBytes, v_s = k_s + kKV;
                 if (k0 + 16 > lim_first + 1 || k0 + 16 > p.keys) {
                     uint8_t *vrow = sm.ring[stage] + kKV + warp * 2 * kGroupBytes;
+#pragma unroll 1
                     for (uint32_t i = lane; i < 16 * D / 8; i += 32) {
                         const uint32_t r = i / (D / 8), c = i % (D / 8);
                         const int32_t key = k0 + (int32_t)r;
@@ -278,11 +425,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
                         if (key >= p.keys) {
                             *at = make_uint4(0, 0, 0, 0);
                         } else if (key > lim_first) {
-                            uint4 v = *at;
-                            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-                            uint32_t z = 0;
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) z |= (w[j] & 0x7C007C00u) + 0x04000400u;
+                            const uint4 x = *at;
+                            const uint32_t z = ((x.x & 0x7C007C00u) + 0x04000400u) | ((x.y & 0x7C007C00u) + 0x04000400u) | ((x.z & 0x7C007C00u) + 0x04000400u) | ((x.w & 0x7C007C00u) + 0x04000400u);
                             if (z & 0x80008000u) {   // an exponent of all ones
                                 __half *h = reinterpret_cast<__half *>(at);
                                 for (uint32_t j = 0; j < 8; ++j) {
@@ -298,178 +442,104 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
                     fence_proxy_async_smem();   // (the next copy into this stage comes after these writes)
                     __syncwarp();
                 }
-                // ---- scores ----
-                float sh[2][4], sl[2][4];
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) sh[n][i] = sl[n][i] = 0.f;
-                const uint32_t mi = lane >> 3, r8 = lane & 7u;
-#pragma unroll
-                for (int kb = 0; kb < D / 16; ++kb) {
-                    uint32_t b[4];
-                    ldsm4(kb_s + (mi >> 1) * kGroupBytes + (kb >> 2) * 1024 + r8 * 128 + (((2 * (kb & 3) + (mi & 1u)) ^ r8) << 4), b);
-                    mma(sh[0], qh[kb], b[0], b[1]);
-                    mma(sh[1], qh[kb], b[2], b[3]);
-                    mma(sl[0], ql[kb], b[0], b[1]);
-                    mma(sl[1], ql[kb], b[2], b[3]);
-                }
-                // ---- softmax: value 2 r + i of n: row g + 8 r, key 8 n + 2 t + i ----
-                float al[2];
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    float x[4];
-#pragma unroll
-                    for (int n = 0; n < 2; ++n)
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const float s = sh[n][2 * r + i] + sl[n][2 * r + i];
-                            x[2 * n + i] = k0 + 8 * n + (int32_t)(2 * t) + i <= lim[r] ? s : -INFINITY;
-                        }
-                    float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    const float mn = fmaxf(m[r], top * f[r]), ref = (mn == -INFINITY ? 0.f : mn) - kShift;
-                    al[r] = exp2_fast(m[r] - kShift - ref);
-                    m[r] = mn;
-                    float sum = 0.f;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float e = exp2_fast(fmaf(x[j], f[r], -ref));
-                        sum += e;
-                        sh[j >> 1][2 * r + (j & 1)] = e;
-                    }
-                    l[r] = fmaf(l[r], al[r], sum);
-                }
-                uint32_t ph[4], pl[4];
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) split2(sh[n][2 * r], sh[n][2 * r + 1], ph[2 * n + r], pl[2 * n + r]);
-                // ---- context ----
-#pragma unroll
-                for (int j = 0; j < D / 16; ++j) {
-                    uint32_t b[4];
-                    ldsm4t(vb_s + (mi & 1u) * kGroupBytes + (j >> 2) * 1024 + r8 * 128 + (((2 * (j & 3) + (mi >> 1)) ^ r8) << 4), b);
-#pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        float d[4] = {0.f, 0.f, 0.f, 0.f};
-                        mma(d, pl, b[2 * n], b[2 * n + 1]);
-                        mma(d, ph, b[2 * n], b[2 * n + 1]);
-                        float (&w)[4] = o[2 * j + n];
-                        w[0] = fmaf(w[0], al[0], d[0]); w[1] = fmaf(w[1], al[0], d[1]);
-                        w[2] = fmaf(w[2], al[1], d[2]); w[3] = fmaf(w[3], al[1], d[3]);
-                    }
-                }
+                if (p.rows <= 4) tile_step<D, 1>(w, k_s, v_s, k0);
+                else if (p.rows <= 8) tile_step<D, 2>(w, k_s, v_s, k0);
+                else tile_step<D, 4>(w, k_s, v_s, k0);
             }
-            __syncwarp();
-            if (lane == 0) arrive(&sm.empty[stage]);
+            if (!__syncthreads_and(landed)) {   // (the tile is used up, or all give up, with no copy in flight)
+                if (tid == 0)
+                    for (uint32_t i = sm.issued - min(sm.issued, kStages); i < sm.issued; ++i) mbar_wait_bounded(&sm.full[i % kStages], i / kStages & 1u, a.status);
+                __syncthreads();
+                return;
+            }
+            if (warp == 0) page = copy_tile<D>(a, sm, page);
             if (++stage == kStages) { stage = 0; parity ^= 1u; }
         }
 
         // ---- the warps' sums, a part of the dimensions at a time ----
-        const uint32_t c0 = owner_of(total, ctas, p.base), c1 = owner_of(total, ctas, p.base + p.tiles - 1), pieces = c1 - c0 + 1;
+        const uint32_t c0 = owner_of(sh, p.base), pieces = owner_of(sh, p.base + p.tiles - 1) - c0 + 1;
         const bool whole = pieces == 1;
         float *rec = a.part + (uint64_t)(blockIdx.x * 2 + (first ? 0 : 1)) * kRowsB * (D + 4);
         first = false;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-            if (t == 0) { sm.m[warp][g + 8 * r] = m[r]; sm.l[warp][g + 8 * r] = l[r]; }
+        for (uint32_t n = 0; n < kBlocks; ++n) {
+            if (n * 4 >= p.rows) break;
+            w.l[n] += __shfl_xor_sync(0xffffffffu, w.l[n], 4);
+            w.l[n] += __shfl_xor_sync(0xffffffffu, w.l[n], 8);
+            w.l[n] += __shfl_xor_sync(0xffffffffu, w.l[n], 16);
+            if (g == 0) { sm.m[warp][n * 4 + t] = w.m[n]; sm.l[warp][n * 4 + t] = w.l[n]; }
         }
-        bar_consumers();
-        float wgt[2];   // this warp's weight, rows g, g + 8
+        __syncthreads();
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
+        for (uint32_t n = 0; n < kBlocks; ++n) {   // contexts relative to the largest maximum
+            if (n * 4 >= p.rows) break;
             float top = -INFINITY;
 #pragma unroll
-            for (uint32_t w = 0; w < kWarps; ++w) top = fmaxf(top, sm.m[w][g + 8 * r]);
-            wgt[r] = m[r] == -INFINITY && top != -INFINITY ? 0.f : exp2_fast(top == -INFINITY ? 0.f : m[r] - top);
+            for (uint32_t x = 0; x < kWarps; ++x) top = fmaxf(top, sm.m[x][n * 4 + t]);
+            const float by = weight(w.m[n], top);
+#pragma unroll
+            for (int dt = 0; dt < D / 16; ++dt) { w.o[n][dt][0] *= by; w.o[n][dt][1] *= by; }
         }
-        const uint32_t row = tid >> 3, c4 = (tid & 7u) * 4;   // the thread's row and 4 of a part's 32 dimensions
-        float top = -INFINITY, sum = 0.f;
-#pragma unroll
-        for (uint32_t w = 0; w < kWarps; ++w) top = fmaxf(top, sm.m[w][row]);
-#pragma unroll
-        for (uint32_t w = 0; w < kWarps; ++w) sum = fmaf(sm.l[w][row], sm.m[w][row] == -INFINITY && top != -INFINITY ? 0.f : exp2_fast(top == -INFINITY ? 0.f : sm.m[w][row] - top), sum);
+        // parts of `wide` dimensions: few rows, wide parts (row_bits: 2, 3, 4 for 4, 8, 16 rows); the thread's row and 4 dimensions of a part
+        const uint32_t row_bits = p.rows <= 4 && D == 128 ? 2 : p.rows <= 8 ? 3 : 4, wide = 512u >> row_bits, pitch = wide + 4;
+        const uint32_t row = tid >> (7 - row_bits), c4 = (tid & ((wide >> 2) - 1u)) * 4;
         const uint32_t tok = row / a.group, head = p.hkv * a.group + row - tok * a.group;
         const int32_t row_lim = p.q.past + (int32_t)tok;
         const uint64_t dst = (p.q.first + tok) * a.out_stride + (uint64_t)head * D;
-        auto put = [&](uint64_t to, const float4 &v) {
-            if (a.half) *reinterpret_cast<uint2 *>((__half *)a.out + to) = make_uint2(half2_bits(v.x, v.y), half2_bits(v.z, v.w));
-            else *reinterpret_cast<float4 *>((float *)a.out + to) = v;
-        };
-        auto put_lse = [&](uint32_t tk, uint32_t hd, float mx, float s) {
-            a.lse[(uint64_t)(p.q.first + tk) * a.n_kv * a.group + hd] = make_float2(mx * 0.693147180559945309f, s * 0.000244140625f);   // 2^-kShift
-        };
-        for (uint32_t part = 0; part < D / 32; ++part) {
-            if (part) bar_consumers();
+        float top = -INFINITY, sum = 0.f;
+        if (row < p.rows) {
 #pragma unroll
-            for (int j = 0; j < D / 8; ++j)
-                if ((uint32_t)j / 4 == part)
+            for (uint32_t x = 0; x < kWarps; ++x) top = fmaxf(top, sm.m[x][row]);
 #pragma unroll
-                    for (int r = 0; r < 2; ++r)
-                        *reinterpret_cast<float2 *>(&sm.o[warp][g + 8 * r][(j & 3) * 8 + 2 * t]) = make_float2(o[j][2 * r] * wgt[r], o[j][2 * r + 1] * wgt[r]);
-            bar_consumers();
+            for (uint32_t x = 0; x < kWarps; ++x) sum = fmaf(sm.l[x][row], weight(sm.m[x][row], top), sum);
+        }
+#pragma unroll 1
+        for (uint32_t d0 = 0; d0 < D; d0 += wide) {
+            if (d0) __syncthreads();
+#pragma unroll
+            for (uint32_t n = 0; n < kBlocks; ++n) {
+                if (n * 4 >= p.rows) break;
+                float *at = sm.o + ((warp << row_bits) + n * 4 + t) * pitch + g;
+#pragma unroll
+                for (int dt = 0; dt < D / 16; ++dt)
+                    if (dt * 16u >= d0 && dt * 16u - d0 < wide) { at[dt * 16u - d0] = w.o[n][dt][0]; at[dt * 16u - d0 + 8] = w.o[n][dt][1]; }
+            }
+            __syncthreads();
             if (row < p.rows) {
                 float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                for (uint32_t w = 0; w < kWarps; ++w) {
-                    const float4 u = *reinterpret_cast<const float4 *>(&sm.o[w][row][c4]);
+                for (uint32_t x = 0; x < kWarps; ++x) {
+                    const float4 u = *reinterpret_cast<const float4 *>(&sm.o[((x << row_bits) + row) * pitch + c4]);
                     v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
                 }
-                const uint32_t d = part * 32 + c4;
+                const uint32_t d = d0 + c4;
                 v.x += unfinite_of(&sm.unfinite[0][0], D, d, row_lim); v.y += unfinite_of(&sm.unfinite[0][0], D, d + 1, row_lim);
                 v.z += unfinite_of(&sm.unfinite[0][0], D, d + 2, row_lim); v.w += unfinite_of(&sm.unfinite[0][0], D, d + 3, row_lim);
                 if (whole) {
                     const float inv = row_lim < 0 ? 0.f : 1.f / sum;
-                    put(dst + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+                    put(a, dst + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
                 } else {
                     __stcg(reinterpret_cast<float4 *>(rec + row * (D + 4) + d), v);
                 }
             }
         }
         if (row < p.rows && c4 == 0) {
-            if (whole) { if (a.lse) put_lse(tok, head, top, sum); }
-            else __stcg(reinterpret_cast<float4 *>(rec + row * (D + 4) + D), make_float4(top, sum, 0.f, 0.f));
+            if (!whole) __stcg(reinterpret_cast<float4 *>(rec + row * (D + 4) + D), make_float4(top, sum, 0.f, 0.f));
+            else if (a.lse) put_lse(a, p.q.first + tok, head, top, sum);
         }
         if (!whole) {
-            __threadfence();
-            bar_consumers();
+            fence_acq_rel_gpu();
+            __syncthreads();
             if (tid == 0) sm.any = atomicAdd(&a.tickets[c0], 1u) == pieces - 1 ? 1u : 0u;
         }
-        bar_consumers();   // (also: everybody has read the unfinite values)
-        for (uint32_t i = tid; i < 3 * D; i += kWarps * 32) (&sm.unfinite[0][0])[i] = 0x7fffffffu;
+        __syncthreads();   // (also: everybody has read the unfinite values)
+        for (uint32_t i = tid; i < 3 * D; i += kThreads) (&sm.unfinite[0][0])[i] = 0x7fffffffu;
         if (!whole && sm.any) {
-            __threadfence();
-            // the records in order: of CTA c0 the piece at its end, of the others the one at their start
-            const bool c0_first = p.base <= share_of(total, ctas, c0);
-            auto record = [&](uint32_t i, uint32_t rw) { return a.part + ((uint64_t)((c0 + i) * 2 + (i || c0_first ? 0 : 1)) * kRowsB + rw) * (D + 4); };
-            for (uint32_t i = tid; i < p.rows * (D / 4); i += kWarps * 32) {
-                const uint32_t rw = i / (D / 4), d = i % (D / 4) * 4;
-                float mx = -INFINITY;
-#pragma unroll 8
-                for (uint32_t k = 0; k < pieces; ++k) mx = fmaxf(mx, __ldcg(record(k, rw) + D));
-                float s = 0.f;
-                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-                for (uint32_t k = 0; k < pieces; ++k) {
-                    const float *rc = record(k, rw);
-                    const float2 ml = __ldcg(reinterpret_cast<const float2 *>(rc + D));
-                    const float4 u = __ldcg(reinterpret_cast<const float4 *>(rc + d));
-                    const float w = ml.x == -INFINITY && mx != -INFINITY ? 0.f : exp2_fast(mx == -INFINITY ? 0.f : ml.x - mx);
-                    s = fmaf(ml.y, w, s);
-                    v.x = fmaf(u.x, w, v.x); v.y = fmaf(u.y, w, v.y); v.z = fmaf(u.z, w, v.z); v.w = fmaf(u.w, w, v.w);
-                }
-                const uint32_t tk = rw / a.group, hd = p.hkv * a.group + rw - tk * a.group;
-                const float inv = p.q.past + (int32_t)tk < 0 ? 0.f : 1.f / s;
-                put((p.q.first + tk) * a.out_stride + (uint64_t)hd * D + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
-                if (a.lse && d == 0) put_lse(tk, hd, mx, s);
-            }
+            fence_acq_rel_gpu();
+            combine<D>(a, sm, p.q, p.hkv, p.rows, c0, pieces, p.base <= share_lo(sh, c0));
             if (tid == 0) a.tickets[c0] = 0;
         }
-        bar_consumers();   // the shared arrays are free for the next piece
+        __syncthreads();   // the shared arrays are free for the next piece
     }
     griddep_launch_dependents();
 }

@@ -49,8 +49,7 @@ struct Job {
     int32_t past;
 };
 struct Walk {
-    uint64_t pos, hi, seq_base;
-    uint32_t seq;
+    uint32_t pos, hi, seq_base, seq;
     bool fresh;
 };
 struct Block { uint32_t rows, tiles; int32_t keys; };
@@ -59,12 +58,11 @@ struct Piece {
     uint32_t seq, hkv, blk, n_blk;
     Block b;
     uint32_t t0, t1;
-    uint64_t base;       // unit of its block's tile 0
+    uint32_t base;       // unit of its block's tile 0
 };
 struct Head {
     uint64_t full[8], empty[8], v_ready[8], s_full[2], p_full[2][2], o_done[2], q_full, drain;
-    uint64_t start_off;
-    uint32_t start_seq, tmem, abort_flag, any_unfinite;
+    uint32_t start_seq, start_off, tmem, abort_flag, any_unfinite;
     Job job;
     Walk walk;
     Piece piece;
@@ -362,18 +360,17 @@ __device__ __forceinline__ bool next_piece(const PagedAttnArgs &a, Walk &w, Piec
         p.n_blk = blocks_of(a, p.q);
         // the KV head, then the block (32 at a time), that hold the share's first unit
         const uint32_t lane = threadIdx.x & 31u;
-        uint64_t per_head = 0;
+        uint32_t per_head = 0;
         for (uint32_t b = lane; b < p.n_blk; b += 32) per_head += block_of(a, p.q, b).tiles;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) per_head += __shfl_xor_sync(0xffffffffu, per_head, o);
-        p.hkv = (uint32_t)((w.pos - w.seq_base) / per_head);
+        per_head = __reduce_add_sync(0xffffffffu, per_head);
+        p.hkv = (w.pos - w.seq_base) / per_head;
         p.base = w.seq_base + p.hkv * per_head;
         for (uint32_t b0 = 0;; b0 += 32) {
-            const uint64_t t = b0 + lane < p.n_blk ? block_of(a, p.q, b0 + lane).tiles : 0u;
-            uint64_t x = t;
+            const uint32_t t = b0 + lane < p.n_blk ? block_of(a, p.q, b0 + lane).tiles : 0u;
+            uint32_t x = t;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const uint64_t y = __shfl_up_sync(0xffffffffu, x, o);
+                const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
                 if (lane >= (uint32_t)o) x += y;
             }
             const uint32_t behind = __ballot_sync(0xffffffffu, p.base + x > w.pos);
@@ -397,8 +394,8 @@ __device__ __forceinline__ bool next_piece(const PagedAttnArgs &a, Walk &w, Piec
         }
         p.b = block_of(a, p.q, p.blk);
     }
-    p.t0 = (uint32_t)(w.pos - p.base);
-    p.t1 = (uint32_t)min((uint64_t)p.b.tiles, w.hi - p.base);
+    p.t0 = w.pos - p.base;
+    p.t1 = min(p.b.tiles, w.hi - p.base);
     w.pos += p.t1 - p.t0;
     return true;
 }
@@ -524,6 +521,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
     uint8_t *q_s = base + T::kHead, *ring = q_s + T::kQ;
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
     if (tid == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&a.kmap) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&a.vmap) : "memory");
         for (uint32_t s = 0; s < T::kSlots; ++s) { mbar_init(&hd.full[s], 1); mbar_init(&hd.empty[s], 1); }
         for (uint32_t s = 0; s < 8; ++s) mbar_init(&hd.v_ready[s], 1);
         for (int l = 0; l < 2; ++l) { mbar_init(&hd.s_full[l], 1); mbar_init(&hd.p_full[l][0], 4); mbar_init(&hd.p_full[l][1], 4); mbar_init(&hd.o_done[l], 1); }
@@ -546,15 +545,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
             any_bad |= bad;
             mine += head_units(a, q, lane) * a.n_kv;
         }
-        if (any_bad && blockIdx.x == 0) atomicCAS(a.status, ST_OK, ST_PAGED_ARGS);
+        if (any_bad) atomicCAS(a.status, ST_OK, ST_PAGED_ARGS);
         for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
         if (lane == 0) hd.sum[warp] = mine;
         __syncthreads();
         for (uint32_t w = 0; w < kThreads / 32; ++w) total += hd.sum[w];
     }
-    const uint32_t ctas = (uint32_t)min((uint64_t)gridDim.x, total);
-    if (blockIdx.x >= ctas) return;
-    const uint64_t lo = share_of(total, ctas, blockIdx.x), hi = share_of(total, ctas, blockIdx.x + 1);
+    if (total >> 32 && tid == 0) atomicCAS(a.status, ST_OK, ST_PAGED_ARGS);
+    const Shares sh = shares_of(total >> 32 ? 0u : (uint32_t)total, gridDim.x);
+    if (blockIdx.x >= sh.n) return;
+    const uint32_t lo = share_lo(sh, blockIdx.x), hi = share_lo(sh, blockIdx.x + 1);
     {
         uint64_t run = 0;
         for (uint32_t s0 = 0; s0 < a.n_seq && run <= lo; s0 += kThreads) {
@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
                 if (w < warp) x += hd.sum[w];
                 run += hd.sum[w];
             }
-            if (lo >= x && lo < x + u) { hd.start_seq = s0 + tid; hd.start_off = x; }
+            if (lo >= x && lo < x + u) { hd.start_seq = s0 + tid; hd.start_off = (uint32_t)x; }
         }
     }
     __syncthreads();
@@ -811,7 +811,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
                     Job &j = hd.job;
                     j.valid = valid;
                     if (valid) {
-                        const uint32_t c0 = owner_of(total, ctas, x.base), c1 = owner_of(total, ctas, x.base + x.b.tiles - 1);
+                        const uint32_t c0 = owner_of(sh, x.base), c1 = owner_of(sh, x.base + x.b.tiles - 1);
                         j.sm = small(x); j.n = x.t1 - x.t0; j.t0 = x.t0;
                         j.first = x.q.first; j.row0 = x.blk * 2 * kRowsL; j.rows = x.b.rows; j.hkv = x.hkv; j.past = x.q.past;
                         j.whole = c0 == c1;

@@ -362,7 +362,10 @@ int fl_b200_paged_append(fl_b200_ctx *c, const fl_b200_paged_cache *cache, int a
     a.q_stride = q_stride; a.kv_stride = kv_stride; a.q_out_stride = q_out_stride;
     a.n_tok = n_tokens; a.n_q = n_q; a.n_kv = cache->n_kv_head; a.dim_shift = dim == 128 ? 7 : 6; a.n_rot = n_rot;
     a.page_shift = (uint32_t)page_shift_of(cache->page_size); a.n_pages = cache->n_pages;
-    for (uint32_t i = 0; i < n_rot / 2; ++i) a.turns[i] = std::pow((double)freq_base, -2.0 * i / n_rot) / 6.283185307179586476925;
+    // (a product more per pair: 64 roundings of 2^-53 at most)
+    const double ratio = n_rot ? std::pow((double)freq_base, -2.0 / n_rot) : 0.0;
+    double turn = 1.0 / 6.283185307179586476925;
+    for (uint32_t i = 0; i < n_rot / 2; ++i, turn *= ratio) a.turns[i] = turn;
     a.tokens = std::max(1u, std::min(4u, n_tokens / (4u * (uint32_t)c->sms)));
     const uint32_t ctas = (n_tokens + a.tokens - 1) / a.tokens, per_tok = (n_q + 2 * a.n_kv) * dim / (act == FL_B200_ACT_F16 ? 8 : 4);
     // few tokens: their heads over several CTAs

@@ -57,9 +57,17 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedAttnArgs &a, uint32_t s
     bad = b < 0 || e < b || (uint32_t)e > a.n_tokens || (uint32_t)(e - b) > a.max_new || len < 0 || (uint64_t)len > room;
     return bad ? PagedSeq{0, 0, 0} : PagedSeq{(uint32_t)b, (uint32_t)(e - b), len - (e - b)};
 }
-__device__ __forceinline__ uint64_t share_of(uint64_t units, uint32_t grid, uint32_t c) { return units * c / grid; }
-// The CTA whose share holds unit u.
-__device__ __forceinline__ uint32_t owner_of(uint64_t units, uint32_t grid, uint64_t u) { return (uint32_t)(((u + 1) * grid - 1) / units); }
+// The line's units over n CTAs, equal shares up to one unit; none is empty (n <= units). 32 bits: a call with 2^32 units or more is refused.
+struct Shares { uint32_t n, each, more; };   // the first `more` CTAs have one unit more than `each`
+__device__ __forceinline__ Shares shares_of(uint32_t units, uint32_t ctas) {
+    const uint32_t n = min(ctas, units);
+    return n ? Shares{n, units / n, units % n} : Shares{0, 0, 0};
+}
+__device__ __forceinline__ uint32_t share_lo(const Shares &s, uint32_t c) { return s.each * c + min(c, s.more); }
+__device__ __forceinline__ uint32_t owner_of(const Shares &s, uint32_t u) {   // the CTA whose share holds unit u
+    const uint32_t front = s.more * (s.each + 1);
+    return u < front ? u / (s.each + 1) : s.more + (u - front) / s.each;
+}
 
 __device__ __forceinline__ float exp2_fast(float x) {   // 2^x to 2^-22 of its value, 0 for -inf
     float r;

@@ -12,8 +12,9 @@ from . import capi
 
 F32, F16 = 0, 1
 _ACT = {torch.float32: F32, torch.float16: F16}
+_I32 = torch.int32
 _u32, _p = C.c_uint32, C.c_void_p
-_signed = set()
+_found = {}
 
 
 class PagedCacheP(C.Structure):
@@ -29,38 +30,37 @@ _ARGS = {
 
 
 def _entry(lib, name):
-    f = getattr(lib, name)
-    if name not in _signed:
+    f = _found.get(name)
+    if f is None:
+        f = getattr(lib, name)
         f.argtypes = _ARGS[name]
-        _signed.add(name)
+        _found[name] = f
     return f
 
 
-def _ints(ctx, name, t, shape):
-    """Device pointer of a contiguous int32 tensor of that shape."""
-    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous() or t.get_device() != ctx.device:
-        raise ValueError("%s: a contiguous int32 tensor %s on device %d is wanted, got %s %s on %s"
-                         % (name, tuple(shape), ctx.device, t.dtype, tuple(t.shape), t.device))
+def _ints(dev, name, t, n):
+    """Device pointer of a contiguous int32 tensor of n values."""
+    if t.dtype is not _I32 or t.numel() != n or not t.is_contiguous() or t.get_device() != dev:
+        raise ValueError("%s: a contiguous int32 tensor of %d values on device %d is wanted, got %s %s on %s" % (name, n, dev, t.dtype, tuple(t.shape), t.device))
     return t.data_ptr()
 
 
-def _rows(ctx, name, t, act, width=0):
-    """(pointer, heads * head_dim, stride) of a 2-D tensor of tokens whose rows are packed."""
-    if t.dim() != 2 or t.stride(1) != 1 or t.dtype not in _ACT or _ACT[t.dtype] != act or t.get_device() != ctx.device or (width and t.shape[1] != width):
-        raise ValueError("%s: 2-D activations%s of one type, packed rows, on device %d are wanted, got %s %s on %s"
-                         % (name, " %d wide" % width if width else "", ctx.device, t.dtype, tuple(t.shape), t.device))
-    return t.data_ptr(), t.shape[1], t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _rows(dev, name, t, dtype, n, width):
+    """(pointer, stride) of a 2-D tensor of n tokens whose rows are packed."""
+    if t.dtype is not dtype or t.dim() != 2 or t.size(0) != n or t.size(1) != width or t.stride(1) != 1 or t.get_device() != dev:
+        raise ValueError("%s: %s activations [%d][%d], packed rows, on device %d are wanted, got %s %s on %s"
+                         % (name, dtype, n, width, dev, t.dtype, tuple(t.shape), t.device))
+    return t.data_ptr(), t.stride(0) if n > 1 else width
 
 
 def plan(ctx, held, past, new, table, free_list, free_count_in, free_count_out, q_start, kv_len, pos, slot, page_size):
     """fl_b200_paged_plan; table [n_seq][max_blocks], free_list [n_pages], pos and slot [max_tokens]."""
-    n_seq, blocks, n_pages, n_tok = held.shape[0], table.shape[-1], free_list.shape[0], pos.shape[0]
+    n_seq, blocks, n_pages, n_tok, dev = held.numel(), table.size(-1), free_list.numel(), pos.numel(), ctx.device
     capi._ck(_entry(ctx.lib, "fl_b200_paged_plan")(
-        ctx._h, _ints(ctx, "held", held, (n_seq,)), _ints(ctx, "past", past, (n_seq,)), _ints(ctx, "new", new, (n_seq,)), n_seq, page_size,
-        _ints(ctx, "table", table, (n_seq, blocks)), blocks, _ints(ctx, "free_list", free_list, (n_pages,)), n_pages,
-        _ints(ctx, "free_count_in", free_count_in, (1,)), _ints(ctx, "free_count_out", free_count_out, (1,)),
-        _ints(ctx, "q_start", q_start, (n_seq + 1,)), _ints(ctx, "kv_len", kv_len, (n_seq,)), _ints(ctx, "pos", pos, (n_tok,)),
-        _ints(ctx, "slot", slot, (n_tok,)), n_tok))
+        ctx._h, _ints(dev, "held", held, n_seq), _ints(dev, "past", past, n_seq), _ints(dev, "new", new, n_seq), n_seq, page_size,
+        _ints(dev, "table", table, n_seq * blocks), blocks, _ints(dev, "free_list", free_list, n_pages), n_pages,
+        _ints(dev, "free_count_in", free_count_in, 1), _ints(dev, "free_count_out", free_count_out, 1), _ints(dev, "q_start", q_start, n_seq + 1),
+        _ints(dev, "kv_len", kv_len, n_seq), _ints(dev, "pos", pos, n_tok), _ints(dev, "slot", slot, n_tok), n_tok))
 
 
 class PagedCache:
@@ -73,35 +73,36 @@ class PagedCache:
                 raise ValueError("%s: a contiguous pool of %d f16 values on device %d is wanted, got %s %s on %s"
                                  % (name, n_pages * n_kv_head * page_size * head_dim, ctx.device, t.dtype, tuple(t.shape), t.device))
         self.ctx, self.k, self.v = ctx, k, v
+        self.width = n_kv_head * head_dim
         self.cfg = PagedCacheP(k.data_ptr(), v.data_ptr(), n_pages, page_size, n_kv_head, head_dim)
 
     def append(self, q, k, v, pos, slot, q_out, freq_base, n_rot=None):
         """RoPE on q (into q_out; both None: no q) and k, then k and v into their slots; q, k, v [n_tokens][heads * head_dim]."""
-        ctx, cfg, n, act = self.ctx, self.cfg, k.shape[0], _ACT.get(k.dtype)
-        width = cfg.n_kv_head * cfg.head_dim
-        kp, _, ks = _rows(ctx, "k", k, act, width)
-        vp, _, vs = _rows(ctx, "v", v, act, width)
+        ctx, dim, width, n, dtype, dev = self.ctx, self.cfg.head_dim, self.width, k.size(0), k.dtype, self.ctx.device
+        kp, ks = _rows(dev, "k", k, dtype, n, width)
+        vp, vs = _rows(dev, "v", v, dtype, n, width)
         qp, qw, qs, op, os_ = None, 0, 0, None, 0
         if q is not None:
-            qp, qw, qs = _rows(ctx, "q", q, act)
-            op, _, os_ = _rows(ctx, "q_out", q_out, act, qw)
-        if n > 1 and vs != ks or v.shape[0] != n or qw % cfg.head_dim or (q is not None and (q.shape[0] != n or q_out.shape[0] != n)):
-            raise ValueError("append: q, k, v and q_out of one number of tokens and whole heads, k and v of one stride")
+            qw = q.size(-1)
+            qp, qs = _rows(dev, "q", q, dtype, n, qw)
+            op, os_ = _rows(dev, "q_out", q_out, dtype, n, qw)
+        if dtype not in _ACT or vs != ks or qw % dim:
+            raise ValueError("append: f32 or f16 activations of whole heads, k and v of one stride")
         capi._ck(_entry(ctx.lib, "fl_b200_paged_append")(
-            ctx._h, self.cfg, act, qp, qw // cfg.head_dim, qs, kp, vp, ks, _ints(ctx, "pos", pos[:n], (n,)), _ints(ctx, "slot", slot[:n], (n,)), n,
-            cfg.head_dim if n_rot is None else n_rot, freq_base, op, os_))
+            ctx._h, self.cfg, _ACT[dtype], qp, qw // dim, qs, kp, vp, ks, _ints(dev, "pos", pos, n), _ints(dev, "slot", slot, n), n,
+            dim if n_rot is None else n_rot, freq_base, op, os_))
 
     def attn(self, q, table, q_start, kv_len, max_new, scale, out, lse=None):
         """Causal attention of every sequence's new tokens; q, out [n_tokens][heads * head_dim], lse [n_tokens][heads][2] f32."""
-        ctx, cfg, act = self.ctx, self.cfg, _ACT.get(q.dtype)
-        n, n_seq, blocks = q.shape[0], kv_len.shape[0], table.shape[-1]
-        qp, qw, qs = _rows(ctx, "q", q, act)
-        op, _, os_ = _rows(ctx, "out", out, act, qw)
-        if qw % cfg.head_dim or out.shape[0] != n:
-            raise ValueError("attn: whole heads, and an out row for every token")
-        if lse is not None and (lse.dtype != torch.float32 or lse.numel() != n * qw // cfg.head_dim * 2 or not lse.is_contiguous() or lse.get_device() != ctx.device):
-            raise ValueError("lse: f32 [n_tokens][heads][2]")
+        ctx, dim, n, qw, dtype, dev = self.ctx, self.cfg.head_dim, q.size(0), q.size(-1), q.dtype, self.ctx.device
+        n_seq, blocks = kv_len.numel(), table.size(-1)
+        qp, qs = _rows(dev, "q", q, dtype, n, qw)
+        op, os_ = _rows(dev, "out", out, dtype, n, qw)
+        if dtype not in _ACT or qw % dim:
+            raise ValueError("attn: f32 or f16 activations of whole heads")
+        if lse is not None and (lse.dtype != torch.float32 or lse.numel() != n * qw // dim * 2 or not lse.is_contiguous() or lse.get_device() != dev):
+            raise ValueError("lse: f32 [n_tokens][heads][2] on device %d" % dev)
         capi._ck(_entry(ctx.lib, "fl_b200_paged_attn")(
-            ctx._h, self.cfg, act, qp, qw // cfg.head_dim, qs, _ints(ctx, "table", table, (n_seq, blocks)), blocks,
-            _ints(ctx, "q_start", q_start, (n_seq + 1,)), _ints(ctx, "kv_len", kv_len, (n_seq,)), n_seq, n, max_new, scale, op, os_,
+            ctx._h, self.cfg, _ACT[dtype], qp, qw // dim, qs, _ints(dev, "table", table, n_seq * blocks), blocks,
+            _ints(dev, "q_start", q_start, n_seq + 1), _ints(dev, "kv_len", kv_len, n_seq), n_seq, n, max_new, scale, op, os_,
             None if lse is None else lse.data_ptr()))

@@ -68,9 +68,9 @@ def test_python_checks():
         device = 0
     i = torch.zeros(4, dtype=torch.int32)
     with pytest.raises(ValueError):          # not on the device
-        paged._ints(Ctx, "pos", i, (4,))
+        paged._ints(0, "pos", i, 4)
     with pytest.raises(ValueError):
-        paged._rows(Ctx, "q", torch.zeros(3, 64), paged.F32)
+        paged._rows(0, "q", torch.zeros(3, 64), torch.float32, 3, 64)
     with pytest.raises(ValueError):
         paged.PagedCache(Ctx, torch.zeros(8).half(), torch.zeros(8).half(), 1, 16, 1, 64)
 
