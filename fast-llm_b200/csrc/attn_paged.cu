@@ -4,8 +4,8 @@
 // o_r = sum_j exp(s_rj - m_r) v_j / sum_j exp(s_rj - m_r), s_rj = scale q_r . k_j, with the running maximum and sum of an online
 // softmax in f32. Bound by the HBM bytes of the keys and values: every tile is read once.
 //
-// CTA = 4 warps, two CTAs per SM. Lanes of warp 0 each copy one page's part of a tile (one TMA box of up to 64 rows) into a ring of three
-// stages of 32 KB; warp w takes keys 16 w .. 16 w + 15 of a tile. All tiles lie on one line (sequence, KV head, tile) and every CTA
+// CTA = 4 warps and a producer, two CTAs per SM. The producer's lanes each copy one page's part of a tile (one TMA box of up to 64 rows) into
+// a ring of three stages of 32 KB; warp w takes keys 16 w .. 16 w + 15 of a tile. All tiles lie on one line (sequence, KV head, tile) and every CTA
 // takes an equal piece of it.
 //   scores : A = 16 keys (ldmatrix), B = 4 rows of q as (hi, lo) f16 parts, scaled by a power of two per row so that both parts stay
 //            normal numbers: lane (g, t) has row t and keys g and g + 8
@@ -26,7 +26,7 @@ namespace flb {
 
 namespace {
 
-constexpr uint32_t kRowsB = kFewRows, kBlocks = kRowsB / 4, kTile = 64, kStages = 3, kWarps = 4, kThreads = kWarps * 32;
+constexpr uint32_t kRowsB = kFewRows, kTile = 64, kStages = 3, kWarps = 4, kThreads = (kWarps + 1) * 32;
 constexpr float kShift = 12.f;   // probabilities are 2^(x - m + 12): their lo parts stay normal f16 numbers down to 2^-14 of the largest
 
 // Rows of a sequence over one KV head, 0 where it is the other kernel's; its tiles: at least one, so that somebody writes its rows.
@@ -41,49 +41,38 @@ struct Piece {
     int32_t keys;
     uint32_t base;                                 // unit of its tile 0
 };
-struct Walk {
-    uint32_t pos, hi, seq_base, seq;               // seq_base: first unit of sequence `seq`
-    bool fresh;
-};
-// The next piece; p keeps the state between calls.
-__device__ __forceinline__ bool next_piece(const PagedAttnArgs &a, Walk &w, Piece &p) {
-    if (w.pos >= w.hi) return false;
-    bool bad;
-    if (w.fresh) {
-        w.fresh = false;
-        p.seq = w.seq;
-        p.q = paged_seq(a, p.seq, bad);
-        p.rows = rows_of(a, p.q);
-        p.tiles = tiles_of(p.q);
-        p.hkv = (w.pos - w.seq_base) / p.tiles;
-        p.base = w.seq_base + p.hkv * p.tiles;
-    } else {
-        p.base += p.tiles;
-        if (++p.hkv == a.n_kv) {
-            p.hkv = 0;
-            do { p.q = paged_seq(a, ++p.seq, bad); } while ((p.rows = rows_of(a, p.q)) == 0);
-            p.tiles = tiles_of(p.q);
-        }
-    }
-    p.keys = max(0, p.q.past + (int32_t)p.q.n);
+struct Walk { uint32_t pos, hi; };                 // the share's units behind the piece
+// Tiles of the piece that begins at w.pos, over KV head p.hkv of the sequence in p.
+__device__ __forceinline__ void cut_piece(Walk &w, Piece &p) {
     p.t0 = w.pos - p.base;
     p.t1 = min(p.tiles, w.hi - p.base);
     w.pos += p.t1 - p.t0;
+}
+// The piece behind p.
+__device__ __forceinline__ bool next_piece(const PagedAttnArgs &a, Walk &w, Piece &p) {
+    if (w.pos >= w.hi) return false;
+    p.base += p.tiles;
+    if (++p.hkv == a.n_kv) {
+        bool bad;
+        p.hkv = 0;
+        do { p.q = paged_seq(a, ++p.seq, bad); } while ((p.rows = rows_of(a, p.q)) == 0);
+        p.tiles = tiles_of(p.q);
+        p.keys = max(0, p.q.past + (int32_t)p.q.n);
+    }
+    cut_piece(w, p);
     return true;
 }
 
 template <int D> struct FewSmem {
     static constexpr uint32_t kHalfStage = kTile * D * 2;                 // K or V of a tile
     uint8_t ring[kStages][2 * kHalfStage];                                // 1024-byte aligned
-    float o[kWarps * kRowsB * 36];                                        // the warps' contexts, a part at a time; then records' maxima and sums
+    float o[kWarps * kRowsB * 36];                                        // q as operands; the warps' contexts, a part at a time; records' maxima and sums
+    float f[kRowsB];                                                      // score -> exponent of 2
     float m[kWarps][kRowsB], l[kWarps][kRowsB];
     uint32_t unfinite[3][D];                                              // see unfinite_of
-    uint64_t full[kStages];
-    uint64_t sum[kWarps];
-    uint32_t start_seq, start_off, any;
-    Walk walk;                                                            // of the copies (warp 0), which run ahead of the tiles in use
-    Piece piece;
-    uint32_t tile, issued;                                                // its next tile; copies begun
+    uint64_t full[kStages], empty[kStages];
+    uint64_t sum[kThreads / 32];
+    uint32_t start_seq, start_off, last, any_unfinite, abort_flag;
 };
 
 // Values of +inf, -inf and NaN (class 0, 1, 2) among the keys that only part of the rows attend: per class and dimension the
@@ -94,6 +83,8 @@ __device__ __forceinline__ float unfinite_of(const uint32_t *u, uint32_t dims, u
     return p <= lim ? INFINITY : n <= lim ? -INFINITY : 0.f;
 }
 
+__device__ __forceinline__ void bar_consumers() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ void arrive(uint64_t *bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory"); }
 __device__ __forceinline__ void prefetch_map(const CUtensorMap *m) { asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory"); }
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -131,112 +122,115 @@ __device__ __forceinline__ void put_lse(const PagedAttnArgs &a, uint64_t tok, ui
 // 2^(m - top); 0 for a maximum of nothing beside one of something
 __device__ __forceinline__ float weight(float m, float top) { return m == -INFINITY && top != -INFINITY ? 0.f : exp2_fast(top == -INFINITY ? 0.f : m - top); }
 
-// Copies the next tile of the share, if there is one, into its slot, which is free (a warp: lane i part i of the tile, one page's or less).
-// The page was looked up a call ahead; returns the next one's. Out of line: its registers are not the loop's.
+// The page that a lane's part of a tile lies on; -1: behind the last key.
+__device__ __forceinline__ int32_t page_at(const PagedAttnArgs &a, const Piece &p, uint32_t tile) {
+    const uint32_t lane = threadIdx.x & 31u, shift = min(a.page_shift, 6u), key = tile * kTile + (lane << shift);
+    return lane < kTile >> shift && key < (uint32_t)p.keys ? a.table[(uint64_t)p.seq * a.max_blocks + (key >> a.page_shift)] : -1;
+}
+// The producer warp: all tiles of the share into the ring, lane i part i of a tile (one page's or less). Pages are looked up a tile ahead.
 template <int D>
-__device__ __noinline__ int32_t copy_tile(const PagedAttnArgs &a, FewSmem<D> &sm, int32_t page) {
+__device__ __forceinline__ void copy_tiles(const PagedAttnArgs &a, FewSmem<D> &sm, Walk &walk, Piece &p) {
     constexpr uint32_t kKV = FewSmem<D>::kHalfStage;
-    const uint32_t lane = threadIdx.x & 31u, shift = min(a.page_shift, 6u), box = 1u << shift, boxes = kTile >> shift;
-    auto page_at = [&](const Piece &p, uint32_t tile) -> int32_t {   // -1: behind the last key
-        const uint32_t key = tile * kTile + (lane << shift);
-        return lane < boxes && key < (uint32_t)p.keys ? a.table[(uint64_t)p.seq * a.max_blocks + (key >> a.page_shift)] : -1;
-    };
-    uint32_t tile = sm.tile;
-    if (tile == sm.piece.t1) {
-        Walk w = sm.walk;
-        Piece p = sm.piece;
-        const bool more = next_piece(a, w, p);
-        __syncwarp();
-        if (!more) return page;
-        if (lane == 0) { sm.walk = w; sm.piece = p; }
-        tile = p.t0;
-        page = page_at(p, tile);
-        __syncwarp();
-    }
-    const Piece &p = sm.piece;
-    const uint32_t page_groups = (1u << a.page_shift) >> 3, key = tile * kTile + (lane << shift), issued = sm.issued, stage = issued % kStages;
-    uint32_t at = a.n_pages * a.n_kv * page_groups;   // behind the pool: copies from there bring zeros
-    if (lane < boxes && key < (uint32_t)p.keys) {
-        if ((uint32_t)page < a.n_pages) at = ((uint32_t)page * a.n_kv + p.hkv) * page_groups + ((key & ((1u << a.page_shift) - 1u)) >> 3);
-        else atomicCAS(a.status, ST_OK, ST_PAGED_PAGE);
-    }
-    if (lane == 0) mbar_arrive_expect_tx(&sm.full[stage], 2 * kKV);
-    __syncwarp();
-    if (lane < boxes) {
-        const uint32_t dst = smem_u32(sm.ring[stage]) + lane * box * D * 2, bar = smem_u32(&sm.full[stage]);
-        asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %2, %2, %3}], [%4];" ::"r"(dst),
-                     "l"(&a.kmap), "r"(0u), "r"(at), "r"(bar) : "memory");
-        asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %2, %2, %3}], [%4];" ::"r"(dst + kKV),
-                     "l"(&a.vmap), "r"(0u), "r"(at), "r"(bar) : "memory");
-    }
-    if (tile + 1 < p.t1) page = page_at(p, tile + 1);
-    __syncwarp();
-    if (lane == 0) { sm.tile = tile + 1; sm.issued = issued + 1; }
-    __syncwarp();
-    return page;
+    const uint32_t lane = threadIdx.x & 31u, shift = min(a.page_shift, 6u), boxes = kTile >> shift;
+    const uint32_t page_groups = (1u << a.page_shift) >> 3, in_page = (1u << a.page_shift) - 1u;
+    uint32_t issued = 0, stage = 0, parity = 1;
+    bool landed = true;
+    do {
+        int32_t page = page_at(a, p, p.t0);
+#pragma unroll 1
+        for (uint32_t tile = p.t0; tile < p.t1; ++tile) {
+            const uint32_t key = tile * kTile + (lane << shift);
+            uint32_t at = a.n_pages * a.n_kv * page_groups;   // behind the pool: copies from there bring zeros
+            if (lane < boxes && key < (uint32_t)p.keys) {
+                if ((uint32_t)page < a.n_pages) at = ((uint32_t)page * a.n_kv + p.hkv) * page_groups + ((key & in_page) >> 3);
+                else atomicCAS(a.status, ST_OK, ST_PAGED_PAGE);
+            }
+            if (tile + 1 < p.t1) page = page_at(a, p, tile + 1);
+            landed = __all_sync(0xffffffffu, mbar_wait_bounded(&sm.empty[stage], parity, a.status));
+            if (!landed) break;
+            if (lane == 0) mbar_arrive_expect_tx(&sm.full[stage], 2 * kKV);
+            __syncwarp();
+            if (lane < boxes) {
+                const uint32_t dst = smem_u32(sm.ring[stage]) + ((lane * D * 2) << shift), bar = smem_u32(&sm.full[stage]);
+                asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %2, %2, %3}], [%4];" ::"r"(dst),
+                             "l"(&a.kmap), "r"(0u), "r"(at), "r"(bar) : "memory");
+                asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %2, %2, %3}], [%4];" ::"r"(dst + kKV),
+                             "l"(&a.vmap), "r"(0u), "r"(at), "r"(bar) : "memory");
+            }
+            ++issued;
+            if (++stage == kStages) { stage = 0; parity ^= 1u; }
+        }
+    } while (landed && next_piece(a, walk, p));
+    if (!landed)   // nothing in flight when the shared memory goes back
+        for (uint32_t i = issued - min(issued, kStages); i < issued; ++i) mbar_wait_bounded(&sm.full[i % kStages], i / kStages & 1u, a.status);
 }
 
 // The records of a sequence over one KV head, added in order: of CTA c0 the piece at its end (or its first), of the others the one at
-// their start. (max, sum) of as many as there is room for at a time to shared memory, then the contexts, kFlight loads of a thread in
-// flight: the launch's tail is a chain of round trips to L2. Out of line: its registers are not the loop's.
+// their start. First the records' weights, a warp a row and a lane a record, then the contexts, eight loads of a thread in flight. This is the
+// launch's tail, and run once: its time is round trips to L2 and the fetching of its instructions, so it is kept short and out of line.
 template <int D>
 __device__ __noinline__ void combine(const PagedAttnArgs &a, FewSmem<D> &sm, const PagedSeq q, uint32_t hkv, uint32_t rows, uint32_t c0, uint32_t pieces, bool c0_first) {
-    constexpr uint32_t kFlight = 10, kRecord = kRowsB * (D + 4);
-    const uint32_t tid = threadIdx.x, items = rows * (D / 4), most = (uint32_t)(sizeof(sm.o) / sizeof(float2)) / rows;
-    const float *base = a.part + (uint64_t)c0 * 2 * kRecord;
-    auto record = [&](uint32_t i) { return base + (2 * i + (i || c0_first ? 0 : 1)) * kRecord; };
-    float2 *ml_s = reinterpret_cast<float2 *>(sm.o);
-    for (uint32_t i0 = 0; i0 < items; i0 += kThreads) {
-        const uint32_t i = i0 + tid, rw = i < items ? i / (D / 4) : rows - 1, d = i % (D / 4) * 4, at = rw * (D + 4) + d;
-        float mx = -INFINITY, s = 0.f;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (uint32_t k0 = 0; k0 < pieces; k0 += most) {
-            const uint32_t nk = min(most, pieces - k0);
-            if (i0 == 0 || pieces > most) {
-                __syncthreads();
-                for (uint32_t e = tid; e < nk * rows; e += kThreads) ml_s[e] = __ldcg(reinterpret_cast<const float2 *>(record(k0 + e / rows) + e % rows * (D + 4) + D));
-                __syncthreads();
-            }
-            float top = mx;
-            for (uint32_t k = 0; k < nk; ++k) top = fmaxf(top, ml_s[k * rows + rw].x);
-            const float w0 = weight(mx, top);
-            s *= w0; v.x *= w0; v.y *= w0; v.z *= w0; v.w *= w0;
-            mx = top;
+    constexpr uint32_t kFlight = 8, kRecord = kRowsB * (D + 4), kChunks = D / 4;
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, at_once = min(rows, (uint32_t)(sizeof(sm.o) / sizeof(float)) / pieces);
+    const float *rec = a.part + (uint64_t)c0 * 2 * kRecord;   // record i >= 1 at rec + 2 i kRecord
+    const uint32_t rec0 = c0_first ? 0 : kRecord;
+    for (uint32_t r0 = 0; r0 < rows; r0 += at_once) {
+        const uint32_t nr = min(at_once, rows - r0);
 #pragma unroll 1
-            for (uint32_t k = 0; k < nk; k += kFlight) {
+        for (uint32_t x = warp; x < nr; x += kWarps) {
+            const uint32_t ml_at = (r0 + x) * (D + 4) + D;
+            float top = -INFINITY, sum = 0.f;
+#pragma unroll 1
+            for (uint32_t k = lane; k < pieces; k += 32) top = fmaxf(top, __ldcg(rec + (k ? 2 * k * kRecord : rec0) + ml_at));
+            top = warp_max(top);
+#pragma unroll 1
+            for (uint32_t k = lane; k < pieces; k += 32) {
+                const float2 ml = __ldcg(reinterpret_cast<const float2 *>(rec + (k ? 2 * k * kRecord : rec0) + ml_at));
+                const float w = weight(ml.x, top);
+                sm.o[x * pieces + k] = w;
+                sum = fmaf(ml.y, w, sum);
+            }
+            sum = warp_sum(sum);
+            if (lane == 0) { sm.m[0][r0 + x] = top; sm.l[0][r0 + x] = sum; }
+        }
+        bar_consumers();
+#pragma unroll 1
+        for (uint32_t i = tid; i < nr * kChunks; i += kWarps * 32) {
+            const uint32_t x = i / kChunks, rw = r0 + x, d = i % kChunks * 4, tk = rw / a.group, hd = hkv * a.group + rw - tk * a.group;
+            const float *from = rec + rw * (D + 4) + d, *w = sm.o + x * pieces;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+            for (uint32_t k = 0; k < pieces; k += kFlight) {
                 float4 u[kFlight];
 #pragma unroll
                 for (uint32_t j = 0; j < kFlight; ++j)
-                    if (k + j < nk) u[j] = __ldcg(reinterpret_cast<const float4 *>(record(k0 + k + j) + at));
+                    u[j] = k + j < pieces ? __ldcg(reinterpret_cast<const float4 *>(from + (k + j ? 2 * (k + j) * kRecord : rec0))) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                 for (uint32_t j = 0; j < kFlight; ++j) {
-                    if (k + j >= nk) break;
-                    const float2 ml = ml_s[(k + j) * rows + rw];
-                    const float w = weight(ml.x, top);
-                    s = fmaf(ml.y, w, s);
-                    v.x = fmaf(u[j].x, w, v.x); v.y = fmaf(u[j].y, w, v.y); v.z = fmaf(u[j].z, w, v.z); v.w = fmaf(u[j].w, w, v.w);
+                    const float by = w[min(k + j, pieces - 1)];
+                    v.x = fmaf(u[j].x, by, v.x); v.y = fmaf(u[j].y, by, v.y); v.z = fmaf(u[j].z, by, v.z); v.w = fmaf(u[j].w, by, v.w);
                 }
             }
+            const float inv = q.past + (int32_t)tk < 0 ? 0.f : 1.f / sm.l[0][rw];
+            put(a, (q.first + tk) * a.out_stride + (uint64_t)hd * D + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+            if (a.lse && d == 0) put_lse(a, q.first + tk, hd, sm.m[0][rw], sm.l[0][rw]);
         }
-        if (i >= items) continue;
-        const uint32_t tk = rw / a.group, hd = hkv * a.group + rw - tk * a.group;
-        const float inv = q.past + (int32_t)tk < 0 ? 0.f : 1.f / s;
-        put(a, (q.first + tk) * a.out_stride + (uint64_t)hd * D + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
-        if (a.lse && d == 0) put_lse(a, q.first + tk, hd, mx, s);
+        bar_consumers();
     }
 }
 
-// The rows of a piece as the threads hold them: blocks of 4, lane (g, t) row t.
-template <int D> struct Rows {
-    uint32_t q[kBlocks][D / 16][2];        // operand: column g = row g / 2, part g & 1; dimensions 2t, 2t + 1, 2t + 8, 2t + 9 of every 16
-    float o[kBlocks][D / 16][2];           // contexts: dimensions g and g + 8 of every 16
-    float f[kBlocks], m[kBlocks], l[kBlocks];   // score -> exponent of 2; maximum, sum
-    int32_t lim[kBlocks];                  // last key
+// The rows of a piece as the threads hold them: blocks of 4 (at most B), lane (g, t) row t. q as operand: column g = row g / 2, part
+// g & 1; dimensions 2t, 2t + 1, 2t + 8, 2t + 9 of every 16; in registers for one block, else it stays in shared memory.
+template <int D, int B> struct Rows {
+    uint2 q[B == 1 ? D / 16 : 1];
+    float o[B][D / 16][2];                 // contexts: dimensions g and g + 8 of every 16
+    float f[B], m[B], l[B];                // score -> exponent of 2; maximum, sum
+    int32_t lim[B];                        // last key
 };
 
 // A warp's 16 keys (from key k0) against N blocks of rows.
-template <int D, int N>
-__device__ __forceinline__ void tile_step(Rows<D> &w, uint32_t k_s, uint32_t v_s, int32_t k0) {
+template <int D, int B, int N>
+__device__ __forceinline__ void tile_step(Rows<D, B> &w, const uint2 *q_s, uint32_t k_s, uint32_t v_s, int32_t k0) {
     constexpr uint32_t kGroupBytes = 8 * D * 2;
     const uint32_t lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u, mi = lane >> 3, r8 = lane & 7u;
     float sc[N][4];
@@ -246,8 +240,9 @@ __device__ __forceinline__ void tile_step(Rows<D> &w, uint32_t k_s, uint32_t v_s
         ldsm4(k_s + (mi & 1u) * kGroupBytes + (kb >> 2) * 1024 + r8 * 128 + (((2 * (kb & 3) + (mi >> 1)) ^ r8) << 4), ka);
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            if (kb == 0) mma_first(sc[n], ka, w.q[n][kb][0], w.q[n][kb][1]);
-            else mma(sc[n], ka, w.q[n][kb][0], w.q[n][kb][1]);
+            const uint2 q = B == 1 ? w.q[kb] : q_s[(n * (D / 16) + kb) * 32];
+            if (kb == 0) mma_first(sc[n], ka, q.x, q.y);
+            else mma(sc[n], ka, q.x, q.y);
         }
     }
     float al[N];
@@ -285,45 +280,54 @@ __device__ __forceinline__ void tile_step(Rows<D> &w, uint32_t k_s, uint32_t v_s
     }
 }
 
-// q of a piece's rows, the factors of their scores, their last keys.
+// Block n of a piece's rows of q as operands into shared memory, with the factors of their scores (a warp).
 template <int D>
-__device__ __forceinline__ void load_rows(const PagedAttnArgs &a, const Piece &p, Rows<D> &w) {
+__device__ __forceinline__ void build_q(const PagedAttnArgs &a, FewSmem<D> &sm, const Piece &p, uint32_t n) {
     const uint32_t lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
+    const uint32_t row = n * 4 + (g >> 1), tok = row / a.group, head = p.hkv * a.group + row - tok * a.group;
+    const uint64_t src = row < p.rows ? (p.q.first + tok) * a.q_stride + (uint64_t)head * D : 0;
+    float2 x[D / 8];
+    if (a.half) {
 #pragma unroll
-    for (uint32_t n = 0; n < kBlocks; ++n) {
-        if (n * 4 >= p.rows) break;
-        const uint32_t row = n * 4 + (g >> 1), tok = row / a.group, head = p.hkv * a.group + row - tok * a.group;
-        const bool there = row < p.rows;
-        const uint64_t src = there ? (p.q.first + tok) * a.q_stride + (uint64_t)head * D : 0;
-        float2 x[D / 8];
+        for (int j = 0; j < D / 8; ++j) x[j] = __half22float2(*reinterpret_cast<const __half2 *>((const __half *)a.q + src + 8 * j + 2 * t));
+    } else {
 #pragma unroll
-        for (int j = 0; j < D / 8; ++j) {
-            if (a.half) x[j] = __half22float2(*reinterpret_cast<const __half2 *>((const __half *)a.q + src + 8 * j + 2 * t));
-            else x[j] = *reinterpret_cast<const float2 *>((const float *)a.q + src + 8 * j + 2 * t);
-        }
-        float top = 0.f;
+        for (int j = 0; j < D / 8; ++j) x[j] = *reinterpret_cast<const float2 *>((const float *)a.q + src + 8 * j + 2 * t);
+    }
+    float top = 0.f;
 #pragma unroll
-        for (int j = 0; j < D / 8; ++j) top = fmaxf(top, fmaxf(fabsf(x[j].x), fabsf(x[j].y)));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // a power of two brings the row's largest value to [2^11, 2^12)
-        const int e = min(100, max(-100, 138 - (int)(__float_as_uint(top) >> 23)));
-        const float up = __uint_as_float((uint32_t)(e + 127) << 23);
-        w.f[n] = __shfl_sync(0xffffffffu, fmaxf(a.scale * 1.44269504088896341f * __uint_as_float((uint32_t)(127 - e) << 23), 1e-37f), 8 * t);
+    for (int j = 0; j < D / 8; ++j) top = fmaxf(top, fmaxf(fabsf(x[j].x), fabsf(x[j].y)));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    // a power of two brings the row's largest value to [2^11, 2^12)
+    const int e = min(100, max(-100, 138 - (int)(__float_as_uint(top) >> 23)));
+    const float up = __uint_as_float((uint32_t)(e + 127) << 23);
+    if (t == 0 && !(g & 1u)) sm.f[row] = fmaxf(a.scale * 1.44269504088896341f * __uint_as_float((uint32_t)(127 - e) << 23), 1e-37f);
+    uint2 *to = reinterpret_cast<uint2 *>(sm.o) + n * (D / 16) * 32 + lane;
 #pragma unroll
-        for (int kb = 0; kb < D / 16; ++kb)
+    for (int kb = 0; kb < D / 16; ++kb)
+        to[kb * 32] = make_uint2(part2(x[2 * kb].x * up, x[2 * kb].y * up, g & 1u), part2(x[2 * kb + 1].x * up, x[2 * kb + 1].y * up, g & 1u));
+}
+static_assert(kRowsB / 4 * (128 / 16) * 32 * sizeof(uint2) <= sizeof(FewSmem<128>::o), "q");
+template <int D, int B>
+__device__ __forceinline__ void begin_rows(const PagedAttnArgs &a, const FewSmem<D> &sm, const Piece &p, Rows<D, B> &w) {
+    const uint32_t lane = threadIdx.x & 31u, t = lane & 3u;
+    if (B == 1)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) w.q[n][kb][j] = part2(x[2 * kb + j].x * up, x[2 * kb + j].y * up, g & 1u);
+        for (int kb = 0; kb < D / 16; ++kb) w.q[kb] = reinterpret_cast<const uint2 *>(sm.o)[kb * 32 + lane];
+#pragma unroll
+    for (uint32_t n = 0; n < B; ++n) {
         const uint32_t mine = n * 4 + t;
+        w.f[n] = sm.f[mine];
         w.lim[n] = mine < p.rows ? p.q.past + (int32_t)(mine / a.group) : -1;
         w.m[n] = -INFINITY;
         w.l[n] = 0.f;
 #pragma unroll
-        for (int dt = 0; dt < D / 16; ++dt) w.o[n][dt][0] = w.o[n][dt][1] = 0.f;
+        for (int kb = 0; kb < D / 16; ++kb) w.o[n][kb][0] = w.o[n][kb][1] = 0.f;
     }
 }
 
-template <int D>
+template <int D, int B>   // at most 4 B rows
 __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_constant__ PagedAttnArgs a) {
     extern __shared__ uint8_t smem_dyn[];
     FewSmem<D> &sm = *reinterpret_cast<FewSmem<D> *>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~(uintptr_t)1023);
@@ -332,8 +336,9 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
     if (tid == 0) {
         prefetch_map(&a.kmap);
         prefetch_map(&a.vmap);
-        for (uint32_t s = 0; s < kStages; ++s) mbar_init(&sm.full[s], 1);
-        sm.issued = 0;
+        for (uint32_t s = 0; s < kStages; ++s) { mbar_init(&sm.full[s], 1); mbar_init(&sm.empty[s], kWarps); }
+        sm.abort_flag = 0;
+        sm.any_unfinite = 0;
         fence_barrier_init();
     }
     for (uint32_t i = tid; i < 3 * D; i += kThreads) (&sm.unfinite[0][0])[i] = 0x7fffffffu;
@@ -342,76 +347,93 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
 
     // ---- this CTA's share of the line: every warp by itself for up to 32 sequences ----
     Shares sh;
-    uint32_t start_off, start_seq;
-    {
-        const bool one_warp = a.n_seq <= 32;
-        const uint32_t threads = one_warp ? 32 : kThreads, i = one_warp ? lane : tid;
-        const uint32_t per = (a.n_seq + threads - 1) / threads, s0 = min(i * per, a.n_seq), s1 = min(s0 + per, a.n_seq);
+    Piece p;
+    Walk walk;
+    if (a.n_seq <= 32) {
+        bool bad = false;
+        const PagedSeq q = lane < a.n_seq ? paged_seq(a, lane, bad) : PagedSeq{0, 0, 0};
+        const uint64_t mine = units_of(a, q);
+        bad |= mine >> 26 != 0;   // (32 of them stay below 2^32; 2^26 tiles are 2^32 keys)
+        const uint32_t u = mine >> 26 ? 0u : (uint32_t)mine;
+        uint32_t x = u;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= (uint32_t)o) x += y;
+        }
+        if (bad && blockIdx.x == 0) atomicCAS(a.status, ST_OK, ST_PAGED_ARGS);
+        sh = shares_of(__shfl_sync(0xffffffffu, x, 31), gridDim.x);
+        if (blockIdx.x >= sh.n) return;
+        walk = Walk{share_lo(sh, blockIdx.x), share_lo(sh, blockIdx.x + 1)};
+        const int src = __ffs(__ballot_sync(0xffffffffu, walk.pos < x)) - 1;   // the first sequence that ends behind the share's begin
+        p.seq = src;
+        p.q.first = __shfl_sync(0xffffffffu, q.first, src);
+        p.q.n = __shfl_sync(0xffffffffu, q.n, src);
+        p.q.past = __shfl_sync(0xffffffffu, q.past, src);
+        p.base = __shfl_sync(0xffffffffu, x - u, src);
+    } else {
+        const uint32_t per = (a.n_seq + kThreads - 1) / kThreads, s0 = min(tid * per, a.n_seq), s1 = min(s0 + per, a.n_seq);
         uint64_t mine = 0;
         bool bad = false, any_bad = false;
         for (uint32_t s = s0; s < s1; ++s) {
             mine += units_of(a, paged_seq(a, s, bad));
             any_bad |= bad;
         }
-        uint64_t x = mine;
+        uint64_t x = mine, total = 0;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint64_t u = __shfl_up_sync(0xffffffffu, x, o);
             if (lane >= (uint32_t)o) x += u;
         }
-        uint64_t total = __shfl_sync(0xffffffffu, x, 31);
-        if (!one_warp) {
-            if (lane == 31) sm.sum[warp] = x;
-            __syncthreads();
-            total = 0;
-            for (uint32_t w = 0; w < kWarps; ++w) {
-                if (w < warp) x += sm.sum[w];
-                total += sm.sum[w];
-            }
+        if (lane == 31) sm.sum[warp] = x;
+        __syncthreads();
+        for (uint32_t w = 0; w < kThreads / 32; ++w) {
+            if (w < warp) x += sm.sum[w];
+            total += sm.sum[w];
         }
         if ((any_bad || total >> 32) && blockIdx.x == 0) atomicCAS(a.status, ST_OK, ST_PAGED_ARGS);
         x -= mine;
         sh = shares_of(total >> 32 ? 0u : (uint32_t)total, gridDim.x);
         if (blockIdx.x >= sh.n) return;
-        const uint32_t lo = share_lo(sh, blockIdx.x);
-        const bool here = lo >= x && lo < x + mine;
-        uint32_t s = s0;
-        if (here)
+        walk = Walk{share_lo(sh, blockIdx.x), share_lo(sh, blockIdx.x + 1)};
+        if (walk.pos >= x && walk.pos < x + mine) {
+            uint32_t s = s0;
             for (;; ++s) {
                 const uint64_t u = units_of(a, paged_seq(a, s, bad));
-                if (lo < x + u) break;
+                if (walk.pos < x + u) break;
                 x += u;
             }
-        if (one_warp) {
-            const int src = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
-            start_seq = __shfl_sync(0xffffffffu, s, src);
-            start_off = __shfl_sync(0xffffffffu, (uint32_t)x, src);
-        } else {
-            if (here) { sm.start_seq = s; sm.start_off = (uint32_t)x; }
-            __syncthreads();
-            start_seq = sm.start_seq;
-            start_off = sm.start_off;
+            sm.start_seq = s;
+            sm.start_off = (uint32_t)x;
         }
+        __syncthreads();
+        p.seq = sm.start_seq;
+        p.base = sm.start_off;
+        p.q = paged_seq(a, p.seq, bad);
     }
-    Walk walk{share_lo(sh, blockIdx.x), share_lo(sh, blockIdx.x + 1), start_off, start_seq, true};
-    Piece p;
-    int32_t page = -1;                // of the next copy (this lane's part of it)
-    if (warp == 0) {
-        if (lane == 0) { sm.walk = walk; sm.piece.t1 = 0; sm.tile = 0; }
-        __syncwarp();
-#pragma unroll 1
-        for (uint32_t i = 0; i < kStages; ++i) page = copy_tile<D>(a, sm, page);
+    p.rows = rows_of(a, p.q);
+    p.tiles = tiles_of(p.q);
+    p.keys = max(0, p.q.past + (int32_t)p.q.n);
+    p.hkv = (walk.pos - p.base) / p.tiles;
+    p.base += p.hkv * p.tiles;
+    cut_piece(walk, p);
+    if (warp == kWarps) {
+        copy_tiles<D>(a, sm, walk, p);
+        return;
     }
 
     uint32_t stage = 0, parity = 0;   // of the ring
-    bool first = true;
-    while (next_piece(a, walk, p)) {
-        Rows<D> w;
-        load_rows<D>(a, p, w);
+    bool first = true, landed = true;   // (landed: no wait of this warp has run out)
+    do {
+        for (uint32_t n = warp; n * 4 < p.rows; n += kWarps) build_q<D>(a, sm, p, n);
+        bar_consumers();
+        Rows<D, B> w;
+        begin_rows<D, B>(a, sm, p, w);
+        const uint2 *q_s = reinterpret_cast<const uint2 *>(sm.o) + lane;
         const int32_t lim_first = p.q.past;   // last key that all rows attend
 #pragma unroll 1
         for (uint32_t tile = p.t0; tile < p.t1; ++tile) {
-            const bool landed = mbar_wait_bounded(&sm.full[stage], parity, a.status);
+            landed = landed && __all_sync(0xffffffffu, mbar_wait_bounded(&sm.full[stage], parity, a.status));
             const int32_t k0 = (int32_t)(tile * kTile + warp * 16);
             if (landed && k0 < p.keys) {
                 const uint32_t k_s = smem_u32(sm.ring[stage]) + warp * 2 * kGroupBytes, v_s = k_s + kKV;
@@ -432,6 +454,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
                                 for (uint32_t j = 0; j < 8; ++j) {
                                     const uint16_t b = __half_as_ushort(h[j]);
                                     if ((b & 0x7C00u) == 0x7C00u) {
+                                        sm.any_unfinite = 1u;
                                         atomicMin(&sm.unfinite[(b & 0x3FFu) ? 2 : b >> 15][c * 8 + j], (uint32_t)key);
                                         h[j] = __ushort_as_half(0);
                                     }
@@ -442,19 +465,15 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
                     fence_proxy_async_smem();   // (the next copy into this stage comes after these writes)
                     __syncwarp();
                 }
-                if (p.rows <= 4) tile_step<D, 1>(w, k_s, v_s, k0);
-                else if (p.rows <= 8) tile_step<D, 2>(w, k_s, v_s, k0);
-                else tile_step<D, 4>(w, k_s, v_s, k0);
+                if (B == 1 || p.rows <= 4) tile_step<D, B, 1>(w, q_s, k_s, v_s, k0);
+                else if (B == 2 || p.rows <= 8) tile_step<D, B, (B < 2 ? 1 : 2)>(w, q_s, k_s, v_s, k0);
+                else tile_step<D, B, B>(w, q_s, k_s, v_s, k0);
             }
-            if (!__syncthreads_and(landed)) {   // (the tile is used up, or all give up, with no copy in flight)
-                if (tid == 0)
-                    for (uint32_t i = sm.issued - min(sm.issued, kStages); i < sm.issued; ++i) mbar_wait_bounded(&sm.full[i % kStages], i / kStages & 1u, a.status);
-                __syncthreads();
-                return;
-            }
-            if (warp == 0) page = copy_tile<D>(a, sm, page);
+            __syncwarp();
+            if (lane == 0) arrive(&sm.empty[stage]);
             if (++stage == kStages) { stage = 0; parity ^= 1u; }
         }
+        if (!landed) sm.abort_flag = 1u;   // (everybody goes on to the barriers, nobody writes)
 
         // ---- the warps' sums, a part of the dimensions at a time ----
         const uint32_t c0 = owner_of(sh, p.base), pieces = owner_of(sh, p.base + p.tiles - 1) - c0 + 1;
@@ -462,16 +481,16 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
         float *rec = a.part + (uint64_t)(blockIdx.x * 2 + (first ? 0 : 1)) * kRowsB * (D + 4);
         first = false;
 #pragma unroll
-        for (uint32_t n = 0; n < kBlocks; ++n) {
+        for (uint32_t n = 0; n < B; ++n) {
             if (n * 4 >= p.rows) break;
             w.l[n] += __shfl_xor_sync(0xffffffffu, w.l[n], 4);
             w.l[n] += __shfl_xor_sync(0xffffffffu, w.l[n], 8);
             w.l[n] += __shfl_xor_sync(0xffffffffu, w.l[n], 16);
             if (g == 0) { sm.m[warp][n * 4 + t] = w.m[n]; sm.l[warp][n * 4 + t] = w.l[n]; }
         }
-        __syncthreads();
+        bar_consumers();
 #pragma unroll
-        for (uint32_t n = 0; n < kBlocks; ++n) {   // contexts relative to the largest maximum
+        for (uint32_t n = 0; n < B; ++n) {   // contexts relative to the largest maximum
             if (n * 4 >= p.rows) break;
             float top = -INFINITY;
 #pragma unroll
@@ -487,6 +506,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
         const int32_t row_lim = p.q.past + (int32_t)tok;
         const uint64_t dst = (p.q.first + tok) * a.out_stride + (uint64_t)head * D;
         float top = -INFINITY, sum = 0.f;
+        const bool writes = row < p.rows && !sm.abort_flag;
         if (row < p.rows) {
 #pragma unroll
             for (uint32_t x = 0; x < kWarps; ++x) top = fmaxf(top, sm.m[x][row]);
@@ -495,17 +515,17 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
         }
 #pragma unroll 1
         for (uint32_t d0 = 0; d0 < D; d0 += wide) {
-            if (d0) __syncthreads();
+            if (d0) bar_consumers();
 #pragma unroll
-            for (uint32_t n = 0; n < kBlocks; ++n) {
+            for (uint32_t n = 0; n < B; ++n) {
                 if (n * 4 >= p.rows) break;
                 float *at = sm.o + ((warp << row_bits) + n * 4 + t) * pitch + g;
 #pragma unroll
                 for (int dt = 0; dt < D / 16; ++dt)
                     if (dt * 16u >= d0 && dt * 16u - d0 < wide) { at[dt * 16u - d0] = w.o[n][dt][0]; at[dt * 16u - d0 + 8] = w.o[n][dt][1]; }
             }
-            __syncthreads();
-            if (row < p.rows) {
+            bar_consumers();
+            if (writes) {
                 float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                 for (uint32_t x = 0; x < kWarps; ++x) {
@@ -513,8 +533,10 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
                     v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
                 }
                 const uint32_t d = d0 + c4;
-                v.x += unfinite_of(&sm.unfinite[0][0], D, d, row_lim); v.y += unfinite_of(&sm.unfinite[0][0], D, d + 1, row_lim);
-                v.z += unfinite_of(&sm.unfinite[0][0], D, d + 2, row_lim); v.w += unfinite_of(&sm.unfinite[0][0], D, d + 3, row_lim);
+                if (sm.any_unfinite) {
+                    v.x += unfinite_of(&sm.unfinite[0][0], D, d, row_lim); v.y += unfinite_of(&sm.unfinite[0][0], D, d + 1, row_lim);
+                    v.z += unfinite_of(&sm.unfinite[0][0], D, d + 2, row_lim); v.w += unfinite_of(&sm.unfinite[0][0], D, d + 3, row_lim);
+                }
                 if (whole) {
                     const float inv = row_lim < 0 ? 0.f : 1.f / sum;
                     put(a, dst + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
@@ -523,24 +545,28 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
                 }
             }
         }
-        if (row < p.rows && c4 == 0) {
+        if (writes && c4 == 0) {
             if (!whole) __stcg(reinterpret_cast<float4 *>(rec + row * (D + 4) + D), make_float4(top, sum, 0.f, 0.f));
             else if (a.lse) put_lse(a, p.q.first + tok, head, top, sum);
         }
         if (!whole) {
             fence_acq_rel_gpu();
-            __syncthreads();
-            if (tid == 0) sm.any = atomicAdd(&a.tickets[c0], 1u) == pieces - 1 ? 1u : 0u;
+            bar_consumers();
+            if (tid == 0) sm.last = !sm.abort_flag && atomicAdd(&a.tickets[c0], 1u) == pieces - 1 ? 1u : 0u;
         }
-        __syncthreads();   // (also: everybody has read the unfinite values)
-        for (uint32_t i = tid; i < 3 * D; i += kThreads) (&sm.unfinite[0][0])[i] = 0x7fffffffu;
-        if (!whole && sm.any) {
+        bar_consumers();   // (also: everybody has read the unfinite values)
+        if (sm.any_unfinite) {
+            for (uint32_t i = tid; i < 3 * D; i += kWarps * 32) (&sm.unfinite[0][0])[i] = 0x7fffffffu;
+            bar_consumers();
+            if (tid == 0) sm.any_unfinite = 0;
+        }
+        if (!whole && sm.last) {
             fence_acq_rel_gpu();
             combine<D>(a, sm, p.q, p.hkv, p.rows, c0, pieces, p.base <= share_lo(sh, c0));
             if (tid == 0) a.tickets[c0] = 0;
         }
-        __syncthreads();   // the shared arrays are free for the next piece
-    }
+        bar_consumers();   // the shared arrays are free for the next piece
+    } while (next_piece(a, walk, p));
     griddep_launch_dependents();
 }
 
@@ -548,9 +574,15 @@ template <int D> constexpr size_t few_smem() { return sizeof(FewSmem<D>) + 1024;
 
 } // namespace
 
+static const struct { void (*k)(const PagedAttnArgs); size_t smem; } kFewKernels[2][3] = {
+    {{paged_few_kernel<64, 1>, few_smem<64>()}, {paged_few_kernel<64, 2>, few_smem<64>()}, {paged_few_kernel<64, 4>, few_smem<64>()}},
+    {{paged_few_kernel<128, 1>, few_smem<128>()}, {paged_few_kernel<128, 2>, few_smem<128>()}, {paged_few_kernel<128, 4>, few_smem<128>()}}};
+
 cudaError_t paged_few_init(void) {
-    if (const cudaError_t e = cudaFuncSetAttribute(paged_few_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)few_smem<64>())) return e;
-    return cudaFuncSetAttribute(paged_few_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)few_smem<128>());
+    for (const auto &row : kFewKernels)
+        for (const auto &k : row)
+            if (const cudaError_t e = cudaFuncSetAttribute(k.k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)k.smem)) return e;
+    return cudaSuccess;
 }
 
 size_t paged_few_part_bytes(int sms) { return (size_t)4 * sms * kRowsB * (128 + 4) * sizeof(float); }
@@ -561,8 +593,9 @@ cudaError_t launch_paged_few(PagedAttnArgs a, const void *k, const void *v, uint
     if (grid > kPagedTickets) return cudaErrorInvalidConfiguration;
     if (const cudaError_t e = tensor_map_groups_swz(&a.kmap, k, rows, head_dim, box)) return e;
     if (const cudaError_t e = tensor_map_groups_swz(&a.vmap, v, rows, head_dim, box)) return e;
-    return head_dim == 128 ? launch_kernel(paged_few_kernel<128>, dim3(grid), dim3(kThreads), few_smem<128>(), stream, true, a)
-                           : launch_kernel(paged_few_kernel<64>, dim3(grid), dim3(kThreads), few_smem<64>(), stream, true, a);
+    const uint64_t most = std::min<uint64_t>((uint64_t)a.max_new * a.group, kRowsB);
+    const auto &k_ = kFewKernels[head_dim == 128][most <= 4 ? 0 : most <= 8 ? 1 : 2];
+    return launch_kernel(k_.k, dim3(grid), dim3(kThreads), k_.smem, stream, true, a);
 }
 
 } // namespace flb
