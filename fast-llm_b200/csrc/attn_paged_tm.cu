@@ -18,7 +18,7 @@
 //
 // The tensor cores truncate their running sum, 1.3e-8 of it per instruction; with f32 activations a part of 32 columns of O is therefore
 // brought out at every tile, in turn, added in f32 to a buffer of the CTA's own that stays in L2, and starts from zero: no sum in
-// tensor memory is longer than four tiles (64 instructions).
+// tensor memory is longer than four tiles (64 instructions), a piece's first one eight.
 #include "common.cuh"
 #include "paged.h"
 
@@ -48,10 +48,7 @@ struct Job {
     uint32_t whole, slot;               // the block is this CTA's alone; its record's
     int32_t past;
 };
-struct Walk {
-    uint32_t pos, hi, seq_base, seq;
-    bool fresh;
-};
+struct Walk { uint32_t pos, hi; };   // the share's units behind the piece
 struct Block { uint32_t rows, tiles; int32_t keys; };
 struct Piece {
     PagedSeq q;
@@ -235,6 +232,8 @@ template <int D, int Parts>
 __device__ __noinline__ float load_q(const PagedAttnArgs &a, uint8_t *dst, uint64_t src, uint32_t row0, uint32_t rows, bool store) {
     constexpr int V = 4, K = D / 32, kBatch = 4;   // values of a load, loads of a lane and row, groups of 4 rows in flight
     const uint32_t lane = threadIdx.x & 31u, sub = lane & 7u, group = lane >> 3;
+    if (row0 + lane < rows)   // (the second half's rows come to L2 beside the first's)
+        for (uint32_t c = 0; c < D * 2 * Parts; c += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint8_t *>(a.q) + src * (2 * Parts) + c));
     float f = 0.f;
 #pragma unroll 1
     for (uint32_t i0 = 0; i0 < 8; i0 += kBatch) {
@@ -349,54 +348,55 @@ __device__ __forceinline__ uint64_t head_units(const PagedAttnArgs &a, const Pag
     return u;
 }
 
-// The next piece of a CTA's share, for a whole warp.
-__device__ __forceinline__ bool next_piece(const PagedAttnArgs &a, Walk &w, Piece &p) {
-    if (w.pos >= w.hi) return false;
-    bool bad;
-    if (w.fresh) {
-        w.fresh = false;
-        p.seq = w.seq;
-        p.q = paged_seq(a, p.seq, bad);
-        p.n_blk = blocks_of(a, p.q);
-        // the KV head, then the block (32 at a time), that hold the share's first unit
-        const uint32_t lane = threadIdx.x & 31u;
-        uint32_t per_head = 0;
-        for (uint32_t b = lane; b < p.n_blk; b += 32) per_head += block_of(a, p.q, b).tiles;
-        per_head = __reduce_add_sync(0xffffffffu, per_head);
-        p.hkv = (w.pos - w.seq_base) / per_head;
-        p.base = w.seq_base + p.hkv * per_head;
-        for (uint32_t b0 = 0;; b0 += 32) {
-            const uint32_t t = b0 + lane < p.n_blk ? block_of(a, p.q, b0 + lane).tiles : 0u;
-            uint32_t x = t;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
-                if (lane >= (uint32_t)o) x += y;
-            }
-            const uint32_t behind = __ballot_sync(0xffffffffu, p.base + x > w.pos);
-            if (behind) {
-                const int at = __ffs(behind) - 1;
-                p.blk = b0 + at;
-                p.base += __shfl_sync(0xffffffffu, x - t, at);
-                break;
-            }
-            p.base += __shfl_sync(0xffffffffu, x, 31);
-        }
-        p.b = block_of(a, p.q, p.blk);
-    } else {
-        p.base += p.b.tiles;
-        if (++p.blk == p.n_blk) {
-            p.blk = 0;
-            if (++p.hkv == a.n_kv) {
-                p.hkv = 0;
-                do { p.q = paged_seq(a, ++p.seq, bad); } while ((p.n_blk = blocks_of(a, p.q)) == 0);
-            }
-        }
-        p.b = block_of(a, p.q, p.blk);
-    }
+// The tiles of the piece that begins at w.pos, in the block in p.
+__device__ __forceinline__ void cut_piece(Walk &w, Piece &p) {
     p.t0 = w.pos - p.base;
     p.t1 = min(p.b.tiles, w.hi - p.base);
     w.pos += p.t1 - p.t0;
+}
+// The share's first piece (a warp): p has its sequence, whose first unit is p.base. The KV head, then the block, 32 at a time.
+__device__ __forceinline__ void first_piece(const PagedAttnArgs &a, Walk &w, Piece &p) {
+    const uint32_t lane = threadIdx.x & 31u;
+    p.n_blk = blocks_of(a, p.q);
+    uint32_t per_head = 0;
+    for (uint32_t b = lane; b < p.n_blk; b += 32) per_head += block_of(a, p.q, b).tiles;
+    per_head = __reduce_add_sync(0xffffffffu, per_head);
+    p.hkv = (w.pos - p.base) / per_head;
+    p.base += p.hkv * per_head;
+    for (uint32_t b0 = 0;; b0 += 32) {
+        const uint32_t t = b0 + lane < p.n_blk ? block_of(a, p.q, b0 + lane).tiles : 0u;
+        uint32_t x = t;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= (uint32_t)o) x += y;
+        }
+        const uint32_t behind = __ballot_sync(0xffffffffu, p.base + x > w.pos);
+        if (behind) {
+            const int at = __ffs(behind) - 1;
+            p.blk = b0 + at;
+            p.base += __shfl_sync(0xffffffffu, x - t, at);
+            break;
+        }
+        p.base += __shfl_sync(0xffffffffu, x, 31);
+    }
+    p.b = block_of(a, p.q, p.blk);
+    cut_piece(w, p);
+}
+// The piece behind p.
+__device__ __forceinline__ bool next_piece(const PagedAttnArgs &a, Walk &w, Piece &p) {
+    if (w.pos >= w.hi) return false;
+    p.base += p.b.tiles;
+    if (++p.blk == p.n_blk) {
+        p.blk = 0;
+        if (++p.hkv == a.n_kv) {
+            bool bad;
+            p.hkv = 0;
+            do { p.q = paged_seq(a, ++p.seq, bad); } while ((p.n_blk = blocks_of(a, p.q)) == 0);
+        }
+    }
+    p.b = block_of(a, p.q, p.blk);
+    cut_piece(w, p);
     return true;
 }
 // A small block: both lanes have its rows, lane l the tiles t0 + l, t0 + l + 2, ..
@@ -535,30 +535,50 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
     griddep_wait();
     if (tid == 0) a.blocks[blockIdx.x].records = 0;
 
-    // ---- this CTA's share of the line ----
-    uint64_t total = 0;
-    {
-        bool bad = false, any_bad = false;
-        uint64_t mine = 0;
+    // ---- this CTA's share of the line: every warp by itself for up to 32 sequences ----
+    Shares sh;
+    Walk walk;
+    Piece p;
+    bool bad = false;
+    if (a.n_seq <= 32) {
+        const PagedSeq q = lane < a.n_seq ? paged_seq(a, lane, bad) : PagedSeq{0, 0, 0};
+        const uint64_t mine = head_units(a, q, lane) * a.n_kv;
+        bad |= mine >> 26 != 0;   // (32 of them stay below 2^32)
+        const uint32_t u = mine >> 26 ? 0u : (uint32_t)mine;
+        uint32_t x = u;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= (uint32_t)o) x += y;
+        }
+        if (bad && blockIdx.x == 0) atomicCAS(a.status, ST_OK, ST_PAGED_ARGS);
+        sh = shares_of(__shfl_sync(0xffffffffu, x, 31), gridDim.x);
+        walk = Walk{share_lo(sh, blockIdx.x), share_lo(sh, blockIdx.x + 1)};
+        const uint32_t at = __ballot_sync(0xffffffffu, walk.pos < x);   // sequences that end behind the share's begin
+        const int src = at ? __ffs(at) - 1 : 0;
+        p.seq = src;
+        p.q.first = __shfl_sync(0xffffffffu, q.first, src);
+        p.q.n = __shfl_sync(0xffffffffu, q.n, src);
+        p.q.past = __shfl_sync(0xffffffffu, q.past, src);
+        p.base = __shfl_sync(0xffffffffu, x - u, src);
+    } else {
+        uint64_t total = 0, mine = 0;
         for (uint32_t s0 = 0; s0 < a.n_seq; s0 += kThreads) {
-            const PagedSeq q = s0 + tid < a.n_seq ? paged_seq(a, s0 + tid, bad) : PagedSeq{0, 0, 0};
-            any_bad |= bad;
+            bool b = false;
+            const PagedSeq q = s0 + tid < a.n_seq ? paged_seq(a, s0 + tid, b) : PagedSeq{0, 0, 0};
+            bad |= b;
             mine += head_units(a, q, lane) * a.n_kv;
         }
-        if (any_bad) atomicCAS(a.status, ST_OK, ST_PAGED_ARGS);
+#pragma unroll
         for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
         if (lane == 0) hd.sum[warp] = mine;
         __syncthreads();
         for (uint32_t w = 0; w < kThreads / 32; ++w) total += hd.sum[w];
-    }
-    if (total >> 32 && tid == 0) atomicCAS(a.status, ST_OK, ST_PAGED_ARGS);
-    const Shares sh = shares_of(total >> 32 ? 0u : (uint32_t)total, gridDim.x);
-    if (blockIdx.x >= sh.n) return;
-    const uint32_t lo = share_lo(sh, blockIdx.x), hi = share_lo(sh, blockIdx.x + 1);
-    {
+        if ((bad || total >> 32) && blockIdx.x == 0) atomicCAS(a.status, ST_OK, ST_PAGED_ARGS);
+        sh = shares_of(total >> 32 ? 0u : (uint32_t)total, gridDim.x);
+        walk = Walk{share_lo(sh, blockIdx.x), share_lo(sh, blockIdx.x + 1)};
         uint64_t run = 0;
-        for (uint32_t s0 = 0; s0 < a.n_seq && run <= lo; s0 += kThreads) {
-            bool bad;
+        for (uint32_t s0 = 0; s0 < a.n_seq && blockIdx.x < sh.n && run <= walk.pos; s0 += kThreads) {
             const PagedSeq q = s0 + tid < a.n_seq ? paged_seq(a, s0 + tid, bad) : PagedSeq{0, 0, 0};
             const uint64_t u = head_units(a, q, lane) * a.n_kv;
             uint64_t x = u;
@@ -575,9 +595,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
                 if (w < warp) x += hd.sum[w];
                 run += hd.sum[w];
             }
-            if (lo >= x && lo < x + u) { hd.start_seq = s0 + tid; hd.start_off = (uint32_t)x; }
+            if (walk.pos >= x && walk.pos < x + u) { hd.start_seq = s0 + tid; hd.start_off = (uint32_t)x; }
+        }
+        __syncthreads();
+        if (blockIdx.x < sh.n) {
+            p.seq = hd.start_seq;
+            p.base = hd.start_off;
+            p.q = paged_seq(a, p.seq, bad);
         }
     }
+    if (blockIdx.x >= sh.n) return;
+    first_piece(a, walk, p);
     __syncthreads();
     for (uint32_t i = tid; i < 3 * D; i += kThreads) hd.unfinite[i] = 0x7fffffffu;
     if (warp == kTensorWarp) {
@@ -588,8 +616,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
     __syncthreads();
     fence_after();
     const uint32_t tmem = hd.tmem;
-    Walk walk{lo, hi, hd.start_off, hd.start_seq, true};
-    Piece p;
     bool dead = false;
     auto wait = [&](uint64_t *bar, uint32_t parity) {
         if (!dead && !__all_sync(0xffffffffu, try_bar(bar, parity))) dead = !wait_slow(bar, parity, a.status, &hd.abort_flag);
@@ -603,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
         const uint32_t box = min(1u << a.page_shift, kTile), boxes = kTile / box, bytes = box * D * 2;
         const uint32_t page_groups = (1u << a.page_shift) >> 3, outside = a.n_pages * a.n_kv * page_groups;
         uint32_t issued = 0;
-        while (!dead && next_piece(a, walk, p)) {
+        for (bool more = true; more && !dead; more = next_piece(a, walk, p)) {
             const int32_t *row = a.table + (uint64_t)p.seq * a.max_blocks;
             const uint32_t n = p.t1 - p.t0;
             const bool sm = small(p);
@@ -691,7 +717,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
             if (elect_one()) commit(&hd.empty[slot]);
             __syncwarp();
         };
-        while (!dead && next_piece(a, walk, p)) {
+        for (bool more = true; more && !dead; more = next_piece(a, walk, p)) {
             const uint32_t n = p.t1 - p.t0;
             const bool sm = small(p);
             if (!wait(&hd.q_full, pieces_in & 1u)) break;
@@ -745,7 +771,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
     } else if (warp == kValueWarp) {
         // ---- values that must not meet the tensor cores ----
         uint32_t v_seen = 0;
-        while (!dead && next_piece(a, walk, p)) {
+        for (bool more = true; more && !dead; more = next_piece(a, walk, p)) {
             const uint32_t n = p.t1 - p.t0;
             const bool sm = small(p);
             if (!wait(&hd.q_full, pieces_in & 1u)) break;   // (the notes of the piece before have been read)
@@ -798,12 +824,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
         const uint32_t ts = tmem + (w4 * 32u << 16) + l * kTile, to = tmem + (w4 * 32u << 16) + kOCol + l * 128;
         float4 *acc_mem = reinterpret_cast<float4 *>(a.part_tm + ((uint64_t)gridDim.x * 4 + blockIdx.x * 2 + l) * T::kRecord) + r;   // this row's sums
         uint32_t s_seen = 0;
-        if (warp == 0) { hd.walk = walk; hd.job.slot = 2; }   // (2: none yet)
+        if (warp == 0 && lane == 0) { hd.walk = walk; hd.piece = p; hd.job.slot = 2; }   // (2: none yet)
+        __syncwarp();
         for (;;) {
             if (warp == 0) {
                 Walk w = hd.walk;
                 Piece x = hd.piece;
-                const bool valid = next_piece(a, w, x);
+                const bool valid = hd.job.slot == 2 || next_piece(a, w, x);
                 __syncwarp();
                 if (lane == 0) {
                     hd.walk = w;
@@ -841,7 +868,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
             for (uint32_t step = 0; step < steps; ++step) {
                 const int32_t k0 = (int32_t)((t0 + (sm ? 2 * step + l : step)) * kTile);
                 const uint32_t c4 = step & 3u;   // the columns of O that go out at this step
-                if (Parts == 2 && active && step && c4 < D / 32) {
+                if (Parts == 2 && active && step >= 4 && c4 < D / 32) {
                     // a part of O to its sum in memory, while the tensor cores form the scores
                     if (!wait(&hd.o_done[l], (s_seen - 1) & 1u)) break;
                     fence_after();

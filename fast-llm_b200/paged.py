@@ -47,7 +47,7 @@ def _ints(dev, name, t, n):
 
 def _rows(dev, name, t, dtype, n, width):
     """(pointer, stride) of a 2-D tensor of n tokens whose rows are packed."""
-    if t.dtype is not dtype or t.dim() != 2 or t.size(0) != n or t.size(1) != width or t.stride(1) != 1 or t.get_device() != dev:
+    if t.dtype is not dtype or t.size() != (n, width) or t.get_device() != dev or t.stride(1) != 1:
         raise ValueError("%s: %s activations [%d][%d], packed rows, on device %d are wanted, got %s %s on %s"
                          % (name, dtype, n, width, dev, t.dtype, tuple(t.shape), t.device))
     return t.data_ptr(), t.stride(0) if n > 1 else width
