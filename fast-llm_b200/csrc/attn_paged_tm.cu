@@ -300,11 +300,20 @@ template <int D, int Parts> __device__ __forceinline__ void stage_out(const uint
     constexpr uint32_t kRowBytes = D * 2 * Parts, kLanes = kRowBytes / 16;   // lanes of a row
     const uint32_t lane = threadIdx.x & 31u, c = lane % kLanes;
     __syncwarp();
-#pragma unroll 4
-    for (uint32_t i = lane / kLanes; i < 32; i += 32 / kLanes) {
-        const uint64_t at = __shfl_sync(0xffffffffu, dst, i);
-        const uint32_t r = row0 + i;
-        if (r < rows) *reinterpret_cast<uint4 *>(static_cast<uint8_t *>(out) + at * (2 * Parts) + c * 16) = *reinterpret_cast<const uint4 *>(stage + r * kRowBytes + ((c ^ (r & (kLanes - 1))) << 4));
+#pragma unroll 1
+    for (uint32_t i0 = 0; i0 < 32; i0 += 8 * (32 / kLanes)) {
+        uint4 v[8];
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) {
+            const uint32_t r = row0 + i0 + j * (32 / kLanes) + lane / kLanes;
+            v[j] = *reinterpret_cast<const uint4 *>(stage + r * kRowBytes + ((c ^ (r & (kLanes - 1))) << 4));
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) {
+            const uint32_t i = i0 + j * (32 / kLanes) + lane / kLanes;
+            const uint64_t at = __shfl_sync(0xffffffffu, dst, i);
+            if (row0 + i < rows) *reinterpret_cast<uint4 *>(static_cast<uint8_t *>(out) + at * (2 * Parts) + c * 16) = v[j];
+        }
     }
     __syncwarp();
 }
@@ -776,6 +785,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
             const bool sm = small(p);
             if (!wait(&hd.q_full, pieces_in & 1u)) break;   // (the notes of the piece before have been read)
             ++pieces_in;
+            {   // the next piece's rows of q to L2
+                Walk w2 = walk;
+                Piece p2 = p;
+                if (next_piece(a, w2, p2))
+                    for (uint32_t i = lane; i < p2.b.rows; i += 32) {
+                        const uint32_t at = p2.blk * 2 * kRowsL + i, tok = at / a.group, head = p2.hkv * a.group + at - tok * a.group;
+                        const uint8_t *from = static_cast<const uint8_t *>(a.q) + ((p2.q.first + tok) * a.q_stride + (uint64_t)head * D) * (2 * Parts);
+                        for (uint32_t c = 0; c < D * 2 * Parts; c += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(from + c));
+                    }
+            }
             const int32_t lim_first = p.q.past + (int32_t)(p.blk * 2 * kRowsL / a.group);
             for (uint32_t t = 0; t < n; ++t, ++v_seen) {
                 const uint32_t i = done + v_index(sm, t, n), slot = i % T::kSlots;
@@ -790,17 +809,32 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
                 uint8_t *vt = ring + slot * T::kPart;
                 const int32_t k0 = (int32_t)((p.t0 + t) * kTile);
                 const uint32_t r0 = (uint32_t)max(0, lim_first + 1 - k0);   // the first key that not all rows attend
-                for (uint32_t j = r0 * (D / 8) + lane; j < kTile * (D / 8); j += 32) {
+                // 16-byte piece j: of key j / (D / 8)
+                auto piece = [&](uint32_t j) {
                     const uint32_t r = j / (D / 8), c = j % (D / 8);
-                    const int32_t key = k0 + (int32_t)r;
-                    uint4 *at = reinterpret_cast<uint4 *>(vt + (r >> 3) * (D * 16) + (c >> 3) * 1024 + (r & 7u) * 128 + (((c ^ r) & 7u) << 4));
-                    if (key >= p.b.keys) {
-                        *at = make_uint4(0, 0, 0, 0);
-                    } else {
-                        const uint4 w = *at;
-                        const uint32_t z = ((w.x & 0x7C007C00u) + 0x04000400u) | ((w.y & 0x7C007C00u) + 0x04000400u) | ((w.z & 0x7C007C00u) + 0x04000400u) | ((w.w & 0x7C007C00u) + 0x04000400u);
-                        if (z & 0x80008000u) {   // an exponent of all ones
-                            hd.any_unfinite = 1u;
+                    return reinterpret_cast<uint4 *>(vt + (r >> 3) * (D * 16) + (c >> 3) * 1024 + (r & 7u) * 128 + (((c ^ r) & 7u) << 4));
+                };
+                auto ones = [](const uint4 &w) {   // bits 15, 31: an exponent of all ones in a half
+                    return ((w.x & 0x7C007C00u) + 0x04000400u) | ((w.y & 0x7C007C00u) + 0x04000400u) | ((w.z & 0x7C007C00u) + 0x04000400u) | ((w.w & 0x7C007C00u) + 0x04000400u);
+                };
+                const uint32_t end = (uint32_t)min((int32_t)kTile, p.b.keys - k0) * (D / 8);
+                for (uint32_t j = end + lane; j < kTile * (D / 8); j += 32) *piece(j) = make_uint4(0, 0, 0, 0);
+                uint32_t any = 0, j0 = r0 * (D / 8) + lane;
+                for (; j0 + 7 * 32 < end; j0 += 8 * 32) {   // (eight loads in flight; the tensor cores may be waiting)
+                    uint4 w[8];
+#pragma unroll
+                    for (uint32_t j = 0; j < 8; ++j) w[j] = *piece(j0 + 32 * j);
+#pragma unroll
+                    for (uint32_t j = 0; j < 8; ++j) any |= ones(w[j]);
+                }
+                for (; j0 < end; j0 += 32) any |= ones(*piece(j0));
+                if (__any_sync(0xffffffffu, any & 0x80008000u)) {
+                    hd.any_unfinite = 1u;
+                    for (uint32_t j = r0 * (D / 8) + lane; j < end; j += 32) {
+                        uint4 *at = piece(j);
+                        const uint32_t r = j / (D / 8), c = j % (D / 8);
+                        const int32_t key = k0 + (int32_t)r;
+                        if (ones(*at) & 0x80008000u) {
                             __half *h = reinterpret_cast<__half *>(at);
                             for (uint32_t e = 0; e < 8; ++e) {
                                 const uint16_t b = __half_as_ushort(h[e]);
