@@ -49,13 +49,13 @@ struct Job {
     int32_t past;
 };
 struct Walk { uint32_t pos, hi; };   // the share's units behind the piece
-struct Block { uint32_t rows, tiles; int32_t keys; };
+struct Block { uint32_t rows, tiles, units; int32_t keys; };
 struct Piece {
     PagedSeq q;
     uint32_t seq, hkv, blk, n_blk;
     Block b;
     uint32_t t0, t1;
-    uint32_t base;       // unit of its block's tile 0
+    uint32_t base;       // first unit of its block
 };
 struct Head {
     uint64_t full[8], empty[8], v_ready[8], s_full[2], p_full[2][2], o_done[2], q_full, drain;
@@ -324,11 +324,17 @@ __device__ __forceinline__ float2 lse_of(float highest, float from, float sum) {
 }
 
 // ---- blocks, shares, pieces --------------------------------------------------------------------------------------------
+// A block's length on the line: its tiles, those of a small block half as long as the others (both lanes work on different ones), and in
+// front of them what its start and end cost in tiles (q in, contexts out). A tile is the CTA's whose share holds its first unit. (Tiles
+// alone: a prompt of 4096 tokens, whose first blocks have a tile or two, 482 us.)
+constexpr uint32_t kStart = 8;
+__device__ __forceinline__ uint32_t tile_units(uint32_t rows) { return rows <= kRowsL ? 1u : 2u; }
 __device__ __forceinline__ Block block_of(const PagedAttnArgs &a, const PagedSeq &q, uint32_t blk) {
     Block b;
     b.rows = min(2 * kRowsL, q.n * a.group - blk * 2 * kRowsL);
     b.keys = max(0, q.past + (int32_t)((blk * 2 * kRowsL + b.rows - 1) / a.group) + 1);
     b.tiles = max(1u, ((uint32_t)b.keys + kTile - 1) / kTile);
+    b.units = kStart + b.tiles * tile_units(b.rows);
     return b;
 }
 __device__ __forceinline__ uint32_t blocks_of(const PagedAttnArgs &a, const PagedSeq &q) {   // of this kernel: sequences of more than few_rows rows
@@ -340,7 +346,7 @@ __device__ __forceinline__ uint64_t head_units(const PagedAttnArgs &a, const Pag
     const uint32_t n = blocks_of(a, q);
     uint64_t u = 0;
     if (n <= 4)
-        for (uint32_t b = 0; b < n; ++b) u += block_of(a, q, b).tiles;
+        for (uint32_t b = 0; b < n; ++b) u += block_of(a, q, b).units;
     for (uint32_t todo = __ballot_sync(0xffffffffu, n > 4); todo; todo &= todo - 1) {
         const int src = __ffs(todo) - 1;
         PagedSeq x;
@@ -349,7 +355,7 @@ __device__ __forceinline__ uint64_t head_units(const PagedAttnArgs &a, const Pag
         x.past = __shfl_sync(0xffffffffu, q.past, src);
         const uint32_t nb = __shfl_sync(0xffffffffu, n, src);
         uint64_t v = 0;
-        for (uint32_t b = lane; b < nb; b += 32) v += block_of(a, x, b).tiles;
+        for (uint32_t b = lane; b < nb; b += 32) v += block_of(a, x, b).units;
 #pragma unroll
         for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         if (lane == (uint32_t)src) u = v;
@@ -357,23 +363,29 @@ __device__ __forceinline__ uint64_t head_units(const PagedAttnArgs &a, const Pag
     return u;
 }
 
-// The tiles of the piece that begins at w.pos, in the block in p.
-__device__ __forceinline__ void cut_piece(Walk &w, Piece &p) {
-    p.t0 = w.pos - p.base;
-    p.t1 = min(p.b.tiles, w.hi - p.base);
-    w.pos += p.t1 - p.t0;
+// The tiles of the piece that begins at w.pos, in the block in p; false: there are none.
+__device__ __forceinline__ bool cut_piece(Walk &w, Piece &p) {
+    const uint32_t front = p.base + kStart, shift = tile_units(p.b.rows) - 1u;
+    auto tile = [&](uint32_t unit) { return unit > front ? min(p.b.tiles, (unit - front + shift) >> shift) : 0u; };
+    p.t0 = tile(w.pos);
+    p.t1 = tile(w.hi);
+    w.pos = min(w.hi, p.base + p.b.units);
+    return p.t0 < p.t1;
 }
-// The share's first piece (a warp): p has its sequence, whose first unit is p.base. The KV head, then the block, 32 at a time.
-__device__ __forceinline__ void first_piece(const PagedAttnArgs &a, Walk &w, Piece &p) {
+// The CTAs that the piece's block's tiles begin and end in.
+__device__ __forceinline__ uint32_t owner_of_tile(const Shares &sh, const Piece &p, uint32_t tile) { return owner_of(sh, p.base + kStart + tile * tile_units(p.b.rows)); }
+// The share's first block (a warp): p has its sequence, whose first unit is p.base. The KV head, then the block, 32 at a time. Whether
+// the share has tiles of it.
+__device__ __forceinline__ bool first_piece(const PagedAttnArgs &a, Walk &w, Piece &p) {
     const uint32_t lane = threadIdx.x & 31u;
     p.n_blk = blocks_of(a, p.q);
     uint32_t per_head = 0;
-    for (uint32_t b = lane; b < p.n_blk; b += 32) per_head += block_of(a, p.q, b).tiles;
+    for (uint32_t b = lane; b < p.n_blk; b += 32) per_head += block_of(a, p.q, b).units;
     per_head = __reduce_add_sync(0xffffffffu, per_head);
     p.hkv = (w.pos - p.base) / per_head;
     p.base += p.hkv * per_head;
     for (uint32_t b0 = 0;; b0 += 32) {
-        const uint32_t t = b0 + lane < p.n_blk ? block_of(a, p.q, b0 + lane).tiles : 0u;
+        const uint32_t t = b0 + lane < p.n_blk ? block_of(a, p.q, b0 + lane).units : 0u;
         uint32_t x = t;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -390,22 +402,23 @@ __device__ __forceinline__ void first_piece(const PagedAttnArgs &a, Walk &w, Pie
         p.base += __shfl_sync(0xffffffffu, x, 31);
     }
     p.b = block_of(a, p.q, p.blk);
-    cut_piece(w, p);
+    return cut_piece(w, p);
 }
 // The piece behind p.
 __device__ __forceinline__ bool next_piece(const PagedAttnArgs &a, Walk &w, Piece &p) {
-    if (w.pos >= w.hi) return false;
-    p.base += p.b.tiles;
-    if (++p.blk == p.n_blk) {
-        p.blk = 0;
-        if (++p.hkv == a.n_kv) {
-            bool bad;
-            p.hkv = 0;
-            do { p.q = paged_seq(a, ++p.seq, bad); } while ((p.n_blk = blocks_of(a, p.q)) == 0);
+    do {
+        if (w.pos >= w.hi) return false;
+        p.base += p.b.units;
+        if (++p.blk == p.n_blk) {
+            p.blk = 0;
+            if (++p.hkv == a.n_kv) {
+                bool bad;
+                p.hkv = 0;
+                do { p.q = paged_seq(a, ++p.seq, bad); } while ((p.n_blk = blocks_of(a, p.q)) == 0);
+            }
         }
-    }
-    p.b = block_of(a, p.q, p.blk);
-    cut_piece(w, p);
+        p.b = block_of(a, p.q, p.blk);
+    } while (!cut_piece(w, p));
     return true;
 }
 // A small block: both lanes have its rows, lane l the tiles t0 + l, t0 + l + 2, ..
@@ -545,6 +558,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
     if (tid == 0) a.blocks[blockIdx.x].records = 0;
 
     // ---- this CTA's share of the line: every warp by itself for up to 32 sequences ----
+    auto shares = [](uint32_t units) {   // (two units at least: every CTA between a block's first and last one has a tile of it)
+        const uint32_t n = min(gridDim.x, units / 2);
+        return n ? Shares{n, units / n, units % n} : Shares{0, 0, 0};
+    };
     Shares sh;
     Walk walk;
     Piece p;
@@ -561,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
             if (lane >= (uint32_t)o) x += y;
         }
         if (bad && blockIdx.x == 0) atomicCAS(a.status, ST_OK, ST_PAGED_ARGS);
-        sh = shares_of(__shfl_sync(0xffffffffu, x, 31), gridDim.x);
+        sh = shares(__shfl_sync(0xffffffffu, x, 31));
         walk = Walk{share_lo(sh, blockIdx.x), share_lo(sh, blockIdx.x + 1)};
         const uint32_t at = __ballot_sync(0xffffffffu, walk.pos < x);   // sequences that end behind the share's begin
         const int src = at ? __ffs(at) - 1 : 0;
@@ -584,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
         __syncthreads();
         for (uint32_t w = 0; w < kThreads / 32; ++w) total += hd.sum[w];
         if ((bad || total >> 32) && blockIdx.x == 0) atomicCAS(a.status, ST_OK, ST_PAGED_ARGS);
-        sh = shares_of(total >> 32 ? 0u : (uint32_t)total, gridDim.x);
+        sh = shares(total >> 32 ? 0u : (uint32_t)total);
         walk = Walk{share_lo(sh, blockIdx.x), share_lo(sh, blockIdx.x + 1)};
         uint64_t run = 0;
         for (uint32_t s0 = 0; s0 < a.n_seq && blockIdx.x < sh.n && run <= walk.pos; s0 += kThreads) {
@@ -614,7 +631,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
         }
     }
     if (blockIdx.x >= sh.n) return;
-    first_piece(a, walk, p);
+    const bool some = first_piece(a, walk, p) || next_piece(a, walk, p);   // (a share may lie within a block's front)
     __syncthreads();
     for (uint32_t i = tid; i < 3 * D; i += kThreads) hd.unfinite[i] = 0x7fffffffu;
     if (warp == kTensorWarp) {
@@ -638,7 +655,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
         const uint32_t box = min(1u << a.page_shift, kTile), boxes = kTile / box, bytes = box * D * 2;
         const uint32_t page_groups = (1u << a.page_shift) >> 3, outside = a.n_pages * a.n_kv * page_groups;
         uint32_t issued = 0;
-        for (bool more = true; more && !dead; more = next_piece(a, walk, p)) {
+        for (bool more = some; more && !dead; more = next_piece(a, walk, p)) {
             const int32_t *row = a.table + (uint64_t)p.seq * a.max_blocks;
             const uint32_t n = p.t1 - p.t0;
             const bool sm = small(p);
@@ -726,7 +743,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
             if (elect_one()) commit(&hd.empty[slot]);
             __syncwarp();
         };
-        for (bool more = true; more && !dead; more = next_piece(a, walk, p)) {
+        for (bool more = some; more && !dead; more = next_piece(a, walk, p)) {
             const uint32_t n = p.t1 - p.t0;
             const bool sm = small(p);
             if (!wait(&hd.q_full, pieces_in & 1u)) break;
@@ -780,7 +797,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
     } else if (warp == kValueWarp) {
         // ---- values that must not meet the tensor cores ----
         uint32_t v_seen = 0;
-        for (bool more = true; more && !dead; more = next_piece(a, walk, p)) {
+        for (bool more = some; more && !dead; more = next_piece(a, walk, p)) {
             const uint32_t n = p.t1 - p.t0;
             const bool sm = small(p);
             if (!wait(&hd.q_full, pieces_in & 1u)) break;   // (the notes of the piece before have been read)
@@ -858,13 +875,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
         const uint32_t ts = tmem + (w4 * 32u << 16) + l * kTile, to = tmem + (w4 * 32u << 16) + kOCol + l * 128;
         float4 *acc_mem = reinterpret_cast<float4 *>(a.part_tm + ((uint64_t)gridDim.x * 4 + blockIdx.x * 2 + l) * T::kRecord) + r;   // this row's sums
         uint32_t s_seen = 0;
-        if (warp == 0 && lane == 0) { hd.walk = walk; hd.piece = p; hd.job.slot = 2; }   // (2: none yet)
+        if (warp == 0 && lane == 0) { hd.walk = walk; hd.piece = p; hd.job.slot = some ? 2 : 3; }   // (2: none yet)
         __syncwarp();
         for (;;) {
             if (warp == 0) {
                 Walk w = hd.walk;
                 Piece x = hd.piece;
-                const bool valid = hd.job.slot == 2 || next_piece(a, w, x);
+                const bool valid = hd.job.slot == 2 || (some && next_piece(a, w, x));
                 __syncwarp();
                 if (lane == 0) {
                     hd.walk = w;
@@ -872,7 +889,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
                     Job &j = hd.job;
                     j.valid = valid;
                     if (valid) {
-                        const uint32_t c0 = owner_of(sh, x.base), c1 = owner_of(sh, x.base + x.b.tiles - 1);
+                        const uint32_t c0 = owner_of_tile(sh, x, 0), c1 = owner_of_tile(sh, x, x.b.tiles - 1);
                         j.sm = small(x); j.n = x.t1 - x.t0; j.t0 = x.t0;
                         j.first = x.q.first; j.row0 = x.blk * 2 * kRowsL; j.rows = x.b.rows; j.hkv = x.hkv; j.past = x.q.past;
                         j.whole = c0 == c1;
