@@ -327,7 +327,7 @@ __device__ __forceinline__ float2 lse_of(float highest, float from, float sum) {
 // A block's length on the line: its tiles, those of a small block half as long as the others (both lanes work on different ones), and in
 // front of them what its start and end cost in tiles (q in, contexts out). A tile is the CTA's whose share holds its first unit. (Tiles
 // alone: a prompt of 4096 tokens, whose first blocks have a tile or two, 482 us.)
-constexpr uint32_t kStart = 8;
+constexpr uint32_t kStart = 12;
 __device__ __forceinline__ uint32_t tile_units(uint32_t rows) { return rows <= kRowsL ? 1u : 2u; }
 __device__ __forceinline__ Block block_of(const PagedAttnArgs &a, const PagedSeq &q, uint32_t blk) {
     Block b;
