@@ -152,8 +152,8 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs
 }
 
 // ---- append ---------------------------------------------------------------------------------------------------------
-// Bound by HBM bytes. A CTA turns kAppTokens tokens: their angles' sines and cosines once in shared memory, then every thread 16
-// bytes of one head at a time. The angle pos * base^(-2i/n) is formed in turns in 64 bits and reduced before it is rounded: in
+// Bound by HBM bytes. A CTA has one token (8192 tokens, 8B shape, f32: 66 us, four of them 69, eight 73), few tokens several CTAs each: the angles'
+// sines and cosines once in shared memory, then every thread 16 bytes of one head at a time, the next ones' load in flight. The angle pos * base^(-2i/n) is formed in turns in 64 bits and reduced before it is rounded: in
 // 32 bits a position of 120000 is 0.004 radians off.
 constexpr uint32_t kAppThreads = 256;
 
@@ -164,7 +164,7 @@ struct AppendArgs {
     const int32_t *pos, *slot;
     uint32_t *status;
     uint64_t q_stride, kv_stride, q_out_stride;
-    uint32_t n_tok, n_q, n_kv, dim_shift, n_rot, page_shift, n_pages, tokens;   // tokens: of a CTA
+    uint32_t n_q, n_kv, dim_shift, n_rot, page_shift, n_pages;
     double turns[64];               // base^(-2i/n_rot) / 2 pi
 };
 
@@ -201,58 +201,67 @@ template <> struct AppVec<__half> {
 
 template <typename T>
 __global__ void __launch_bounds__(kAppThreads) paged_append_kernel(const __grid_constant__ AppendArgs a) {
-    extern __shared__ float2 cs[];   // [tokens][n_rot / 2]
+    __shared__ float2 cs[64];   // cosine, sine per pair
     constexpr uint32_t N = AppVec<T>::N;
-    const uint32_t tid = threadIdx.x, t0 = blockIdx.x * a.tokens, nt = min(a.tokens, a.n_tok - t0), half = a.n_rot / 2;
+    const uint32_t tid = threadIdx.x, tok = blockIdx.x, half = a.n_rot / 2;
+    const uint32_t vec_shift = a.dim_shift - (N == 4 ? 2u : 3u), n_vec = (a.n_q + 2 * a.n_kv) << vec_shift, step = gridDim.y * kAppThreads;
     griddep_launch_dependents();
     griddep_wait();
-    for (uint32_t i = tid; i < nt * half; i += kAppThreads) {
-        const uint32_t t = i / half, p = i - t * half;
-        const double turn = (double)a.pos[t0 + t] * a.turns[p];
+    const int32_t pos = a.pos[tok], slot = a.slot[tok];
+    if (pos < 0) return;   // a row behind the last token
+    const uint32_t page = (uint32_t)slot >> a.page_shift;
+    const bool stored = slot >= 0 && page < a.n_pages;
+    if (slot >= 0 && !stored && tid == 0) atomicCAS(a.status, ST_OK, ST_PAGED_PAGE);
+    // piece i: its head, its dimension, where it comes from
+    auto head_of = [&](uint32_t i) { return i >> vec_shift; };
+    auto dim_of = [&](uint32_t i) { return (i & ((1u << vec_shift) - 1u)) * N; };
+    auto wanted = [&](uint32_t i) { return i < n_vec && (stored || head_of(i) < a.n_q); };
+    auto load = [&](uint32_t i, float (&x)[N]) {
+        const uint32_t h = head_of(i);
+        const T *src = h < a.n_q ? (const T *)a.q + tok * a.q_stride + ((uint64_t)h << a.dim_shift)
+                                 : (const T *)(h < a.n_q + a.n_kv ? a.k : a.v) + tok * a.kv_stride + ((uint64_t)(h - a.n_q - (h < a.n_q + a.n_kv ? 0u : a.n_kv)) << a.dim_shift);
+        AppVec<T>::load(src + dim_of(i), x);
+    };
+    float x[N];
+    uint32_t i = blockIdx.y * kAppThreads + tid;
+    if (wanted(i)) load(i, x);   // (in flight while the angles are formed)
+    for (uint32_t p = tid; p < half; p += kAppThreads) {
+        const double turn = (double)pos * a.turns[p];
         float s, c;
         sincospif((float)(2.0 * (turn - rint(turn))), &s, &c);
-        cs[i] = make_float2(c, s);
+        cs[p] = make_float2(c, s);
     }
     __syncthreads();
-    const uint32_t vecs = (1u << a.dim_shift) / N, vec_shift = 31u - __clz(vecs), heads = a.n_q + 2 * a.n_kv, per_tok = heads << vec_shift;
-    for (uint32_t i = blockIdx.y * kAppThreads + tid; i < nt * per_tok; i += gridDim.y * kAppThreads) {
-        const uint32_t t = i / per_tok, r = i - t * per_tok, h = r >> vec_shift, d = (r & (vecs - 1u)) * N;
-        const int32_t pos = a.pos[t0 + t], slot = a.slot[t0 + t];
-        if (pos < 0) continue;   // a row behind the last token
-        const bool is_q = h < a.n_q, is_k = !is_q && h < a.n_q + a.n_kv;
-        const uint32_t hk = is_q ? 0 : is_k ? h - a.n_q : h - a.n_q - a.n_kv, page = (uint32_t)slot >> a.page_shift;
-        if (!is_q && (slot < 0 || page >= a.n_pages)) {
-            if (slot >= 0) atomicCAS(a.status, ST_OK, ST_PAGED_PAGE);
-            continue;
-        }
-        const T *src = is_q ? (const T *)a.q + (t0 + t) * a.q_stride + ((uint64_t)h << a.dim_shift)
-                            : (const T *)(is_k ? a.k : a.v) + (t0 + t) * a.kv_stride + ((uint64_t)hk << a.dim_shift);
-        float x[N];
-        AppVec<T>::load(src + d, x);
-        if ((is_q || is_k) && d < a.n_rot) {
+    for (; i < n_vec; i += step) {
+        if (wanted(i)) {
+            const uint32_t h = head_of(i), d = dim_of(i);
+            const bool is_q = h < a.n_q, is_v = h >= a.n_q + a.n_kv;
+            if (!is_v && d < a.n_rot) {
 #pragma unroll
-            for (uint32_t j = 0; j < N; j += 2)
-                if (d + j < a.n_rot) {
-                    const float2 w = cs[t * half + (d + j) / 2];
-                    const float x0 = x[j], x1 = x[j + 1];
-                    x[j] = fmaf(x0, w.x, -(x1 * w.y));
-                    x[j + 1] = fmaf(x0, w.y, x1 * w.x);
-                }
-        }
-        if (is_q) {
-            AppVec<T>::store((T *)a.q_out + (t0 + t) * a.q_out_stride + ((uint64_t)h << a.dim_shift) + d, x);
-        } else {
-            const uint64_t row = (((uint64_t)page * a.n_kv + hk) << a.page_shift) + ((uint32_t)slot & ((1u << a.page_shift) - 1u));
-            __half *dst = (is_k ? a.kc : a.vc) + (row << a.dim_shift) + d;
-            uint32_t w[N / 2];
-#pragma unroll
-            for (uint32_t j = 0; j < N / 2; ++j) {
-                const __half2 y = __floats2half2_rn(x[2 * j], x[2 * j + 1]);
-                w[j] = *reinterpret_cast<const uint32_t *>(&y);
+                for (uint32_t j = 0; j < N; j += 2)
+                    if (d + j < a.n_rot) {
+                        const float2 w = cs[(d + j) / 2];
+                        const float x0 = x[j], x1 = x[j + 1];
+                        x[j] = fmaf(x0, w.x, -(x1 * w.y));
+                        x[j + 1] = fmaf(x0, w.y, x1 * w.x);
+                    }
             }
-            if constexpr (N == 4) *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
-            else *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+            if (is_q) {
+                AppVec<T>::store((T *)a.q_out + tok * a.q_out_stride + ((uint64_t)h << a.dim_shift) + d, x);
+            } else {
+                const uint64_t row = (((uint64_t)page * a.n_kv + h - a.n_q - (is_v ? a.n_kv : 0u)) << a.page_shift) + ((uint32_t)slot & ((1u << a.page_shift) - 1u));
+                __half *dst = (is_v ? a.vc : a.kc) + (row << a.dim_shift) + d;
+                uint32_t w[N / 2];
+#pragma unroll
+                for (uint32_t j = 0; j < N / 2; ++j) {
+                    const __half2 y = __floats2half2_rn(x[2 * j], x[2 * j + 1]);
+                    w[j] = *reinterpret_cast<const uint32_t *>(&y);
+                }
+                if constexpr (N == 4) *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
+                else *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
         }
+        if (wanted(i + step)) load(i + step, x);
     }
 }
 
@@ -360,20 +369,16 @@ int fl_b200_paged_append(fl_b200_ctx *c, const fl_b200_paged_cache *cache, int a
     a.kc = (__half *)cache->k_dev; a.vc = (__half *)cache->v_dev;
     a.pos = pos; a.slot = slot; a.status = c->status;
     a.q_stride = q_stride; a.kv_stride = kv_stride; a.q_out_stride = q_out_stride;
-    a.n_tok = n_tokens; a.n_q = n_q; a.n_kv = cache->n_kv_head; a.dim_shift = dim == 128 ? 7 : 6; a.n_rot = n_rot;
+    a.n_q = n_q; a.n_kv = cache->n_kv_head; a.dim_shift = dim == 128 ? 7 : 6; a.n_rot = n_rot;
     a.page_shift = (uint32_t)page_shift_of(cache->page_size); a.n_pages = cache->n_pages;
     // (a product more per pair: 64 roundings of 2^-53 at most)
     const double ratio = n_rot ? std::pow((double)freq_base, -2.0 / n_rot) : 0.0;
     double turn = 1.0 / 6.283185307179586476925;
     for (uint32_t i = 0; i < n_rot / 2; ++i, turn *= ratio) a.turns[i] = turn;
-    a.tokens = std::max(1u, std::min(4u, n_tokens / (4u * (uint32_t)c->sms)));
-    const uint32_t ctas = (n_tokens + a.tokens - 1) / a.tokens, per_tok = (n_q + 2 * a.n_kv) * dim / (act == FL_B200_ACT_F16 ? 8 : 4);
-    // few tokens: their heads over several CTAs
-    const uint32_t y = std::max(1u, std::min((a.tokens * per_tok + kAppThreads - 1) / kAppThreads, 2u * (uint32_t)c->sms / ctas));
-    const size_t smem = (size_t)a.tokens * (n_rot / 2) * sizeof(float2);
-    const cudaError_t e = act == FL_B200_ACT_F16
-        ? launch_kernel(paged_append_kernel<__half>, dim3(ctas, y), dim3(kAppThreads), smem, c->stream, true, a)
-        : launch_kernel(paged_append_kernel<float>, dim3(ctas, y), dim3(kAppThreads), smem, c->stream, true, a);
+    const uint32_t n_vec = (n_q + 2 * a.n_kv) * dim / (act == FL_B200_ACT_F16 ? 8 : 4);
+    const uint32_t y = std::max(1u, std::min((n_vec + kAppThreads - 1) / kAppThreads, 2u * (uint32_t)c->sms / n_tokens));
+    const auto kernel = act == FL_B200_ACT_F16 ? paged_append_kernel<__half> : paged_append_kernel<float>;
+    const cudaError_t e = launch_kernel(kernel, dim3(n_tokens, y), dim3(kAppThreads), 0, c->stream, true, a);
     return cuda_err(e, "paged_append launch");
 }
 
