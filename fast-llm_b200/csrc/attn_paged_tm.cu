@@ -16,7 +16,7 @@
 // tiles; a smaller block gives both lanes its rows, every other tile each, and their results are added as two records.
 // Tiles of all blocks lie on one line (sequence, KV head, block, tile); shares, records and tickets as in attn_paged.cu.
 //
-// The tensor cores truncate their running sum, 1.3e-8 of it per instruction; with f32 activations a part of 32 columns of O is therefore
+// The tensor cores truncate their running sum, 3.1e-8 of it per instruction (see kLoss); with f32 activations a part of 32 columns of O is therefore
 // brought out at every tile, in turn, added in f32 to a buffer of the CTA's own that stays in L2, and starts from zero: no sum in
 // tensor memory is longer than four tiles (64 instructions), a piece's first one eight.
 #include "common.cuh"
@@ -32,6 +32,10 @@ constexpr uint32_t kRowsL = 128, kTile = 128;
 constexpr uint32_t kCopyWarp = 8, kTensorWarp = 9, kValueWarp = 10, kThreads = 11 * 32;
 constexpr float kShift = 6.f;   // probabilities are 2^(x - ref), ref = maximum - 6 when it is set and kept while they stay below 2^14
 constexpr uint32_t kOCol = 256, kTmemCols = 512;
+// What a tensor instruction cuts off its 24-bit running sum, on average and relative to it: half a unit in the last place, 2^-25 times the mean of 1 / mantissa.
+// A sum of n equal steps ends n / 2 times that too small in the mean, which is given back where f32 results allow to see it (results against 64
+// bits, 4 x 8 tokens over 4096 keys: 1.4e-6 off without, of which 1.2e-6 were one common factor).
+constexpr float kLoss = 3.1e-8f;
 
 template <int D, int Parts> struct Tm {
     static constexpr uint32_t kPart = kRowsL * D * 2;               // one part of a lane's q; a K or V tile
@@ -268,7 +272,7 @@ __device__ __noinline__ float load_q(const PagedAttnArgs &a, uint8_t *dst, uint6
             for (int o = 4; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
             const int e = min(100, max(-100, 138 - (int)(__float_as_uint(top) >> 23)));
             const float up = __uint_as_float((uint32_t)(e + 127) << 23);
-            const float mine = fmaxf(a.scale * 1.44269504088896341f * __uint_as_float((uint32_t)(127 - e) << 23), 1e-37f);
+            const float mine = fmaxf(a.scale * (float)(1.44269504088896341 * (1.0 + (Parts == 2 ? D / 32 * (double)kLoss : 0.0))) * __uint_as_float((uint32_t)(127 - e) << 23), 1e-37f);
             // thread t's row is t: group t / 8's at i = t % 8
             const float got = __shfl_sync(0xffffffffu, mine, lane & 24u);
             if ((lane & 7u) == i0 + i) f = got;
@@ -439,6 +443,10 @@ __device__ __forceinline__ bool partly(const PagedAttnArgs &a, const Piece &p, u
 __device__ __forceinline__ void bar_both() { asm volatile("bar.sync 1, 256;" ::: "memory"); }   // the softmax warps
 
 struct Sums { float ref, sum, highest, acc_ref; uint32_t out_of; };   // of a row
+// The factor of contexts that were summed over that many tiles (8 instructions per tile and part).
+__device__ __forceinline__ float given_back(uint32_t tiles) { return fmaf(8.f * kLoss, (float)tiles, 1.f); }
+// The tiles of a lane that columns 32 c .. were summed over since they last went out (see the loop over the tiles), of `steps`.
+__device__ __forceinline__ uint32_t tiles_since(uint32_t steps, uint32_t c, bool went) { return went ? steps - ((steps - 1 - c) / 4 * 4 + c) : steps; }
 // The results of a lane's piece: the rows themselves, or a record. done: the lane has any, and they are in tensor memory.
 template <int D, int Parts>
 __device__ __noinline__ void finish(const PagedAttnArgs &a, Head &hd, uint8_t *q_s, const Sums s, bool done, uint32_t tmem) {
@@ -483,7 +491,7 @@ __device__ __noinline__ void finish(const PagedAttnArgs &a, Head &hd, uint8_t *q
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
             float o[32];
-            auto lane_part = [&](uint32_t from, const float4 *mem, uint32_t out, float before, float rf) {   // 32 columns of a lane's contexts
+            auto lane_part = [&](uint32_t from, const float4 *mem, uint32_t out, float before, float rf, uint32_t steps) {   // 32 columns of a lane's contexts
                 load32(from + 32 * c, o);
                 const bool acc = Parts == 2 && (out >> c & 1u);
                 float4 old[8];
@@ -491,6 +499,11 @@ __device__ __noinline__ void finish(const PagedAttnArgs &a, Head &hd, uint8_t *q
 #pragma unroll
                     for (int j = 0; j < 8; ++j) old[j] = __ldcg(mem + (8 * c + j) * kRowsL);
                 wait_ld(o);
+                if (Parts == 2) {
+                    const float back = given_back(tiles_since(steps, c, acc));
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) o[j] *= back;
+                }
                 if (acc) {
                     const float keep = before == rf ? 1.f : exp2_fast(before - rf);
 #pragma unroll
@@ -502,11 +515,11 @@ __device__ __noinline__ void finish(const PagedAttnArgs &a, Head &hd, uint8_t *q
             };
             float v[32];
             if (two) {
-                lane_part(to + 128, acc_mem + T::kRecord / 4, out2, acc2_ref, ref2);
+                lane_part(to + 128, acc_mem + T::kRecord / 4, out2, acc2_ref, ref2, job.n / 2);
 #pragma unroll
                 for (int j = 0; j < 32; ++j) v[j] = o[j] * w2;
             }
-            lane_part(to, acc_mem, s.out_of, s.acc_ref, ref);
+            lane_part(to, acc_mem, s.out_of, s.acc_ref, ref, sm ? (job.n + 1) / 2 : job.n);
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = two ? fmaf(o[j], w1, v[j]) : o[j];
             if (any_unfinite)
@@ -931,7 +944,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
                     store16(to + 32 * c4 + 16, zero);
                     if (out_of == 0) acc_ref = ref;
                     if (ref - acc_ref > 40.f) acc_ref = move_sums(acc_mem, out_of, acc_ref, ref);   // (far below what f32 holds: |O| < 2^47)
-                    const float by = ref == acc_ref ? 1.f : exp2_fast(ref - acc_ref);
+                    const float by = (ref == acc_ref ? 1.f : exp2_fast(ref - acc_ref)) * given_back(out_of >> c4 & 1u ? 4u : step);
                     float4 *at = acc_mem + 8 * c4 * kRowsL;
                     const bool adds = out_of >> c4 & 1u;
 #pragma unroll
