@@ -411,3 +411,215 @@ def test_plan_refuses_impossible_lengths(ctx, held, past, new, count):
     got = run_plan(ctx, held, past, new, table, free, count, 16, 3)
     assert ctx.status() == 4
     assert got == dict(table=table, free=free, count=count, pos=[-1] * 3, slot=[-1] * 3, start=[0, 0], length=[-9])
+
+
+# ---- together ----------------------------------------------------------------------------------------------------------------
+
+
+class Server:
+    """Requests that come, grow, are rewound and go, over one layer: plan, append and attention as a server calls them, beside a
+    plain copy of every request's rotated keys and values."""
+
+    def __init__(self, ctx, n_seq, blocks, n_pages, page, n_q, n_kv, dim, act, max_tokens, base=10000.0):
+        from fast_llm_b200 import paged
+        self.paged, self.ctx, self.page, self.n_q, self.n_kv, self.dim, self.act, self.base = paged, ctx, page, n_q, n_kv, dim, act, base
+        self.k = torch.full((n_pages, n_kv, page, dim), float("nan"), device="cuda", dtype=torch.float16)
+        self.v = self.k.clone()
+        self.cache = paged.PagedCache(ctx, self.k, self.v, n_pages, page, n_kv, dim)
+        self.table = torch.full((n_seq, blocks), -1, dtype=torch.int32, device="cuda")
+        self.free, self.count = torch.arange(n_pages, dtype=torch.int32, device="cuda"), ints([n_pages])
+        self.held, self.past, self.new = ints([0] * n_seq), ints([0] * n_seq), ints([0] * n_seq)
+        self.q_start = ints([0] * (n_seq + 1))
+        self.pos, self.slot = ints([0] * max_tokens), ints([0] * max_tokens)
+        self.rows = torch.zeros((max_tokens, (n_q + 2 * n_kv) * dim), device="cuda", dtype=DT[act])
+        self.q = torch.zeros((max_tokens, n_q * dim), device="cuda", dtype=DT[act])
+        self.out = torch.full((max_tokens, n_q * dim), CANARY, device="cuda", dtype=DT[act])
+        self.keys = [torch.zeros((0, n_kv, dim), device="cuda", dtype=torch.float16) for _ in range(n_seq)]
+        self.values = [torch.zeros((0, n_kv, dim), device="cuda", dtype=torch.float16) for _ in range(n_seq)]
+        self.scale = 1.0 / math.sqrt(dim)
+
+    def step(self, max_new):
+        """What the device runs; held becomes the new lengths, the count of free pages is kept in place."""
+        nq, nk, w = self.n_q * self.dim, self.n_kv * self.dim, self.rows
+        self.paged.plan(self.ctx, self.held, self.past, self.new, self.table, self.free, self.count, self.count, self.q_start, self.held, self.pos, self.slot,
+                        page_size=self.page)
+        self.cache.append(w[:, :nq], w[:, nq:nq + nk], w[:, nq + nk:], self.pos, self.slot, self.q, freq_base=self.base)
+        self.cache.attn(self.q, self.table, self.q_start, self.held, max_new, self.scale, self.out)
+
+    def check(self, past, new):
+        """The rows of the last step against 64 bits, from the plain copies."""
+        first = 0
+        for s, (p, m) in enumerate(zip(past, new)):
+            pos = torch.arange(p, p + m, device="cuda")
+            x = self.rows[first:first + m].view(m, self.n_q + 2 * self.n_kv, self.dim)
+            turned = append_expect(x[:, :self.n_q + self.n_kv], pos, self.dim, self.base)
+            # the stored keys may round the other way where the f32 rotation lies on the border: they are read back
+            slot = self.slot[first:first + m].long()
+            k = self.k[slot // self.page, :, slot % self.page]
+            assert ((k.double() - turned[:, self.n_q:]).abs() <= 2.0 ** -10 * turned[:, self.n_q:].abs() + 2.0 ** -20).all()
+            v = self.v[slot // self.page, :, slot % self.page]
+            assert torch.equal(v, x[:, self.n_q + self.n_kv:].half())
+            self.keys[s] = torch.cat([self.keys[s][:p], k])
+            self.values[s] = torch.cat([self.values[s][:p], v])
+            q = self.q[first:first + m].view(m, self.n_q, self.dim)
+            size = x[:, :self.n_q].double().abs().amax().item() if m else 0
+            assert ((q.double() - turned[:, :self.n_q]).abs() <= (2.0 ** -20 + (2.0 ** -11 if self.act == "f16" else 0)) * 2 * size).all()
+            got = self.out[first:first + m].double().view(m, self.n_q, self.dim)
+            for h in range(self.n_q):
+                kk, vv = (t[s][:, h * self.n_kv // self.n_q].double() for t in (self.keys, self.values))
+                a = q[:, h].double() @ kk.t() * self.scale
+                A = (q[:, h].double().abs() @ kk.t().abs() * self.scale).amax(-1, keepdim=True) if m else 0
+                a = a.masked_fill(torch.arange(p + m, device="cuda")[None, :] > pos[:, None], -math.inf)
+                w = a.softmax(-1)
+                tol = (A + 1) * 2.0 ** -18 * (w @ vv.abs())
+                if self.act == "f16":
+                    tol = tol + 2.0 ** -11 * (w @ vv.abs()) + 2.0 ** -11 * (w @ vv).abs() + 2.0 ** -25
+                assert ((got[:, h] - w @ vv).abs() <= tol).all(), (s, h)
+            first += m
+        assert (self.out[first:] == CANARY).all()
+        self.out.fill_(CANARY)
+
+
+STEPS = [  # (kept, new) per request; kept below the length: rewound, (0, 0): ended
+    [(0, 70), (0, 5), (0, 1), (0, 0)],
+    [(70, 1), (5, 1), (1, 1), (0, 150)],
+    [(71, 1), (6, 4), (2, 1), (150, 33)],
+    [(72, 1), (7, 3), (0, 0), (183, 1)],      # a draft is rewound by three tokens, a request ends
+    [(73, 90), (10, 1), (0, 40), (180, 2)],   # its row is used again
+    [(0, 0), (0, 0), (0, 0), (182, 1)],
+    [(0, 3), (0, 200), (0, 0), (0, 0)],
+]
+
+
+@pytest.mark.parametrize("n_q,n_kv,dim,page,act", [(8, 2, 128, 16, "f32"), (8, 2, 64, 32, "f16"), (5, 1, 128, 64, "f32")])
+def test_a_server(ctx, n_q, n_kv, dim, page, act):
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    srv = Server(ctx, 4, 20, 40, page, n_q, n_kv, dim, act, 300)
+    pages = 40
+    for step in STEPS:
+        past, new = [p for p, _ in step], [m for _, m in step]
+        srv.rows.copy_(torch.randn(srv.rows.shape, generator=g, device="cuda"))
+        srv.past.copy_(ints(past))
+        srv.new.copy_(ints(new))
+        srv.step(max(new))
+        ctx.sync()
+        assert ctx.status() == 0
+        srv.check(past, new)
+        pages_used = sum(-(-(p + m) // page) for p, m in step)
+        assert srv.count.item() == pages - pages_used
+        # every page is in one place
+        used = [x for s, (p, m) in enumerate(step) for x in srv.table[s, :-(-(p + m) // page)].tolist()]
+        assert sorted(used + srv.free[:srv.count.item()].tolist()) == list(range(pages))
+
+
+def test_a_captured_step(ctx):
+    """A step recorded once into a graph and replayed for other lengths: everything comes from the device."""
+    from fast_llm_b200 import capi as c_
+    own = c_.Context(0)
+    try:
+        srv = Server(own, 4, 20, 40, 16, 8, 2, 128, "f32", 300)
+        g = torch.Generator(device="cuda").manual_seed(1)
+        stream = torch.cuda.ExternalStream(own.stream())
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with pytest.raises(capi.Fl200Error) as e:          # the first call of a context allocates
+            with torch.cuda.graph(graph, stream=stream, capture_error_mode="thread_local"):
+                srv.cache.attn(srv.q, srv.table, srv.q_start, srv.held, 200, srv.scale, srv.out)
+        assert "capture" in str(e.value)
+        torch.cuda.synchronize()
+        srv.cache.attn(srv.q, srv.table, srv.q_start, srv.held, 200, srv.scale, srv.out)
+        own.sync()
+        assert own.status() == 0
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream, capture_error_mode="thread_local"):
+            srv.step(200)
+        for step in STEPS:
+            past, new = [p for p, _ in step], [m for _, m in step]
+            srv.rows.copy_(torch.randn(srv.rows.shape, generator=g, device="cuda"))
+            srv.past.copy_(ints(past))
+            srv.new.copy_(ints(new))
+            torch.cuda.synchronize()
+            with torch.cuda.stream(stream):
+                graph.replay()
+            torch.cuda.synchronize()
+            assert own.status() == 0
+            srv.check(past, new)
+        del graph
+    finally:
+        own.close()
+
+
+def test_calls_in_a_row_and_two_contexts(ctx):
+    """Calls of unlike shapes without a wait between them share the context's scratch; another context has its own."""
+    from fast_llm_b200 import paged
+    shapes = [([(900, 1), (300, 1)], 32, 8, 128, 16, "f32"), ([(700, 300)], 8, 2, 128, 64, "f32"), ([(50, 1), (400, 90)], 8, 8, 64, 32, "f16"), ([(5000, 4)], 4, 1, 128, 16, "f32"),
+              ([(300, 20)] * 9, 16, 8, 64, 16, "f32")]
+    cases = [make(30 + i, *s) for i, s in enumerate(shapes)]
+    other = capi.Context(0)
+    try:
+        for c, s in zip(cases, shapes):
+            c["caches"] = [paged.PagedCache(x, c["k"], c["v"], c["n_pages"], s[4], s[2], s[3]) for x in (ctx, other)]
+            c["outs"] = [torch.full_like(c["out_all"], CANARY) for _ in range(2)]
+        torch.cuda.synchronize()
+        for _ in range(6):
+            for i in (0, 1):
+                for c, s in zip(cases, shapes):
+                    c["caches"][i].attn(c["q"], c["table"], c["q_start"], c["kv_len"], c["max_new"], 0.1, c["outs"][i][:, :s[1] * s[3]])
+        ctx.sync()
+        other.sync()
+        assert ctx.status() == 0 and other.status() == 0
+        for c, (seqs, n_q, n_kv, dim, page, act) in zip(cases, shapes):
+            assert torch.equal(c["outs"][0], c["outs"][1])
+            c["out"], c["out_all"] = c["outs"][0][:, :n_q * dim], c["outs"][0]
+            want, tol, _ = expect(c, seqs, n_q, n_kv, dim, 0.1, act)
+            got = c["out"].double().view(-1, n_q, dim)
+            assert ((got[:c["n"]] - want[:c["n"]]).abs() <= tol[:c["n"]]).all()
+            assert (c["out"][c["n"]:] == CANARY).all()
+    finally:
+        other.close()
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_pools_past_32_bit_offsets(ctx, new):
+    """Pools of more than 2^32 bytes and 2^31 values: pages at their very end, read and written."""
+    from fast_llm_b200 import paged
+    n_kv, dim, page, n_q = 8, 128, 64, 32
+    n_pages = (1 << 31) // (n_kv * dim * page) + 70
+    k = torch.zeros((n_pages, n_kv, page, dim), device="cuda", dtype=torch.float16)
+    v = torch.zeros_like(k)
+    cache = paged.PagedCache(ctx, k, v, n_pages, page, n_kv, dim)
+    L = 200
+    table = ints([[n_pages - 1, n_pages - 3, 0, n_pages - 40]])
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x = torch.randn((L, (n_q + 2 * n_kv) * dim), generator=g, device="cuda")
+    slot = (table[0].long()[torch.arange(L, device="cuda") // page] * page + torch.arange(L, device="cuda") % page).int()
+    nq, nk = n_q * dim, n_kv * dim
+    q = torch.zeros((L, nq), device="cuda")
+    torch.cuda.synchronize()
+    cache.append(x[:, :nq], x[:, nq:nq + nk], x[:, nq + nk:], torch.arange(L, device="cuda", dtype=torch.int32), slot, q, freq_base=10000.0)
+    out = torch.zeros((new, nq), device="cuda")
+    cache.attn(q[L - new:], table, ints([0, new]), ints([L]), new, 0.088, out)
+    ctx.sync()
+    assert ctx.status() == 0
+    at = slot.long()
+    kk, vv = (t[at // page, :, at % page] for t in (k, v))
+    assert torch.equal(vv, x[:, nq + nk:].view(L, n_kv, dim).half()) and (kk != 0).any(-1).all()
+    c = dict(q=q[L - new:], ks=[kk.transpose(0, 1)], vs=[vv.transpose(0, 1)], start=[0, new])
+    want, tol, _ = expect(c, [(L, new)], n_q, n_kv, dim, 0.088, "f32")
+    assert ((out.double().view(new, n_q, dim) - want).abs() <= tol).all()
+
+
+def test_long_chunk_over_many_tiles(ctx):
+    """Many tiles per piece: contexts go out and come back a quarter at a time; one key outweighs all others late in the walk, so
+    that every sum changes its reference."""
+    n_q, n_kv, dim, page = 8, 1, 128, 64
+    for act in ("f32", "f16"):
+        seqs = [(9000, 70)]
+        c = make(77, seqs, n_q, n_kv, dim, page, act)
+        for j in (3000, 6500):       # keys along q's mean direction, far larger than the others
+            pg, r = int(c["table"][0, j // page]), j % page
+            big = (4 + j // 1000) * torch.sign(c["q"][0].view(n_q, dim)[0]).half()
+            c["k"][pg, 0, r] = big
+            c["ks"][0][0, j] = big
+        attn(ctx, c, n_q, n_kv, dim, page, 0.088)
+        check(ctx, c, seqs, n_q, n_kv, dim, 0.088, act)
