@@ -114,6 +114,13 @@ __device__ __forceinline__ void load32(uint32_t addr, float *r) {
         : "r"(addr)
         : "memory");
 }
+__device__ __forceinline__ void load16(uint32_t addr, float *r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]),
+                   "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+                 : "r"(addr)
+                 : "memory");
+}
 template <int N> __device__ __forceinline__ void wait_ld(float (&r)[N]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
@@ -442,6 +449,15 @@ __device__ __forceinline__ bool partly(const PagedAttnArgs &a, const Piece &p, u
 
 __device__ __forceinline__ void bar_both() { asm volatile("bar.sync 1, 256;" ::: "memory"); }   // the softmax warps
 
+// The rows of q of a piece to L2 (a warp).
+template <int D, int Parts>
+__device__ __noinline__ void prefetch_q(const PagedAttnArgs &a, const Piece p) {
+    for (uint32_t i = threadIdx.x & 31u; i < p.b.rows; i += 32) {
+        const uint32_t at = p.blk * 2 * kRowsL + i, tok = at / a.group, head = p.hkv * a.group + at - tok * a.group;
+        const uint8_t *from = static_cast<const uint8_t *>(a.q) + ((p.q.first + tok) * a.q_stride + (uint64_t)head * D) * (2 * Parts);
+        for (uint32_t c = 0; c < D * 2 * Parts; c += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(from + c));
+    }
+}
 struct Sums { float ref, sum, highest, acc_ref; uint32_t out_of; };   // of a row
 // The factor of contexts that were summed over that many tiles (8 instructions per tile and part).
 __device__ __forceinline__ float given_back(uint32_t tiles) { return fmaf(8.f * kLoss, (float)tiles, 1.f); }
@@ -488,51 +504,44 @@ __device__ __noinline__ void finish(const PagedAttnArgs &a, Head &hd, uint8_t *q
         // Rows go out through shared memory, where the lane's q was (a small block's lanes share the first q; the second is free).
         uint8_t *stage = q_s + (sm ? 1 : l) * Parts * T::kPart;
         const bool any_unfinite = hd.any_unfinite != 0;
+        // 16 columns at a time (32 spill, and local memory is L2 here)
+        struct Part { uint32_t at; const float4 *mem; uint32_t out; float keep; uint32_t steps; };
+        const Part part1{to, acc_mem, s.out_of, s.acc_ref == ref ? 1.f : exp2_fast(s.acc_ref - ref), sm ? (job.n + 1) / 2 : job.n};
+        const Part part2{to + 128, acc_mem + T::kRecord / 4, out2, acc2_ref == ref2 ? 1.f : exp2_fast(acc2_ref - ref2), job.n / 2};
+        auto add_part = [&](const Part &p, int c, float w, float (&v)[16]) {   // v += w times the contexts of columns 16 c ..
+            float o[16];
+            load16(p.at + 16 * c, o);
+            const bool acc = Parts == 2 && (p.out >> (c / 2) & 1u);
+            float4 old[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) old[j] = acc ? __ldcg(p.mem + (4 * c + j) * kRowsL) : make_float4(0.f, 0.f, 0.f, 0.f);
+            const float back = Parts == 2 ? w * given_back(tiles_since(p.steps, c / 2, acc)) : w, keep = w * p.keep;
+            wait_ld(o);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = fmaf(o[j], back, v[j]);
+            if (acc)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    v[4 * j] = fmaf(old[j].x, keep, v[4 * j]); v[4 * j + 1] = fmaf(old[j].y, keep, v[4 * j + 1]);
+                    v[4 * j + 2] = fmaf(old[j].z, keep, v[4 * j + 2]); v[4 * j + 3] = fmaf(old[j].w, keep, v[4 * j + 3]);
+                }
+        };
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-            float o[32];
-            auto lane_part = [&](uint32_t from, const float4 *mem, uint32_t out, float before, float rf, uint32_t steps) {   // 32 columns of a lane's contexts
-                load32(from + 32 * c, o);
-                const bool acc = Parts == 2 && (out >> c & 1u);
-                float4 old[8];
-                if (acc)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) old[j] = __ldcg(mem + (8 * c + j) * kRowsL);
-                wait_ld(o);
-                if (Parts == 2) {
-                    const float back = given_back(tiles_since(steps, c, acc));
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) o[j] *= back;
-                }
-                if (acc) {
-                    const float keep = before == rf ? 1.f : exp2_fast(before - rf);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        o[4 * j] = fmaf(old[j].x, keep, o[4 * j]); o[4 * j + 1] = fmaf(old[j].y, keep, o[4 * j + 1]);
-                        o[4 * j + 2] = fmaf(old[j].z, keep, o[4 * j + 2]); o[4 * j + 3] = fmaf(old[j].w, keep, o[4 * j + 3]);
-                    }
-                }
-            };
-            float v[32];
-            if (two) {
-                lane_part(to + 128, acc_mem + T::kRecord / 4, out2, acc2_ref, ref2, job.n / 2);
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = o[j] * w2;
-            }
-            lane_part(to, acc_mem, s.out_of, s.acc_ref, ref, sm ? (job.n + 1) / 2 : job.n);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = two ? fmaf(o[j], w1, v[j]) : o[j];
+        for (int c = 0; c < D / 16; ++c) {
+            float v[16] = {};
+            add_part(part1, c, two ? w1 : 1.f, v);
+            if (two) add_part(part2, c, w2, v);
             if (any_unfinite)
 #pragma unroll 1
-                for (int j = 0; j < 32; ++j) {
-                    const float u = unfinite_at(hd.unfinite, D, 32 * c + j, lim);
+                for (int j = 0; j < 16; ++j) {
+                    const float u = unfinite_at(hd.unfinite, D, 16 * c + j, lim);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] += i == j ? u : 0.f;
+                    for (int i = 0; i < 16; ++i) v[i] += i == j ? u : 0.f;
                 }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                if (!whole) __stcg(reinterpret_cast<float4 *>(rec) + (8 * c + j) * kRowsL + r, make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
-                else stage_put<D, Parts>(stage, r, 8 * c + j, make_float4(v[4 * j] * inv, v[4 * j + 1] * inv, v[4 * j + 2] * inv, v[4 * j + 3] * inv));
+            for (int j = 0; j < 4; ++j) {
+                if (!whole) __stcg(reinterpret_cast<float4 *>(rec) + (4 * c + j) * kRowsL + r, make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+                else stage_put<D, Parts>(stage, r, 4 * c + j, make_float4(v[4 * j] * inv, v[4 * j + 1] * inv, v[4 * j + 2] * inv, v[4 * j + 3] * inv));
             }
         }
         const float from = two ? both : ref, total_sum = two ? all : sum;
@@ -645,6 +654,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
     }
     if (blockIdx.x >= sh.n) return;
     const bool some = first_piece(a, walk, p) || next_piece(a, walk, p);   // (a share may lie within a block's front)
+    if (warp == kValueWarp && some) prefetch_q<D, Parts>(a, p);
     __syncthreads();
     for (uint32_t i = tid; i < 3 * D; i += kThreads) hd.unfinite[i] = 0x7fffffffu;
     if (warp == kTensorWarp) {
@@ -818,12 +828,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
             {   // the next piece's rows of q to L2
                 Walk w2 = walk;
                 Piece p2 = p;
-                if (next_piece(a, w2, p2))
-                    for (uint32_t i = lane; i < p2.b.rows; i += 32) {
-                        const uint32_t at = p2.blk * 2 * kRowsL + i, tok = at / a.group, head = p2.hkv * a.group + at - tok * a.group;
-                        const uint8_t *from = static_cast<const uint8_t *>(a.q) + ((p2.q.first + tok) * a.q_stride + (uint64_t)head * D) * (2 * Parts);
-                        for (uint32_t c = 0; c < D * 2 * Parts; c += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(from + c));
-                    }
+                if (next_piece(a, w2, p2)) prefetch_q<D, Parts>(a, p2);
             }
             const int32_t lim_first = p.q.past + (int32_t)(p.blk * 2 * kRowsL / a.group);
             for (uint32_t t = 0; t < n; ++t, ++v_seen) {
