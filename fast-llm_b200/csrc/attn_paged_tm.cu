@@ -236,22 +236,21 @@ template <int Parts> __device__ __forceinline__ void exp_chunk(const float (&s)[
     if (Parts == 2) store16(at + 16, pl);
 }
 
-// The 32 rows of a warp from global memory, as f16 parts into shared memory (K-major, 128-byte swizzle), every row times a power of two that
-// brings its largest value to [2^11, 2^12): 8 lanes a row, 4 rows at a time. src: of the thread's own row; returns what its scores are to be
-// multiplied by (exponents of 2).
+// 32 rows (16, half) from global memory, as f16 parts into shared memory (K-major, 128-byte swizzle), every row times a power of two that
+// brings its largest value to [2^11, 2^12): 8 lanes a row, rows i, i + 4, i + 8, i + 12 at a time, whose lines lie in both halves of the
+// banks. A warp; lane t has row row0 + t: src is where that begins; returns what its scores are to be multiplied by (exponents of 2).
 template <int D, int Parts>
-__device__ __noinline__ float load_q(const PagedAttnArgs &a, uint8_t *dst, uint64_t src, uint32_t row0, uint32_t rows, bool store) {
+__device__ __noinline__ float load_q(const PagedAttnArgs &a, uint8_t *dst, uint64_t src, uint32_t row0, uint32_t rows, bool half) {
     constexpr int V = 4, K = D / 32, kBatch = 4;   // values of a load, loads of a lane and row, groups of 4 rows in flight
     const uint32_t lane = threadIdx.x & 31u, sub = lane & 7u, group = lane >> 3;
-    if (row0 + lane < rows)   // (the second half's rows come to L2 beside the first's)
-        for (uint32_t c = 0; c < D * 2 * Parts; c += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint8_t *>(a.q) + src * (2 * Parts) + c));
+    auto row_of = [&](uint32_t i) { return (i & 3u) + 4 * group + 16 * (i >> 2); };
     float f = 0.f;
 #pragma unroll 1
-    for (uint32_t i0 = 0; i0 < 8; i0 += kBatch) {
+    for (uint32_t i0 = 0; i0 < (half ? 4u : 8u); i0 += kBatch) {
         float x[kBatch][K][V];
 #pragma unroll
         for (uint32_t i = 0; i < kBatch; ++i) {
-            const uint32_t rr = (i0 + i) + 8 * group;   // (rows 8 apart: their lines of shared memory are permuted alike, in banks of their own)
+            const uint32_t rr = row_of(i0 + i);
             const uint64_t at = __shfl_sync(0xffffffffu, src, rr);
             const bool there = row0 + rr < rows;
 #pragma unroll
@@ -269,7 +268,7 @@ __device__ __noinline__ float load_q(const PagedAttnArgs &a, uint8_t *dst, uint6
         }
 #pragma unroll
         for (uint32_t i = 0; i < kBatch; ++i) {
-            const uint32_t rw = (i0 + i) + 8 * group, rr = row0 + rw;
+            const uint32_t rr = row0 + row_of(i0 + i);
             float top = 0.f;
 #pragma unroll
             for (int k = 0; k < K; ++k)
@@ -280,10 +279,9 @@ __device__ __noinline__ float load_q(const PagedAttnArgs &a, uint8_t *dst, uint6
             const int e = min(100, max(-100, 138 - (int)(__float_as_uint(top) >> 23)));
             const float up = __uint_as_float((uint32_t)(e + 127) << 23);
             const float mine = fmaxf(a.scale * (float)(1.44269504088896341 * (1.0 + (Parts == 2 ? D / 32 * (double)kLoss : 0.0))) * __uint_as_float((uint32_t)(127 - e) << 23), 1e-37f);
-            // thread t's row is t: group t / 8's at i = t % 8
-            const float got = __shfl_sync(0xffffffffu, mine, lane & 24u);
-            if ((lane & 7u) == i0 + i) f = got;
-            if (store) {
+            const float got = __shfl_sync(0xffffffffu, mine, (lane >> 2 & 3u) * 8);
+            if ((lane & 3u) + 4 * (lane >> 4) == i0 + i) f = got;
+            {
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
                     const uint32_t d = (8 * k + sub) * V;
@@ -654,7 +652,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
     }
     if (blockIdx.x >= sh.n) return;
     const bool some = first_piece(a, walk, p) || next_piece(a, walk, p);   // (a share may lie within a block's front)
-    if (warp == kValueWarp && some) prefetch_q<D, Parts>(a, p);
     __syncthreads();
     for (uint32_t i = tid; i < 3 * D; i += kThreads) hd.unfinite[i] = 0x7fffffffu;
     if (warp == kTensorWarp) {
@@ -820,6 +817,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
     } else if (warp == kValueWarp) {
         // ---- values that must not meet the tensor cores ----
         uint32_t v_seen = 0;
+        if (some) prefetch_q<D, Parts>(a, p);
         for (bool more = some; more && !dead; more = next_piece(a, walk, p)) {
             const uint32_t n = p.t1 - p.t0;
             const bool sm = small(p);
@@ -926,7 +924,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
             const bool there = r < rows, active = w4 * 32 < rows;
             const int32_t lim = there ? job.past + (int32_t)tok : 0x7fffffff;   // (what a row that is not there comes to stays in it)
             float f = 0.f;
-            if (!dead && active) f = load_q<D, Parts>(a, q_s + (sm ? 0 : l) * Parts * T::kPart, (job.first + tok) * a.q_stride + (uint64_t)head * D, w4 * 32, rows, !sm || l == 0);
+            if (!sm) {
+                if (!dead && active) f = load_q<D, Parts>(a, q_s + l * Parts * T::kPart, (job.first + tok) * a.q_stride + (uint64_t)head * D, w4 * 32, rows, false);
+            } else {
+                // one q for both lanes: 16 rows a warp; the factors by way of memory
+                const uint32_t at = job.row0 + warp * 16 + (lane & 15u), t = at / a.group, h = job.hkv * a.group + at - t * a.group;
+                float *f_mem = a.part_tm + ((uint64_t)gridDim.x * 4 + blockIdx.x * 2) * T::kRecord + D * kRowsL;
+                if (!dead && warp * 16 < rows) {
+                    const float mine = load_q<D, Parts>(a, q_s, (job.first + t) * a.q_stride + (uint64_t)h * D, warp * 16, rows, true);
+                    if (lane < 16) __stcg(f_mem + warp * 16 + lane, mine);
+                }
+                bar_both();
+                if (active) f = __ldcg(f_mem + r);
+            }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) arrive(&hd.q_full);
