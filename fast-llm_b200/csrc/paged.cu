@@ -126,8 +126,11 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs
             const uint32_t s = find_in(tok, a.n_seq, i), p = (uint32_t)a.past[s] + (i - tok[s]), j = p >> a.page_shift,
                            have = pages_of((uint32_t)a.held[s]);
             const int32_t page = j < have ? a.table[(uint64_t)s * a.max_blocks + j] : popped(take[s] + j - have);
+            // (a page whose slots 31 bits do not hold would come out as another page's)
+            const bool there = (uint32_t)page <= 0x7fffffffu >> a.page_shift;
+            if (!there) atomicCAS(a.status, ST_OK, ST_PAGED_PAGE);
             a.pos[i] = (int32_t)p;
-            a.slot[i] = (int32_t)(((uint32_t)page << a.page_shift) | (p & round_up));
+            a.slot[i] = there ? (int32_t)(((uint32_t)page << a.page_shift) | (p & round_up)) : -1;
         }
     }
     for (uint32_t i = n_tok + gthread; i < a.max_tokens; i += threads) { a.pos[i] = -1; a.slot[i] = -1; }

@@ -228,7 +228,7 @@ enum { FL_B200_ACT_F32 = 0, FL_B200_ACT_F16 = 1 };
  * free_count_in itself), q_start[n_seq + 1] = first token of each sequence in the step's batch, kv_len[s] = past + fresh (may be held,
  * past or fresh itself), and per token of the batch its position and its slot; the rest of pos and slot (max_tokens
  * each) is -1. Where pages or max_tokens do not suffice (status 5) or lengths are impossible (status 4) the plan is empty: q_start 0, every
- * pos and slot -1, all else unchanged. No page may be listed twice. Other buffers must not overlap. */
+ * pos and slot -1, all else unchanged. A token on a page that no pool has (negative, or past 2^31 rows) gets slot -1 (status 3). No page may be listed twice. Other buffers must not overlap. */
 int fl_b200_paged_plan(fl_b200_ctx *ctx, const int32_t *held_dev, const int32_t *past_dev, const int32_t *fresh_dev,
                        uint32_t n_seq, uint32_t page_size, int32_t *table_dev, uint32_t max_blocks, int32_t *free_list_dev,
                        uint32_t n_pages, const int32_t *free_count_in_dev, int32_t *free_count_out_dev, int32_t *q_start_dev,

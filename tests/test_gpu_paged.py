@@ -413,6 +413,19 @@ def test_plan_refuses_impossible_lengths(ctx, held, past, new, count):
     assert got == dict(table=table, free=free, count=count, pos=[-1] * 3, slot=[-1] * 3, start=[0, 0], length=[-9])
 
 
+@pytest.mark.parametrize("page", [16, 256])
+@pytest.mark.parametrize("wrong", [-1, 1 << 28, (1 << 31) - 1, -(1 << 31)])
+def test_plan_of_pages_that_no_pool_has(ctx, page, wrong):
+    """Their slots are -1, not another page's whose number is the same in 31 bits."""
+    n = page + 3
+    got = run_plan(ctx, [n, n], [n, n], [1, 1], [[1, wrong], [2, 0]], [3, 4], 2, page, 3)          # a page held
+    assert ctx.status() == 3
+    assert got["slot"] == [-1, 3, -1] and got["pos"] == [n, n, -1] and got["length"] == [n + 1, n + 1]
+    got = run_plan(ctx, [page, n], [page, n], [2, 1], [[1, -9], [2, 0]], [3, wrong], 2, page, 3)   # a page taken
+    assert ctx.status() == 3
+    assert got["slot"] == [-1, -1, 3] and got["table"] == [[1, wrong], [2, 0]] and got["count"] == 1
+
+
 # ---- together ----------------------------------------------------------------------------------------------------------------
 
 
