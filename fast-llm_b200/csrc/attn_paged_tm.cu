@@ -592,8 +592,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
     if (a.n_seq <= 32) {
         const PagedSeq q = lane < a.n_seq ? paged_seq(a, lane, bad) : PagedSeq{0, 0, 0};
         const uint64_t mine = head_units(a, q, lane) * a.n_kv;
-        bad |= mine >> 26 != 0;   // (32 of them stay below 2^32)
-        const uint32_t u = mine >> 26 ? 0u : (uint32_t)mine;
+        const bool fits = __reduce_add_sync(0xffffffffu, (uint32_t)min(mine >> 16, (uint64_t)0x10000u) + 1u) <= 0x10000u;   // (then all of them stay below 2^32)
+        bad |= !fits;
+        const uint32_t u = fits ? (uint32_t)mine : 0u;
         uint32_t x = u;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {

@@ -622,6 +622,30 @@ def test_pools_past_32_bit_offsets(ctx, new):
     assert ((out.double().view(new, n_q, dim) - want).abs() <= tol).all()
 
 
+def test_a_prompt_of_131072_tokens(ctx):
+    """One sequence of 2^26 tiles and more: shares and owners of tiles past 32-bit products."""
+    from fast_llm_b200 import paged
+    N, n_q, dim, page = 131072, 128, 64, 256
+    g = torch.Generator(device="cuda").manual_seed(12)
+    k, v = (torch.randn((N // page, 1, page, dim), generator=g, device="cuda").half() for _ in range(2))
+    table = torch.randperm(N // page, generator=g, device="cuda").int().view(1, -1)
+    q = torch.empty((N, n_q * dim), device="cuda", dtype=torch.float16).normal_(generator=g)
+    out = torch.full_like(q, CANARY)
+    cache = paged.PagedCache(ctx, k, v, N // page, page, 1, dim)
+    torch.cuda.synchronize()
+    cache.attn(q, table, ints([0, N]), ints([N]), N, 0.125, out)
+    ctx.sync()
+    assert ctx.status() == 0
+    kk, vv = (t[table[0].long()].reshape(N, dim).double() for t in (k, v))
+    for tok in (0, 1, 2, 127, 128, 4097, 65535, 65536, 100001, N - 2, N - 1):
+        x = q[tok].double().view(n_q, dim) @ kk[:tok + 1].t() * 0.125
+        A = (q[tok].double().abs().view(n_q, dim) @ kk[:tok + 1].abs().t() * 0.125).amax(-1, keepdim=True)
+        p = torch.softmax(x, -1)
+        want, spread = p @ vv[:tok + 1], p @ vv[:tok + 1].abs()
+        tol = (A + 1) * 2.0 ** -18 * spread + 2.0 ** -11 * spread + 2.0 ** -11 * want.abs() + 2.0 ** -25
+        assert ((out[tok].double().view(n_q, dim) - want).abs() <= tol).all(), tok
+
+
 def test_long_chunk_over_many_tiles(ctx):
     """Many tiles per piece: contexts go out and come back a quarter at a time; one key outweighs all others late in the walk, so
     that every sum changes its reference."""
