@@ -399,7 +399,8 @@ int fl_b200_paged_attn(fl_b200_ctx *c, const fl_b200_paged_cache *cache, int act
         return set_err(FL_B200_ERR_ARG, "paged_attn: table, q_start or kv_len is null or misaligned");
     if (!aligned(lse_out, 8)) return set_err(FL_B200_ERR_ARG, "paged_attn: lse_out must be 8-byte aligned");
     if (n_seq == 0 || n_seq > kPagedMaxSeq) return set_err(FL_B200_ERR_ARG, "paged_attn: %u sequences (1 to %u)", n_seq, kPagedMaxSeq);
-    if (max_blocks == 0 || ((uint64_t)max_blocks << shift) >= (1ull << 31)) return set_err(FL_B200_ERR_ARG, "paged_attn: %u blocks a sequence", max_blocks);
+    // (a tile of the last key ends within 31 bits)
+    if (max_blocks == 0 || ((uint64_t)max_blocks << shift) > (1ull << 31) - 256) return set_err(FL_B200_ERR_ARG, "paged_attn: %u blocks a sequence", max_blocks);
     if (n_tokens == 0 || (uint64_t)n_tokens * (n_q / n_kv) >= (1ull << 31)) return set_err(FL_B200_ERR_ARG, "paged_attn: %u tokens", n_tokens);
     if (max_new == 0 || max_new > n_tokens) return set_err(FL_B200_ERR_ARG, "paged_attn: max_new %u of %u tokens", max_new, n_tokens);
     if (!(std::isfinite(scale) && scale > 0.f)) return set_err(FL_B200_ERR_ARG, "paged_attn: scale %g (positive)", (double)scale);

@@ -246,7 +246,7 @@ int fl_b200_paged_append(fl_b200_ctx *ctx, const fl_b200_paged_cache *cache, int
 /* Causal grouped-query attention of every sequence's new tokens over its pages: fl_b200_attn_decode, fl_b200_attn_verify and prompt chunks in
  * one call. Sequence s has tokens q_start[s] .. q_start[s + 1] - 1 of the batch and kv_len[s] keys, its new tokens' own
  * the last of them; token i of n attends keys 0 .. kv_len - n + i. A token without a key gets zeros. n_q_head is a multiple of
- * n_kv_head (groups of up to 128), q and out [n_tokens][stride] as above, table [n_seq][max_blocks], scale positive. n_tokens: rows of q and
+ * n_kv_head (groups of up to 128), q and out [n_tokens][stride] as above, table [n_seq][max_blocks] (max_blocks * page_size <= 2^31 - 256), scale positive. n_tokens: rows of q and
  * out; max_new: the most new tokens any sequence has. Sequences whose lengths break these bounds are left out (status 4), and so are
  * prompts of together 2^31 or more tiles of 256 rows by 128 keys (a minute's work); rows of
  * out that belong to no sequence stay as they are, keys on a page outside the pool count as zero vectors (status 3). lse_out

@@ -88,3 +88,10 @@ def test_rows_of_bad_pages_stay_outside_the_pool():
                 for row in (0, (1 << shift) - 8):
                     at = (u * n_kv + hkv) * groups + (row >> 3) if u < n_pages else outside
                     assert at <= outside and (at < outside) == (0 <= page < n_pages)
+
+
+@pytest.mark.parametrize("page", [16, 64, 128, 256])
+def test_attn_refuses_tables_whose_last_tile_ends_past_31_bits(lib, page):
+    change = dict(cache=cache(page=page), blocks=((1 << 31) - 256) // page + 1)
+    assert call(lib, "fl_b200_paged_attn", dict(ATTN, **change).values()) == 1
+    assert b"blocks" in lib.fl_b200_last_error()
