@@ -77,14 +77,6 @@ template <int D> struct FewSmem {
     uint32_t start_seq, start_off, last, any_unfinite, abort_flag;
 };
 
-// Values of +inf, -inf and NaN (class 0, 1, 2) among the keys that only part of the rows attend: per class and dimension the
-// first such key. A row that attends keys 0 .. lim is affected by those <= lim.
-__device__ __forceinline__ float unfinite_of(const uint32_t *u, uint32_t dims, uint32_t d, int32_t lim) {
-    const int32_t p = (int32_t)u[d], n = (int32_t)u[dims + d], x = (int32_t)u[2 * dims + d];   // (0x7fffffff: none)
-    if (x <= lim || (p <= lim && n <= lim)) return __int_as_float(0x7fffffff);
-    return p <= lim ? INFINITY : n <= lim ? -INFINITY : 0.f;
-}
-
 __device__ __forceinline__ void bar_consumers() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 __device__ __forceinline__ void arrive(uint64_t *bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory"); }
 __device__ __forceinline__ void prefetch_map(const CUtensorMap *m) { asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory"); }
@@ -554,7 +546,11 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
         if (!whole) {
             fence_acq_rel_gpu();
             bar_consumers();
-            if (tid == 0) sm.last = !sm.abort_flag && atomicAdd(&a.tickets[c0], 1u) == pieces - 1 ? 1u : 0u;
+            if (tid == 0) {   // (the ticket is the next launch's again whatever became of this one)
+                const bool last = atomicAdd(&a.tickets[c0], 1u) == pieces - 1;
+                if (last) a.tickets[c0] = 0;
+                sm.last = last && !sm.abort_flag;
+            }
         }
         bar_consumers();   // (also: everybody has read the unfinite values)
         if (sm.any_unfinite) {
@@ -565,7 +561,6 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
         if (!whole && sm.last) {
             fence_acq_rel_gpu();
             combine<D>(a, sm, p.q, p.hkv, p.rows, c0, pieces, p.base <= share_lo(sh, c0));
-            if (tid == 0) a.tickets[c0] = 0;
         }
         bar_consumers();   // the shared arrays are free for the next piece
     } while (next_piece(a, walk, p));

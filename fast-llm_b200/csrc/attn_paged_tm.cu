@@ -16,8 +16,9 @@
 //   values  (1 warp)     : V tiles that hold keys which only part of the rows attend: keys behind the last are cleared, values that
 //                          are not finite are taken out and noted (0 x NaN; see unfinite_of)
 // While one lane's softmax runs the tensor cores work for the other: a block of more than 128 rows gives each lane 128 of them over the same
-// tiles; a smaller block gives both lanes its rows, every other tile each, and their results are added as two records.
-// Tiles of all blocks lie on one line (sequence, KV head, block, tile); shares, records and tickets as in attn_paged.cu.
+// tiles; a smaller block gives both lanes its rows, every other tile each, and their results are added in tensor memory.
+// Tiles of all blocks lie on one line (sequence, KV head, block, tile) and every CTA takes an equal piece of it; the records of a block that
+// several CTAs share are added by a launch of its own behind.
 //
 // The tensor cores truncate their running sum, 3.1e-8 of it per instruction (see kLoss); with f32 activations a part of 32 columns of O is therefore
 // brought out at every tile, in turn, added in f32 to a buffer of the CTA's own that stays in L2, and starts from zero: no sum in
@@ -73,12 +74,6 @@ struct Head {
     union { uint32_t unfinite[3 * 128]; uint64_t sum[kThreads / 32]; };   // (the sums while the share is found)
 };
 static_assert(sizeof(Head) <= 2048, "head");
-
-__device__ __forceinline__ float unfinite_at(const uint32_t *u, uint32_t dims, uint32_t d, int32_t lim) {   // attn_paged.cu's unfinite_of
-    const int32_t p = (int32_t)u[d], n = (int32_t)u[dims + d], x = (int32_t)u[2 * dims + d];
-    if (x <= lim || (p <= lim && n <= lim)) return __int_as_float(0x7fffffff);
-    return p <= lim ? INFINITY : n <= lim ? -INFINITY : 0.f;
-}
 
 __device__ __forceinline__ bool try_bar(uint64_t *bar, uint32_t parity) { return mbar_try_wait(bar, parity); }
 // A warp's wait: at most a second, and no longer once another role has given up.
@@ -535,7 +530,7 @@ __device__ __noinline__ void finish(const PagedAttnArgs &a, Head &hd, uint8_t *q
             if (any_unfinite)
 #pragma unroll 1
                 for (int j = 0; j < 16; ++j) {
-                    const float u = unfinite_at(hd.unfinite, D, 16 * c + j, lim);
+                    const float u = unfinite_of(hd.unfinite, D, 16 * c + j, lim);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) v[i] += i == j ? u : 0.f;
                 }
@@ -914,7 +909,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
                         j.first = x.q.first; j.row0 = x.blk * 2 * kRowsL; j.rows = x.b.rows; j.hkv = x.hkv; j.past = x.q.past;
                         j.whole = c0 == c1;
                         j.slot = j.slot == 2 ? 0 : 1;
-                        if (!j.whole && c0 == blockIdx.x) a.blocks[c0] = PagedTmBlock{c1 - c0 + 1, j.sm, j.slot, j.first, j.row0, j.rows, j.hkv, j.past};
+                        if (!j.whole && c0 == blockIdx.x) a.blocks[c0] = PagedTmBlock{c1 - c0 + 1, j.slot, j.first, j.row0, j.rows, j.hkv, j.past};
                     }
                 }
             }

@@ -15,10 +15,10 @@ constexpr uint32_t kPagedMaxSeq = 4096;   // sequences of a call: the plan keeps
 // Rows: row r of a sequence with n new tokens is token r / group, query head hkv * group + r % group (group = n_q_head / n_kv_head).
 // Token i of n attends keys 0 .. kv_len - n + i. A block of rows over one KV head walks tiles of keys; the tiles of all blocks lie
 // on one line and every CTA takes an equal, contiguous piece of it, so that ragged batches load all SMs alike. A block that several
-// CTAs share leaves one record per CTA; the CTA that arrives last adds them in order (no CTA waits for another).
+// CTAs share leaves one record per CTA; the CTA that arrives last, or the launch behind, adds them in order (no CTA waits for another).
 // A block that several CTAs of attn_paged_tm.cu share, noted by the one that begins it.
 struct PagedTmBlock {
-    uint32_t records, sm, slot, first, row0, rows, hkv;   // records: CTAs; 0: none. slot: of the first CTA's record
+    uint32_t records, slot, first, row0, rows, hkv;   // records: CTAs; 0: none. slot: of the first CTA's record
     int32_t past;
 };
 struct PagedAttnArgs {
@@ -29,7 +29,7 @@ struct PagedAttnArgs {
     const int32_t *table, *q_start, *kv_len;
     float *part, *part_tm;          // records
     PagedTmBlock *blocks;           // one per CTA
-    uint32_t *tickets;              // zero between launches
+    uint32_t *tickets;              // zero between launches (attn_paged.cu)
     uint32_t *status;
     uint64_t q_stride, out_stride;  // elements between tokens
     uint32_t n_seq, max_blocks, n_tokens, max_new, n_pages, page_shift;
@@ -67,6 +67,14 @@ __device__ __forceinline__ uint32_t share_lo(const Shares &s, uint32_t c) { retu
 __device__ __forceinline__ uint32_t owner_of(const Shares &s, uint32_t u) {   // the CTA whose share holds unit u
     const uint32_t front = s.more * (s.each + 1);
     return u < front ? u / (s.each + 1) : s.more + (u - front) / s.each;
+}
+
+// Values of +inf, -inf and NaN (class 0, 1, 2) among the keys that only part of the rows attend: per class and dimension the
+// first such key. A row that attends keys 0 .. lim is affected by those <= lim.
+__device__ __forceinline__ float unfinite_of(const uint32_t *u, uint32_t dims, uint32_t d, int32_t lim) {
+    const int32_t p = (int32_t)u[d], n = (int32_t)u[dims + d], x = (int32_t)u[2 * dims + d];   // (0x7fffffff: none)
+    if (x <= lim || (p <= lim && n <= lim)) return __int_as_float(0x7fffffff);
+    return p <= lim ? INFINITY : n <= lim ? -INFINITY : 0.f;
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {   // 2^x to 2^-22 of its value, 0 for -inf

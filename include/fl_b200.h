@@ -249,7 +249,8 @@ int fl_b200_paged_append(fl_b200_ctx *ctx, const fl_b200_paged_cache *cache, int
  * n_kv_head (groups of up to 128), q and out [n_tokens][stride] as above, table [n_seq][max_blocks] (max_blocks * page_size <= 2^31 - 256), scale positive. n_tokens: rows of q and
  * out; max_new: the most new tokens any sequence has. Sequences whose lengths break these bounds are left out (status 4), and so are
  * prompts of together 2^31 or more tiles of 256 rows by 128 keys (a minute's work); rows of
- * out that belong to no sequence stay as they are, keys on a page outside the pool count as zero vectors (status 3). lse_out
+ * out that belong to no sequence stay as they are, keys on a page outside the pool count as zero vectors (status 3). What a row does not attend may hold
+ * anything; an infinity that it does attend may make it NaN. lse_out
  * (optional): per token and query head (max score, sum of exp(score - max)), (-inf, 0) without a key: what fl_b200_seqpar_combine merges.
  * f32 activations: q and the probabilities go to the tensor cores as two f16 parts each (22 bits), sums in f32; f16
  * activations: as one. out must not overlap q. The first call on a context allocates scratch (65 MB): make it before a capture. */
