@@ -65,16 +65,24 @@ __device__ __forceinline__ bool next_piece(const PagedAttnArgs &a, Walk &w, Piec
     return true;
 }
 
+// A sequence over one KV head whose last record was this CTA's.
+struct Late {
+    PagedSeq q;
+    uint32_t hkv, rows, c0, pieces;
+    bool c0_first;      // of CTA c0 the first record is meant
+};
+
 template <int D> struct FewSmem {
     static constexpr uint32_t kHalfStage = kTile * D * 2;                 // K or V of a tile
     uint8_t ring[kStages][2 * kHalfStage];                                // 1024-byte aligned
-    float o[kWarps * kRowsB * 36];                                        // q as operands; the warps' contexts, a part at a time; records' maxima and sums
+    float o[kWarps * kRowsB * 36];                                        // q as operands; the warps' contexts, a part at a time
     float f[kRowsB];                                                      // score -> exponent of 2
     float m[kWarps][kRowsB], l[kWarps][kRowsB];
     uint32_t unfinite[3][D];                                              // see unfinite_of
     uint64_t full[kStages], empty[kStages];
     uint64_t sum[kThreads / 32];
-    uint32_t start_seq, start_off, last, any_unfinite, abort_flag;
+    uint32_t start_seq, start_off, any_unfinite, abort_flag, n_late;
+    Late late[2];                                                         // (a CTA shares two at most: its first and its last)
 };
 
 __device__ __forceinline__ void bar_consumers() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
@@ -160,56 +168,59 @@ __device__ __forceinline__ void copy_tiles(const PagedAttnArgs &a, FewSmem<D> &s
 }
 
 // The records of a sequence over one KV head, added in order: of CTA c0 the piece at its end (or its first), of the others the one at
-// their start. First the records' weights, a warp a row and a lane a record, then the contexts, eight loads of a thread in flight. This is the
-// launch's tail, and run once: its time is round trips to L2 and the fetching of its instructions, so it is kept short and out of line.
+// their start. This is the launch's tail: its time is round trips to L2, so that as many records as the ring holds, which is free by then, are
+// copied into it at once (16 rows, 37 records: two loads of a row in registers 42 us for the whole call). Run once, so out of line.
 template <int D>
-__device__ __noinline__ void combine(const PagedAttnArgs &a, FewSmem<D> &sm, const PagedSeq q, uint32_t hkv, uint32_t rows, uint32_t c0, uint32_t pieces, bool c0_first) {
-    constexpr uint32_t kFlight = 8, kRecord = kRowsB * (D + 4), kChunks = D / 4;
-    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, at_once = min(rows, (uint32_t)(sizeof(sm.o) / sizeof(float)) / pieces);
-    const float *rec = a.part + (uint64_t)c0 * 2 * kRecord;   // record i >= 1 at rec + 2 i kRecord
-    const uint32_t rec0 = c0_first ? 0 : kRecord;
-    for (uint32_t r0 = 0; r0 < rows; r0 += at_once) {
-        const uint32_t nr = min(at_once, rows - r0);
-#pragma unroll 1
-        for (uint32_t x = warp; x < nr; x += kWarps) {
-            const uint32_t ml_at = (r0 + x) * (D + 4) + D;
-            float top = -INFINITY, sum = 0.f;
-#pragma unroll 1
-            for (uint32_t k = lane; k < pieces; k += 32) top = fmaxf(top, __ldcg(rec + (k ? 2 * k * kRecord : rec0) + ml_at));
-            top = warp_max(top);
-#pragma unroll 1
-            for (uint32_t k = lane; k < pieces; k += 32) {
-                const float2 ml = __ldcg(reinterpret_cast<const float2 *>(rec + (k ? 2 * k * kRecord : rec0) + ml_at));
-                const float w = weight(ml.x, top);
-                sm.o[x * pieces + k] = w;
-                sum = fmaf(ml.y, w, sum);
+__device__ __noinline__ void combine(const PagedAttnArgs &a, FewSmem<D> &sm, const Late late) {
+    constexpr uint32_t kRecord = kRowsB * (D + 4), kChunks = D / 4, kThr = kWarps * 32, kItems = kRowsB * kChunks / kThr;
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, len = late.rows * (D + 4);
+    const uint32_t at_once = (uint32_t)(sizeof(sm.ring) / sizeof(float)) / len;
+    const float *rec = a.part + (uint64_t)late.c0 * 2 * kRecord;   // record i >= 1 at rec + 2 i kRecord
+    const float *in = reinterpret_cast<const float *>(sm.ring);
+    const uint32_t in_s = smem_u32(sm.ring);
+    float4 v[kItems];
+    float top[kItems], sum[kItems];
+#pragma unroll
+    for (uint32_t j = 0; j < kItems; ++j) { v[j] = make_float4(0.f, 0.f, 0.f, 0.f); top[j] = -INFINITY; sum[j] = 0.f; }
+    for (uint32_t k0 = 0; k0 < late.pieces; k0 += at_once) {
+        const uint32_t n = min(at_once, late.pieces - k0);
+        for (uint32_t k = warp; k < n; k += kWarps) {
+            const float *from = rec + (k0 + k ? 2 * (k0 + k) * kRecord : late.c0_first ? 0 : kRecord);
+            for (uint32_t i = lane * 4; i < len; i += 128)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(in_s + (k * len + i) * 4), "l"(from + i) : "memory");
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        bar_consumers();
+#pragma unroll
+        for (uint32_t j = 0; j < kItems; ++j) {
+            const uint32_t i = tid + j * kThr, x = i / kChunks;
+            if (x >= late.rows) break;
+            const float *row = in + x * (D + 4);
+            float t = top[j];
+            for (uint32_t k = 0; k < n; ++k) t = fmaxf(t, row[k * len + D]);
+            const float old = weight(top[j], t);
+            top[j] = t;
+            sum[j] *= old;
+            v[j].x *= old; v[j].y *= old; v[j].z *= old; v[j].w *= old;
+#pragma unroll 4
+            for (uint32_t k = 0; k < n; ++k) {
+                const float2 ml = *reinterpret_cast<const float2 *>(row + k * len + D);
+                const float4 u = *reinterpret_cast<const float4 *>(row + k * len + i % kChunks * 4);
+                const float w = weight(ml.x, t);
+                sum[j] = fmaf(ml.y, w, sum[j]);
+                v[j].x = fmaf(u.x, w, v[j].x); v[j].y = fmaf(u.y, w, v[j].y); v[j].z = fmaf(u.z, w, v[j].z); v[j].w = fmaf(u.w, w, v[j].w);
             }
-            sum = warp_sum(sum);
-            if (lane == 0) { sm.m[0][r0 + x] = top; sm.l[0][r0 + x] = sum; }
         }
         bar_consumers();
-#pragma unroll 1
-        for (uint32_t i = tid; i < nr * kChunks; i += kWarps * 32) {
-            const uint32_t x = i / kChunks, rw = r0 + x, d = i % kChunks * 4, tk = rw / a.group, hd = hkv * a.group + rw - tk * a.group;
-            const float *from = rec + rw * (D + 4) + d, *w = sm.o + x * pieces;
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-            for (uint32_t k = 0; k < pieces; k += kFlight) {
-                float4 u[kFlight];
+    }
 #pragma unroll
-                for (uint32_t j = 0; j < kFlight; ++j)
-                    u[j] = k + j < pieces ? __ldcg(reinterpret_cast<const float4 *>(from + (k + j ? 2 * (k + j) * kRecord : rec0))) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-                for (uint32_t j = 0; j < kFlight; ++j) {
-                    const float by = w[min(k + j, pieces - 1)];
-                    v.x = fmaf(u[j].x, by, v.x); v.y = fmaf(u[j].y, by, v.y); v.z = fmaf(u[j].z, by, v.z); v.w = fmaf(u[j].w, by, v.w);
-                }
-            }
-            const float inv = q.past + (int32_t)tk < 0 ? 0.f : 1.f / sm.l[0][rw];
-            put(a, (q.first + tk) * a.out_stride + (uint64_t)hd * D + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
-            if (a.lse && d == 0) put_lse(a, q.first + tk, hd, sm.m[0][rw], sm.l[0][rw]);
-        }
-        bar_consumers();
+    for (uint32_t j = 0; j < kItems; ++j) {
+        const uint32_t i = tid + j * kThr, rw = i / kChunks, d = i % kChunks * 4;
+        if (rw >= late.rows) break;
+        const uint32_t tk = rw / a.group, hd = late.hkv * a.group + rw - tk * a.group;
+        const float inv = late.q.past + (int32_t)tk < 0 ? 0.f : 1.f / sum[j];
+        put(a, (late.q.first + tk) * a.out_stride + (uint64_t)hd * D + d, make_float4(v[j].x * inv, v[j].y * inv, v[j].z * inv, v[j].w * inv));
+        if (a.lse && d == 0) put_lse(a, late.q.first + tk, hd, top[j], sum[j]);
     }
 }
 
@@ -332,6 +343,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
         prefetch_map(&a.vmap);
         for (uint32_t s = 0; s < kStages; ++s) { mbar_init(&sm.full[s], 1); mbar_init(&sm.empty[s], kWarps); }
         sm.abort_flag = 0;
+        sm.n_late = 0;
         sm.any_unfinite = 0;
         fence_barrier_init();
     }
@@ -549,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
             if (tid == 0) {   // (the ticket is the next launch's again whatever became of this one)
                 const bool last = atomicAdd(&a.tickets[c0], 1u) == pieces - 1;
                 if (last) a.tickets[c0] = 0;
-                sm.last = last && !sm.abort_flag;
+                if (last && !sm.abort_flag) sm.late[sm.n_late++] = Late{p.q, p.hkv, p.rows, c0, pieces, p.base <= share_lo(sh, c0)};
             }
         }
         bar_consumers();   // (also: everybody has read the unfinite values)
@@ -558,12 +570,13 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
             bar_consumers();
             if (tid == 0) sm.any_unfinite = 0;
         }
-        if (!whole && sm.last) {
-            fence_acq_rel_gpu();
-            combine<D>(a, sm, p.q, p.hkv, p.rows, c0, pieces, p.base <= share_lo(sh, c0));
-        }
         bar_consumers();   // the shared arrays are free for the next piece
     } while (next_piece(a, walk, p));
+    // (the last: every copy into the ring has been waited for, unless a wait ran out)
+    if (sm.n_late && !sm.abort_flag) {
+        fence_acq_rel_gpu();
+        for (uint32_t i = 0; i < sm.n_late; ++i) combine<D>(a, sm, sm.late[i]);
+    }
     griddep_launch_dependents();
 }
 
