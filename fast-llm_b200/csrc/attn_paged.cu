@@ -15,7 +15,8 @@
 // Keys as rows of A cost 16 instructions per 16 keys and 4 rows; the rows as A cost 64 for any number of them, and a tile then took 1.25 us
 // of mma.sync.
 // Measured (8 KV heads, groups of 4, head_dim 128): 4 x 65000 keys 149 us (6.4 TB/s; rows as A 187), 16 x 5500 to 8192 keys on pages of 16 rows
-// 78 us (5.9 TB/s), one sequence over 1024 keys 9.1 us, of which the host's call takes 8.3.
+// 78 us (5.9 TB/s), one sequence over 1024 keys 9.1 us, of which the host's call takes 8.3. Four tokens of 4 heads a sequence, 16 rows (bound by
+// mma.sync and the softmax): 4 x 65000 keys 164 us, 1 x 8000 30 us.
 // A masked value never meets the tensor core as it is, since 0 x NaN is NaN: rows behind the last key are cleared in shared
 // memory, and among the keys of the new tokens, which not all rows attend, values that are not finite are taken out there and
 // their effect added to the rows that do attend them (see unfinite_of).
@@ -169,19 +170,21 @@ __device__ __forceinline__ void copy_tiles(const PagedAttnArgs &a, FewSmem<D> &s
 
 // The records of a sequence over one KV head, added in order: of CTA c0 the piece at its end (or its first), of the others the one at
 // their start. This is the launch's tail: its time is round trips to L2, so that as many records as the ring holds, which is free by then, are
-// copied into it at once (16 rows, 37 records: two loads of a row in registers 42 us for the whole call). Run once, so out of line.
-template <int D>
+// copied into it at once; then their weights, 8 lanes a row, then the contexts. Run once, so out of line. (16 rows, 42 records: 11 us;
+// loads into registers, 8 at a time, 20.)
+template <int D, int B>
 __device__ __noinline__ void combine(const PagedAttnArgs &a, FewSmem<D> &sm, const Late late) {
-    constexpr uint32_t kRecord = kRowsB * (D + 4), kChunks = D / 4, kThr = kWarps * 32, kItems = kRowsB * kChunks / kThr;
-    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, len = late.rows * (D + 4);
+    constexpr uint32_t kRecord = kRowsB * (D + 4), kChunks = D / 4, kThr = kWarps * 32, kItems = 4 * B * kChunks <= kThr ? 1 : 4 * B * kChunks / kThr;
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, len = late.rows * (D + 4), wr = tid >> 3;
     const uint32_t at_once = (uint32_t)(sizeof(sm.ring) / sizeof(float)) / len;
     const float *rec = a.part + (uint64_t)late.c0 * 2 * kRecord;   // record i >= 1 at rec + 2 i kRecord
     const float *in = reinterpret_cast<const float *>(sm.ring);
     const uint32_t in_s = smem_u32(sm.ring);
+    static_assert(sizeof(sm.ring) / 4 / (D + 4) <= sizeof(sm.o) / 4 && kThr / 8 == kRowsB, "weights");
     float4 v[kItems];
-    float top[kItems], sum[kItems];
 #pragma unroll
-    for (uint32_t j = 0; j < kItems; ++j) { v[j] = make_float4(0.f, 0.f, 0.f, 0.f); top[j] = -INFINITY; sum[j] = 0.f; }
+    for (uint32_t j = 0; j < kItems; ++j) v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+    float top = -INFINITY, sum = 0.f;   // of row wr
     for (uint32_t k0 = 0; k0 < late.pieces; k0 += at_once) {
         const uint32_t n = min(at_once, late.pieces - k0);
         for (uint32_t k = warp; k < n; k += kWarps) {
@@ -191,26 +194,44 @@ __device__ __noinline__ void combine(const PagedAttnArgs &a, FewSmem<D> &sm, con
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         bar_consumers();
+        const float *ml = in + wr * (D + 4) + D;
+        float t = top, add = 0.f;
+        if (wr < late.rows)
+            for (uint32_t k = lane & 7u; k < n; k += 8) t = fmaxf(t, ml[k * len]);
+        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
+        const float old = weight(top, t);
+        top = t;
+        if (wr < late.rows)
+            for (uint32_t k = lane & 7u; k < n; k += 8) {
+                const float w = weight(ml[k * len], t);
+                sm.o[wr * n + k] = w;
+                add = fmaf(ml[k * len + 1], w, add);
+            }
+        add += __shfl_xor_sync(0xffffffffu, add, 1);
+        add += __shfl_xor_sync(0xffffffffu, add, 2);
+        add += __shfl_xor_sync(0xffffffffu, add, 4);
+        sum = fmaf(sum, old, add);
+        if (!(lane & 7u)) { sm.f[wr] = old; sm.m[0][wr] = t; sm.l[0][wr] = sum; }
+        bar_consumers();
+        const float *u[kItems], *w[kItems];
 #pragma unroll
         for (uint32_t j = 0; j < kItems; ++j) {
-            const uint32_t i = tid + j * kThr, x = i / kChunks;
-            if (x >= late.rows) break;
-            const float *row = in + x * (D + 4);
-            float t = top[j];
-            for (uint32_t k = 0; k < n; ++k) t = fmaxf(t, row[k * len + D]);
-            const float old = weight(top[j], t);
-            top[j] = t;
-            sum[j] *= old;
-            v[j].x *= old; v[j].y *= old; v[j].z *= old; v[j].w *= old;
-#pragma unroll 4
-            for (uint32_t k = 0; k < n; ++k) {
-                const float2 ml = *reinterpret_cast<const float2 *>(row + k * len + D);
-                const float4 u = *reinterpret_cast<const float4 *>(row + k * len + i % kChunks * 4);
-                const float w = weight(ml.x, t);
-                sum[j] = fmaf(ml.y, w, sum[j]);
-                v[j].x = fmaf(u.x, w, v[j].x); v[j].y = fmaf(u.y, w, v[j].y); v[j].z = fmaf(u.z, w, v[j].z); v[j].w = fmaf(u.w, w, v[j].w);
-            }
+            const uint32_t i = tid + j * kThr, x = min(i / kChunks, late.rows - 1);
+            const float by = sm.f[x];
+            v[j].x *= by; v[j].y *= by; v[j].z *= by; v[j].w *= by;
+            u[j] = in + x * (D + 4) + i % kChunks * 4;
+            w[j] = sm.o + x * n;
         }
+#pragma unroll 4
+        for (uint32_t k = 0; k < n; ++k)
+#pragma unroll
+            for (uint32_t j = 0; j < kItems; ++j) {
+                const float4 y = *reinterpret_cast<const float4 *>(u[j] + k * len);
+                const float by = w[j][k];
+                v[j].x = fmaf(y.x, by, v[j].x); v[j].y = fmaf(y.y, by, v[j].y); v[j].z = fmaf(y.z, by, v[j].z); v[j].w = fmaf(y.w, by, v[j].w);
+            }
         bar_consumers();
     }
 #pragma unroll
@@ -218,10 +239,15 @@ __device__ __noinline__ void combine(const PagedAttnArgs &a, FewSmem<D> &sm, con
         const uint32_t i = tid + j * kThr, rw = i / kChunks, d = i % kChunks * 4;
         if (rw >= late.rows) break;
         const uint32_t tk = rw / a.group, hd = late.hkv * a.group + rw - tk * a.group;
-        const float inv = late.q.past + (int32_t)tk < 0 ? 0.f : 1.f / sum[j];
+        const float inv = late.q.past + (int32_t)tk < 0 ? 0.f : 1.f / sm.l[0][rw];
         put(a, (late.q.first + tk) * a.out_stride + (uint64_t)hd * D + d, make_float4(v[j].x * inv, v[j].y * inv, v[j].z * inv, v[j].w * inv));
-        if (a.lse && d == 0) put_lse(a, late.q.first + tk, hd, top[j], sum[j]);
+        if (a.lse && d == 0) put_lse(a, late.q.first + tk, hd, sm.m[0][rw], sm.l[0][rw]);
     }
+    bar_consumers();   // (another one may follow)
+}
+// What values that are not finite add to four dimensions of a row
+template <int D> __device__ __noinline__ float4 add_unfinite(const uint32_t *u, uint32_t d, int32_t lim, const float4 v) {
+    return make_float4(v.x + unfinite_of(u, D, d, lim), v.y + unfinite_of(u, D, d + 1, lim), v.z + unfinite_of(u, D, d + 2, lim), v.w + unfinite_of(u, D, d + 3, lim));
 }
 
 // The rows of a piece as the threads hold them: blocks of 4 (at most B), lane (g, t) row t. q as operand: column g = row g / 2, part
@@ -505,30 +531,30 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
 #pragma unroll
             for (int dt = 0; dt < D / 16; ++dt) { w.o[n][dt][0] *= by; w.o[n][dt][1] *= by; }
         }
-        // parts of `wide` dimensions: few rows, wide parts (row_bits: 2, 3, 4 for 4, 8, 16 rows); the thread's row and 4 dimensions of a part
-        const uint32_t row_bits = p.rows <= 4 && D == 128 ? 2 : p.rows <= 8 ? 3 : 4, wide = 512u >> row_bits, pitch = wide + 4;
+        // parts of `wide` dimensions: few rows, wide parts; the thread's row and 4 dimensions of a part. (All parts in line: as a loop
+        // with the registers of a part found at run time 4.2 us for 16 rows, now 2.0.)
+        constexpr uint32_t row_bits = B == 4 ? 4 : B == 1 && D == 128 ? 2 : 3, wide = 512u >> row_bits, pitch = wide + 4;
         const uint32_t row = tid >> (7 - row_bits), c4 = (tid & ((wide >> 2) - 1u)) * 4;
         const uint32_t tok = row / a.group, head = p.hkv * a.group + row - tok * a.group;
         const int32_t row_lim = p.q.past + (int32_t)tok;
         const uint64_t dst = (p.q.first + tok) * a.out_stride + (uint64_t)head * D;
         float top = -INFINITY, sum = 0.f;
-        const bool writes = row < p.rows && !sm.abort_flag;
+        const bool writes = row < p.rows && !sm.abort_flag, unfinite = sm.any_unfinite != 0;
         if (row < p.rows) {
 #pragma unroll
             for (uint32_t x = 0; x < kWarps; ++x) top = fmaxf(top, sm.m[x][row]);
 #pragma unroll
             for (uint32_t x = 0; x < kWarps; ++x) sum = fmaf(sm.l[x][row], weight(sm.m[x][row], top), sum);
         }
-#pragma unroll 1
+        const float inv = row_lim < 0 ? 0.f : 1.f / sum;
+#pragma unroll
         for (uint32_t d0 = 0; d0 < D; d0 += wide) {
             if (d0) bar_consumers();
 #pragma unroll
             for (uint32_t n = 0; n < B; ++n) {
-                if (n * 4 >= p.rows) break;
                 float *at = sm.o + ((warp << row_bits) + n * 4 + t) * pitch + g;
 #pragma unroll
-                for (int dt = 0; dt < D / 16; ++dt)
-                    if (dt * 16u >= d0 && dt * 16u - d0 < wide) { at[dt * 16u - d0] = w.o[n][dt][0]; at[dt * 16u - d0 + 8] = w.o[n][dt][1]; }
+                for (uint32_t dt = 0; dt < wide / 16; ++dt) { at[dt * 16] = w.o[n][d0 / 16 + dt][0]; at[dt * 16 + 8] = w.o[n][d0 / 16 + dt][1]; }
             }
             bar_consumers();
             if (writes) {
@@ -539,16 +565,9 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
                     v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
                 }
                 const uint32_t d = d0 + c4;
-                if (sm.any_unfinite) {
-                    v.x += unfinite_of(&sm.unfinite[0][0], D, d, row_lim); v.y += unfinite_of(&sm.unfinite[0][0], D, d + 1, row_lim);
-                    v.z += unfinite_of(&sm.unfinite[0][0], D, d + 2, row_lim); v.w += unfinite_of(&sm.unfinite[0][0], D, d + 3, row_lim);
-                }
-                if (whole) {
-                    const float inv = row_lim < 0 ? 0.f : 1.f / sum;
-                    put(a, dst + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
-                } else {
-                    __stcg(reinterpret_cast<float4 *>(rec + row * (D + 4) + d), v);
-                }
+                if (unfinite) v = add_unfinite<D>(&sm.unfinite[0][0], d, row_lim, v);
+                if (whole) put(a, dst + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+                else __stcg(reinterpret_cast<float4 *>(rec + row * (D + 4) + d), v);
             }
         }
         if (writes && c4 == 0) {
@@ -575,7 +594,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
     // (the last: every copy into the ring has been waited for, unless a wait ran out)
     if (sm.n_late && !sm.abort_flag) {
         fence_acq_rel_gpu();
-        for (uint32_t i = 0; i < sm.n_late; ++i) combine<D>(a, sm, sm.late[i]);
+        for (uint32_t i = 0; i < sm.n_late; ++i) combine<D, B>(a, sm, sm.late[i]);
     }
     griddep_launch_dependents();
 }
@@ -604,6 +623,8 @@ cudaError_t launch_paged_few(PagedAttnArgs a, const void *k, const void *v, uint
     if (const cudaError_t e = tensor_map_groups_swz(&a.kmap, k, rows, head_dim, box)) return e;
     if (const cudaError_t e = tensor_map_groups_swz(&a.vmap, v, rows, head_dim, box)) return e;
     const uint64_t most = std::min<uint64_t>((uint64_t)a.max_new * a.group, kRowsB);
+    // Fewer blocks of rows at most, fewer registers and instructions. us at 4 x 65000, 32 x 4000 and 1 x 8000 keys: 4 rows 150, 75, 17.4 (as part of
+    // 16: 154, 76, 18.4), 8 rows 158, 80, 24.6 (163, 83, 26.2).
     const auto &k_ = kFewKernels[head_dim == 128][most <= 4 ? 0 : most <= 8 ? 1 : 2];
     return launch_kernel(k_.k, dim3(grid), dim3(kThreads), k_.smem, stream, true, a);
 }
