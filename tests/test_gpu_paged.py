@@ -646,6 +646,19 @@ def test_a_prompt_of_131072_tokens(ctx):
         assert ((out[tok].double().view(n_q, dim) - want).abs() <= tol).all(), tok
 
 
+@pytest.mark.parametrize("n_q,n_kv,dim", [(4, 1, 128), (4, 1, 64), (10, 5, 128), (32, 8, 64)])
+@pytest.mark.parametrize("new", [1, 2, 3, 4])
+def test_few_rows_over_long_caches(ctx, n_q, n_kv, dim, new):
+    """Up to 296 records of up to 16 rows: more than are added at once; a CTA may be the last of two blocks."""
+    seqs = [(40001, new), (33, 1), (5000, new)]
+    c = make(dim + new, seqs, n_q, n_kv, dim, 64, "f32")
+    attn(ctx, c, n_q, n_kv, dim, 64, 1.0 / math.sqrt(dim))
+    check(ctx, c, seqs, n_q, n_kv, dim, 1.0 / math.sqrt(dim), "f32")
+    first = c["out"].clone()
+    attn(ctx, c, n_q, n_kv, dim, 64, 1.0 / math.sqrt(dim))
+    assert torch.equal(first, c["out"])
+
+
 def test_long_chunk_over_many_tiles(ctx):
     """Many tiles per piece: contexts go out and come back a quarter at a time; one key outweighs all others late in the walk, so
     that every sum changes its reference."""
