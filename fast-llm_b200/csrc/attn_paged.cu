@@ -16,7 +16,7 @@
 // of mma.sync.
 // Measured (8 KV heads, groups of 4, head_dim 128): 4 x 65000 keys 149 us (6.4 TB/s; rows as A 187), 16 x 5500 to 8192 keys on pages of 16 rows
 // 78 us (5.9 TB/s), one sequence over 1024 keys 9.1 us, of which the host's call takes 8.3. Four tokens of 4 heads a sequence, 16 rows (bound by
-// mma.sync and the softmax): 4 x 65000 keys 164 us, 1 x 8000 30 us.
+// mma.sync and the softmax): 4 x 65000 keys 164 us, 1 x 8000 27 us.
 // A masked value never meets the tensor core as it is, since 0 x NaN is NaN: rows behind the last key are cleared in shared
 // memory, and among the keys of the new tokens, which not all rows attend, values that are not finite are taken out there and
 // their effect added to the rows that do attend them (see unfinite_of).
@@ -36,6 +36,31 @@ constexpr float kShift = 12.f;   // probabilities are 2^(x - m + 12): their lo p
 __device__ __forceinline__ uint32_t rows_of(const PagedAttnArgs &a, const PagedSeq &q) { return q.n * a.group > a.few_rows ? 0u : q.n * a.group; }
 __device__ __forceinline__ uint32_t tiles_of(const PagedSeq &q) { return max(1u, ((uint32_t)max(0, q.past + (int32_t)q.n) + kTile - 1) / kTile); }
 __device__ __forceinline__ uint64_t units_of(const PagedAttnArgs &a, const PagedSeq &q) { return rows_of(a, q) ? (uint64_t)tiles_of(q) * a.n_kv : 0u; }
+
+// An end of a share that lies in a sequence's tiles b .. e over one KV head, within kSnap tiles of b or e, moves there: a CTA with a few
+// tiles of another head builds rows of q, leaves a record, is the last to arrive at both and adds the records of both (one sequence over 8000
+// keys 17.0 us, moved 15.1; 8 over 2000 17.6, 15.4; 16 over 5500 to 8192, where shares are long, 78.1, 78.6). Up by less than half a share, down by half of one at most, so that none gets empty.
+constexpr uint32_t kSnap = 4;
+// The line over at most `ctas` CTAs: where shares are that small no more of them than keep the largest one, which leaves fewer records. (Longer
+// shares: all of them, for the HBM's sake; 16 x 5500 to 8192 keys 78.5 us, 79.9 with 292 CTAs of 296.)
+__device__ __forceinline__ Shares few_shares(uint32_t units, uint32_t ctas) {
+    const uint32_t most = units / ctas + (units % ctas ? 1u : 0u);
+    return shares_of(units, most == 0 || most > 2 * kSnap ? ctas : units / most + (units % most ? 1u : 0u));
+}
+__device__ __forceinline__ uint32_t snapped(const Shares &sh, uint32_t snap, uint32_t at, uint32_t b, uint32_t e) {
+    const uint32_t down = at - b, up = e - at;
+    const bool may_down = down <= snap && 2 * down <= sh.each, may_up = up <= snap && 2 * up < sh.each;
+    return may_down && (!may_up || down <= up) ? b : may_up ? e : at;
+}
+// The first and the last CTA of tiles b .. e - 1
+__device__ __forceinline__ uint32_t first_of(const Shares &sh, uint32_t snap, uint32_t b, uint32_t e) {
+    const uint32_t c = owner_of(sh, b), hi = share_lo(sh, c + 1);
+    return hi < e && snapped(sh, snap, hi, b, e) == b ? c + 1 : c;
+}
+__device__ __forceinline__ uint32_t last_of(const Shares &sh, uint32_t snap, uint32_t b, uint32_t e) {
+    const uint32_t c = owner_of(sh, e - 1), lo = share_lo(sh, c);
+    return lo > b && snapped(sh, snap, lo, b, e) == e ? c - 1 : c;
+}
 
 // The pieces of a CTA's share: consecutive tiles of one sequence over one KV head.
 struct Piece {
@@ -70,7 +95,6 @@ __device__ __forceinline__ bool next_piece(const PagedAttnArgs &a, Walk &w, Piec
 struct Late {
     PagedSeq q;
     uint32_t hkv, rows, c0, pieces;
-    bool c0_first;      // of CTA c0 the first record is meant
 };
 
 template <int D> struct FewSmem {
@@ -82,7 +106,7 @@ template <int D> struct FewSmem {
     uint32_t unfinite[3][D];                                              // see unfinite_of
     uint64_t full[kStages], empty[kStages];
     uint64_t sum[kThreads / 32];
-    uint32_t start_seq, start_off, any_unfinite, abort_flag, n_late;
+    uint32_t start_seq, start_off, any_unfinite, abort_flag, n_late, c0, pieces;                // c0, pieces: the CTAs of the piece's tiles
     Late late[2];                                                         // (a CTA shares two at most: its first and its last)
 };
 
@@ -168,8 +192,8 @@ __device__ __forceinline__ void copy_tiles(const PagedAttnArgs &a, FewSmem<D> &s
         for (uint32_t i = issued - min(issued, kStages); i < issued; ++i) mbar_wait_bounded(&sm.full[i % kStages], i / kStages & 1u, a.status);
 }
 
-// The records of a sequence over one KV head, added in order: of CTA c0 the piece at its end (or its first), of the others the one at
-// their start. This is the launch's tail: its time is round trips to L2, so that as many records as the ring holds, which is free by then, are
+// The records of a sequence over one KV head, added in order: of CTA c0 the one of the tiles that begin in its share, of the others the one of
+// tiles that began before. This is the launch's tail: its time is round trips to L2, so that as many records as the ring holds, which is free by then, are
 // copied into it at once; then their weights, 8 lanes a row, then the contexts. Run once, so out of line. (16 rows, 42 records: 11 us;
 // loads into registers, 8 at a time, 20.)
 template <int D, int B>
@@ -188,7 +212,7 @@ __device__ __noinline__ void combine(const PagedAttnArgs &a, FewSmem<D> &sm, con
     for (uint32_t k0 = 0; k0 < late.pieces; k0 += at_once) {
         const uint32_t n = min(at_once, late.pieces - k0);
         for (uint32_t k = warp; k < n; k += kWarps) {
-            const float *from = rec + (k0 + k ? 2 * (k0 + k) * kRecord : late.c0_first ? 0 : kRecord);
+            const float *from = rec + (k0 + k ? 2 * (k0 + k) * kRecord : kRecord);
             for (uint32_t i = lane * 4; i < len; i += 128)
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(in_s + (k * len + i) * 4), "l"(from + i) : "memory");
         }
@@ -358,6 +382,12 @@ __device__ __forceinline__ void begin_rows(const PagedAttnArgs &a, const FewSmem
     }
 }
 
+// (out of line, and by way of memory: in line 4 x 65000 keys with 16 rows went from 164 to 191 us)
+template <int D> __device__ __noinline__ void note_ctas(const PagedAttnArgs &a, FewSmem<D> &sm, const Shares sh, uint32_t b, uint32_t e) {
+    const uint32_t snap = a.n_seq <= 32 ? kSnap : 0;
+    sm.c0 = first_of(sh, snap, b, e);
+    sm.pieces = last_of(sh, snap, b, e) - sm.c0 + 1;
+}
 template <int D, int B>   // at most 4 B rows
 __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_constant__ PagedAttnArgs a) {
     extern __shared__ uint8_t smem_dyn[];
@@ -394,9 +424,18 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
             if (lane >= (uint32_t)o) x += y;
         }
         if (bad && blockIdx.x == 0) atomicCAS(a.status, ST_OK, ST_PAGED_ARGS);
-        sh = shares_of(__shfl_sync(0xffffffffu, x, 31), gridDim.x);
+        sh = few_shares(__shfl_sync(0xffffffffu, x, 31), gridDim.x);
         if (blockIdx.x >= sh.n) return;
-        walk = Walk{share_lo(sh, blockIdx.x), share_lo(sh, blockIdx.x + 1)};
+        const uint32_t tiles = max(1u, u / a.n_kv);   // (of the lane's sequence over a KV head)
+        auto edge = [&](uint32_t c) {
+            const uint32_t at = share_lo(sh, c);
+            if (c == 0 || c == sh.n) return at;
+            const int src = __ffs(__ballot_sync(0xffffffffu, at < x)) - 1;
+            const uint32_t n = __shfl_sync(0xffffffffu, tiles, src), b = at - (at - __shfl_sync(0xffffffffu, x - u, src)) % n;
+            return snapped(sh, kSnap, at, b, b + n);
+        };
+        walk.pos = edge(blockIdx.x);
+        walk.hi = edge(blockIdx.x + 1);
         const int src = __ffs(__ballot_sync(0xffffffffu, walk.pos < x)) - 1;   // the first sequence that ends behind the share's begin
         p.seq = src;
         p.q.first = __shfl_sync(0xffffffffu, q.first, src);
@@ -425,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
         }
         if ((any_bad || total >> 32) && blockIdx.x == 0) atomicCAS(a.status, ST_OK, ST_PAGED_ARGS);
         x -= mine;
-        sh = shares_of(total >> 32 ? 0u : (uint32_t)total, gridDim.x);
+        sh = few_shares(total >> 32 ? 0u : (uint32_t)total, gridDim.x);
         if (blockIdx.x >= sh.n) return;
         walk = Walk{share_lo(sh, blockIdx.x), share_lo(sh, blockIdx.x + 1)};
         if (walk.pos >= x && walk.pos < x + mine) {
@@ -455,9 +494,10 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
     }
 
     uint32_t stage = 0, parity = 0;   // of the ring
-    bool first = true, landed = true;   // (landed: no wait of this warp has run out)
+    bool landed = true;   // no wait of this warp has run out
     do {
         for (uint32_t n = warp; n * 4 < p.rows; n += kWarps) build_q<D>(a, sm, p, n);
+        if (tid == 0) note_ctas<D>(a, sm, sh, p.base, p.base + p.tiles);
         bar_consumers();
         Rows<D, B> w;
         begin_rows<D, B>(a, sm, p, w);
@@ -508,10 +548,9 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
         if (!landed) sm.abort_flag = 1u;   // (everybody goes on to the barriers, nobody writes)
 
         // ---- the warps' sums, a part of the dimensions at a time ----
-        const uint32_t c0 = owner_of(sh, p.base), pieces = owner_of(sh, p.base + p.tiles - 1) - c0 + 1;
+        const uint32_t c0 = sm.c0, pieces = sm.pieces;
         const bool whole = pieces == 1;
-        float *rec = a.part + (uint64_t)(blockIdx.x * 2 + (first ? 0 : 1)) * kRowsB * (D + 4);
-        first = false;
+        float *rec = a.part + (uint64_t)(blockIdx.x * 2 + (p.t0 == 0 ? 1 : 0)) * kRowsB * (D + 4);   // tiles that begin here, or before
 #pragma unroll
         for (uint32_t n = 0; n < B; ++n) {
             if (n * 4 >= p.rows) break;
@@ -580,7 +619,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
             if (tid == 0) {   // (the ticket is the next launch's again whatever became of this one)
                 const bool last = atomicAdd(&a.tickets[c0], 1u) == pieces - 1;
                 if (last) a.tickets[c0] = 0;
-                if (last && !sm.abort_flag) sm.late[sm.n_late++] = Late{p.q, p.hkv, p.rows, c0, pieces, p.base <= share_lo(sh, c0)};
+                if (last && !sm.abort_flag) sm.late[sm.n_late++] = Late{p.q, p.hkv, p.rows, c0, pieces};
             }
         }
         bar_consumers();   // (also: everybody has read the unfinite values)

@@ -39,7 +39,7 @@ struct PagedAttnArgs {
 };
 
 // Sequences of few rows over a KV head (mma.sync: attn_paged.cu) and of many (tcgen05: attn_paged_tm.cu). kmap and vmap are filled in there. us of
-// both at 4 x 65000, 32 x 4000 and 1 x 8000 keys, 8 KV heads: 4 rows 150, 75, 17 and 212, 136, 34 (f16: 158, 92, 29); 16 rows 164, 91, 30 and
+// both at 4 x 65000, 32 x 4000 and 1 x 8000 keys, 8 KV heads: 4 rows 150, 76, 15 and 212, 136, 34 (f16: 158, 92, 29); 16 rows 165, 92, 27 and
 // 215, 137, 34 (f16: 158, 92, 29).
 constexpr uint32_t kFewRows = 16;
 cudaError_t paged_few_init(void);
