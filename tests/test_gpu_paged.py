@@ -659,6 +659,21 @@ def test_few_rows_over_long_caches(ctx, n_q, n_kv, dim, new):
     assert torch.equal(first, c["out"])
 
 
+@pytest.mark.parametrize("seed", range(16))
+def test_ragged_batches_of_few_rows(ctx, seed):
+    """Lengths, heads and counts at random: ends of shares fall anywhere among the sequences' tiles."""
+    rng = np.random.default_rng(seed)
+    n_kv = int(rng.choice([1, 2, 5, 8]))
+    group = int(rng.choice([1, 2, 4]))
+    most = 16 // group if seed % 2 else 1
+    longest = int(rng.choice([70, 700, 7000]))
+    seqs = [(int(L), int(min(m, L))) for L, m in zip(rng.integers(0, longest, 1 + 2 * seed), rng.integers(0, most + 1, 1 + 2 * seed))] + [(longest, 1)]
+    dim, act = (64, "f16") if seed % 3 == 0 else (128, "f32")
+    c = make(100 + seed, seqs, n_kv * group, n_kv, dim, 16, act)
+    attn(ctx, c, n_kv * group, n_kv, dim, 16, 0.1)
+    check(ctx, c, seqs, n_kv * group, n_kv, dim, 0.1, act)
+
+
 def test_long_chunk_over_many_tiles(ctx):
     """Many tiles per piece: contexts go out and come back a quarter at a time; one key outweighs all others late in the walk, so
     that every sum changes its reference."""
