@@ -39,7 +39,7 @@ __device__ __forceinline__ uint64_t units_of(const PagedAttnArgs &a, const Paged
 
 // An end of a share that lies in a sequence's tiles b .. e over one KV head, within kSnap tiles of b or e, moves there: a CTA with a few
 // tiles of another head builds rows of q, leaves a record, is the last to arrive at both and adds the records of both (one sequence over 8000
-// keys 17.0 us, moved 15.1; 8 over 2000 17.6, 15.4; 16 over 5500 to 8192, where shares are long, 78.1, 78.6). Up by less than half a share, down by half of one at most, so that none gets empty.
+// keys 17.0 us, moved 15.1; 4 over 1023 13.0, 10.2; 8 over 2000 17.6, 15.4; 16 over 5500 to 8192, where shares are long, 78.1, 78.6). Up by less than half a share, down by half of one at most, so that none gets empty.
 constexpr uint32_t kSnap = 4;
 // The line over at most `ctas` CTAs: where shares are that small no more of them than keep the largest one, which leaves fewer records. (Longer
 // shares: all of them, for the HBM's sake; 16 x 5500 to 8192 keys 78.5 us, 79.9 with 292 CTAs of 296.)
@@ -385,6 +385,11 @@ __device__ __forceinline__ void begin_rows(const PagedAttnArgs &a, const FewSmem
 // (out of line, and by way of memory: in line 4 x 65000 keys with 16 rows went from 164 to 191 us)
 template <int D> __device__ __noinline__ void note_ctas(const PagedAttnArgs &a, FewSmem<D> &sm, const Shares sh, uint32_t b, uint32_t e) {
     const uint32_t snap = a.n_seq <= 32 ? kSnap : 0;
+    if (sh.each < 2) {
+        sm.c0 = owner_of(sh, b);
+        sm.pieces = owner_of(sh, e - 1) - sm.c0 + 1;
+        return;
+    }
     sm.c0 = first_of(sh, snap, b, e);
     sm.pieces = last_of(sh, snap, b, e) - sm.c0 + 1;
 }
@@ -429,7 +434,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
         const uint32_t tiles = max(1u, u / a.n_kv);   // (of the lane's sequence over a KV head)
         auto edge = [&](uint32_t c) {
             const uint32_t at = share_lo(sh, c);
-            if (c == 0 || c == sh.n) return at;
+            if (c == 0 || c == sh.n || sh.each < 2) return at;   // (shares of a tile cannot move: the smallest calls, 9.8 -> 9.4 us)
             const int src = __ffs(__ballot_sync(0xffffffffu, at < x)) - 1;
             const uint32_t n = __shfl_sync(0xffffffffu, tiles, src), b = at - (at - __shfl_sync(0xffffffffu, x - u, src)) % n;
             return snapped(sh, kSnap, at, b, b + n);
