@@ -39,7 +39,8 @@ __device__ __forceinline__ uint64_t units_of(const PagedAttnArgs &a, const Paged
 
 // An end of a share that lies in a sequence's tiles b .. e over one KV head, within kSnap tiles of b or e, moves there: a CTA with a few
 // tiles of another head builds rows of q, leaves a record, is the last to arrive at both and adds the records of both (one sequence over 8000
-// keys 17.0 us, moved 15.1; 4 over 1023 13.0, 10.2; 8 over 2000 17.6, 15.4; 16 over 5500 to 8192, where shares are long, 78.1, 78.6). Up by less than half a share, down by half of one at most, so that none gets empty.
+// keys 17.0 us, moved 15.1; 4 over 1023 13.0, 10.2; 8 over 2000 17.6, 15.4; 16 over 5500 to 8192, where shares are long, 78.1, 78.6). Up by
+// less than half a share, down by half of one at most, so that none gets empty.
 constexpr uint32_t kSnap = 4;
 // The line over at most `ctas` CTAs: where shares are that small no more of them than keep the largest one, which leaves fewer records. (Longer
 // shares: all of them, for the HBM's sake; 16 x 5500 to 8192 keys 78.5 us, 79.9 with 292 CTAs of 296.)
