@@ -20,9 +20,10 @@
 // Tiles of all blocks lie on one line (sequence, KV head, block, tile) and every CTA takes an equal piece of it; the records of a block that
 // several CTAs share are added by a launch of its own behind.
 //
-// The tensor cores truncate their running sum, 3.1e-8 of it per instruction (see kLoss); with f32 activations a part of 32 columns of O is therefore
-// brought out at every tile, in turn, added in f32 to a buffer of the CTA's own that stays in L2, and starts from zero: no sum in
-// tensor memory is longer than four tiles (64 instructions), a piece's first one eight.
+// The tensor cores truncate their running sum, 3.1e-8 of it per instruction in the mean; with f32 activations half of O's columns are therefore
+// brought out at every tile, in turn, added in f32 to a buffer of the CTA's own that stays in L2, and start from zero: no sum in
+// tensor memory is longer than three tiles (48 instructions). (us with a quarter at every tile, sums of up to eight: 4 x 8 tokens over 4096
+// keys 32.7, now 35.2; 4096 tokens 310, 320; 1000 over 20000 keys 554, 603.)
 #include "common.cuh"
 #include "paged.h"
 
@@ -36,10 +37,6 @@ constexpr uint32_t kRowsL = 128, kTile = 128;
 constexpr uint32_t kCopyWarp = 8, kTensorWarp = 9, kValueWarp = 10, kThreads = 11 * 32;
 constexpr float kShift = 6.f;   // probabilities are 2^(x - ref), ref = maximum - 6 when it is set and kept while they stay below 2^14
 constexpr uint32_t kOCol = 256, kTmemCols = 512;
-// What a tensor instruction cuts off its 24-bit running sum, on average and relative to it: half a unit in the last place, 2^-25 times the mean of 1 / mantissa.
-// A sum of n equal steps ends n / 2 times that too small in the mean, which is given back where f32 results allow to see it (results against 64
-// bits, 4 x 8 tokens over 4096 keys: 1.4e-6 off without, of which 1.2e-6 were one common factor).
-constexpr float kLoss = 3.1e-8f;
 
 template <int D, int Parts> struct Tm {
     static constexpr uint32_t kPart = kRowsL * D * 2;               // one part of a lane's q; a K or V tile
@@ -276,7 +273,7 @@ __device__ __noinline__ float load_q(const PagedAttnArgs &a, uint8_t *dst, uint6
             for (int o = 4; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
             const int e = min(100, max(-100, 138 - (int)(__float_as_uint(top) >> 23)));
             const float up = __uint_as_float((uint32_t)(e + 127) << 23);
-            const float mine = fmaxf(a.scale * (float)(1.44269504088896341 * (1.0 + (Parts == 2 ? D / 32 * (double)kLoss : 0.0))) * __uint_as_float((uint32_t)(127 - e) << 23), 1e-37f);
+            const float mine = fmaxf(a.scale * 1.44269504088896341f * __uint_as_float((uint32_t)(127 - e) << 23), 1e-37f);
             const float got = __shfl_sync(0xffffffffu, mine, (lane >> 2 & 3u) * 8);
             if ((lane & 3u) + 4 * (lane >> 4) == i0 + i) f = got;
             {
@@ -455,10 +452,6 @@ __device__ __noinline__ void prefetch_q(const PagedAttnArgs &a, const Piece p) {
     }
 }
 struct Sums { float ref, sum, highest, acc_ref; uint32_t out_of; };   // of a row
-// The factor of contexts that were summed over that many tiles (8 instructions per tile and part).
-__device__ __forceinline__ float given_back(uint32_t tiles) { return fmaf(8.f * kLoss, (float)tiles, 1.f); }
-// The tiles of a lane that columns 32 c .. were summed over since they last went out (see the loop over the tiles), of `steps`.
-__device__ __forceinline__ uint32_t tiles_since(uint32_t steps, uint32_t c, bool went) { return went ? steps - ((steps - 1 - c) / 4 * 4 + c) : steps; }
 // The results of a lane's piece: the rows themselves, or a record. done: the lane has any, and they are in tensor memory.
 template <int D, int Parts>
 __device__ __noinline__ void finish(const PagedAttnArgs &a, Head &hd, uint8_t *q_s, const Sums s, bool done, uint32_t tmem) {
@@ -501,9 +494,9 @@ __device__ __noinline__ void finish(const PagedAttnArgs &a, Head &hd, uint8_t *q
         uint8_t *stage = q_s + (sm ? 1 : l) * Parts * T::kPart;
         const bool any_unfinite = hd.any_unfinite != 0;
         // 16 columns at a time (32 spill, and local memory is L2 here)
-        struct Part { uint32_t at; const float4 *mem; uint32_t out; float keep; uint32_t steps; };
-        const Part part1{to, acc_mem, s.out_of, s.acc_ref == ref ? 1.f : exp2_fast(s.acc_ref - ref), sm ? (job.n + 1) / 2 : job.n};
-        const Part part2{to + 128, acc_mem + T::kRecord / 4, out2, acc2_ref == ref2 ? 1.f : exp2_fast(acc2_ref - ref2), job.n / 2};
+        struct Part { uint32_t at; const float4 *mem; uint32_t out; float keep; };
+        const Part part1{to, acc_mem, s.out_of, s.acc_ref == ref ? 1.f : exp2_fast(s.acc_ref - ref)};
+        const Part part2{to + 128, acc_mem + T::kRecord / 4, out2, acc2_ref == ref2 ? 1.f : exp2_fast(acc2_ref - ref2)};
         auto add_part = [&](const Part &p, int c, float w, float (&v)[16]) {   // v += w times the contexts of columns 16 c ..
             float o[16];
             load16(p.at + 16 * c, o);
@@ -511,10 +504,10 @@ __device__ __noinline__ void finish(const PagedAttnArgs &a, Head &hd, uint8_t *q
             float4 old[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) old[j] = acc ? __ldcg(p.mem + (4 * c + j) * kRowsL) : make_float4(0.f, 0.f, 0.f, 0.f);
-            const float back = Parts == 2 ? w * given_back(tiles_since(p.steps, c / 2, acc)) : w, keep = w * p.keep;
+            const float keep = w * p.keep;
             wait_ld(o);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = fmaf(o[j], back, v[j]);
+            for (int j = 0; j < 16; ++j) v[j] = fmaf(o[j], w, v[j]);
             if (acc)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -945,29 +938,31 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
             uint32_t out_of = 0;                                               // bit c: columns 32 c .. have a sum in memory
             for (uint32_t step = 0; step < steps; ++step) {
                 const int32_t k0 = (int32_t)((t0 + (sm ? 2 * step + l : step)) * kTile);
-                const uint32_t c4 = step & 3u;   // the columns of O that go out at this step
-                if (Parts == 2 && active && step >= 4 && c4 < D / 32) {
-                    // a part of O to its sum in memory, while the tensor cores form the scores
+                if (Parts == 2 && active && step >= 2 && (step + 1 < steps || step == 3)) {   // (three tiles of a half at the end: they stay)
+                    // half of O to its sum in memory, while the tensor cores form the scores
                     if (!wait(&hd.o_done[l], (s_seen - 1) & 1u)) break;
                     fence_after();
-                    float o[32];
-                    load32(to + 32 * c4, o);
-                    wait_ld(o);
-                    const uint32_t zero[16] = {};
-                    store16(to + 32 * c4, zero);
-                    store16(to + 32 * c4 + 16, zero);
                     if (out_of == 0) acc_ref = ref;
                     if (ref - acc_ref > 40.f) acc_ref = move_sums(acc_mem, out_of, acc_ref, ref);   // (far below what f32 holds: |O| < 2^47)
-                    const float by = (ref == acc_ref ? 1.f : exp2_fast(ref - acc_ref)) * given_back(out_of >> c4 & 1u ? 4u : step);
-                    float4 *at = acc_mem + 8 * c4 * kRowsL;
-                    const bool adds = out_of >> c4 & 1u;
+                    const float by = ref == acc_ref ? 1.f : exp2_fast(ref - acc_ref);
+#pragma unroll 1
+                    for (uint32_t c4 = (step & 1u) * (D / 64); c4 < ((step & 1u) + 1) * (D / 64); ++c4) {   // 32 columns
+                        float o[32];
+                        load32(to + 32 * c4, o);
+                        wait_ld(o);
+                        const uint32_t zero[16] = {};
+                        store16(to + 32 * c4, zero);
+                        store16(to + 32 * c4 + 16, zero);
+                        float4 *at = acc_mem + 8 * c4 * kRowsL;
+                        const bool adds = out_of >> c4 & 1u;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float4 v = make_float4(o[4 * j] * by, o[4 * j + 1] * by, o[4 * j + 2] * by, o[4 * j + 3] * by);
-                        if (adds) add4(at + j * kRowsL, v);
-                        else __stcg(at + j * kRowsL, v);
+                        for (int j = 0; j < 8; ++j) {
+                            const float4 v = make_float4(o[4 * j] * by, o[4 * j + 1] * by, o[4 * j + 2] * by, o[4 * j + 3] * by);
+                            if (adds) add4(at + j * kRowsL, v);
+                            else __stcg(at + j * kRowsL, v);
+                        }
+                        out_of |= 1u << c4;
                     }
-                    out_of |= 1u << c4;
                 }
                 if (!wait(&hd.s_full[l], s_seen & 1u)) break;
                 ++s_seen;

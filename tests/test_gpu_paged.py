@@ -688,3 +688,25 @@ def test_long_chunk_over_many_tiles(ctx):
             c["ks"][0][0, j] = big
         attn(ctx, c, n_q, n_kv, dim, page, 0.088)
         check(ctx, c, seqs, n_q, n_kv, dim, 0.088, act)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("key", [0, 130])
+def test_a_row_of_one_key_keeps_its_value(ctx, dim, key):
+    """Prompts whose rows attend one key alone, or one that outweighs the others by 2^-100 over up to eight tiles: the result is that key's
+    value. Off by: the probability's two parts 2^-21 (cut after 10 bits, then half a step of 2^-11), the two products' sum cut to 24 bits 2^-23, the row's
+    sum, its inverse, the products with the inverse and with the change of reference 2^-24 each: below 2^-20."""
+    n_q, n_kv, page = 32, 8, 64
+    seqs = [(1000, 1000), (900, 900), (700, 700), (1000, 1000)]   # about 450 blocks of rows: most are one CTA's
+    c = make(dim + key, seqs, n_q, n_kv, dim, page, "f32", kv_scale=0.1)
+    c["q"].abs_().add_(1.0)
+    for s in range(len(seqs)):
+        c["k"][int(c["table"][s, key // page]), :, key % page] = 4.0
+    attn(ctx, c, n_q, n_kv, dim, page, 0.6)    # 0.6 sum q k: above 150 for the key, below 25 for the others
+    assert ctx.status() == 0
+    for s, (L, m) in enumerate(seqs):
+        want = c["vs"][s][:, key].double().repeat_interleave(n_q // n_kv, 0)
+        got = c["out"].double().view(-1, n_q, dim)[c["start"][s] + key:c["start"][s] + m]
+        assert ((got - want).abs() <= 2.0 ** -20 * want.abs()).all(), ((got - want).abs() / want.abs()).max().item()
+        first = c["vs"][s][:, 0].double().repeat_interleave(n_q // n_kv, 0)
+        assert ((c["out"].double().view(-1, n_q, dim)[c["start"][s]] - first).abs() <= 2.0 ** -20 * first.abs()).all()
