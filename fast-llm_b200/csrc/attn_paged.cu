@@ -30,7 +30,7 @@ namespace flb {
 namespace {
 
 constexpr uint32_t kRowsB = kFewRows, kTile = 64, kStages = 3, kWarps = 4, kThreads = (kWarps + 1) * 32;
-constexpr float kShift = 12.f;   // probabilities are 2^(x - m + 12): their lo parts stay normal f16 numbers down to 2^-14 of the largest
+constexpr float kShift = 12.f;   // probabilities are 2^(x - m + 12): their lo parts stay normal f16 numbers down to 2^-14 of the largest, below it are held to 2^-37 of that
 
 // Rows of a sequence over one KV head, 0 where it is the other kernel's; its tiles: at least one, so that somebody writes its rows.
 __device__ __forceinline__ uint32_t rows_of(const PagedAttnArgs &a, const PagedSeq &q) { return q.n * a.group > a.few_rows ? 0u : q.n * a.group; }

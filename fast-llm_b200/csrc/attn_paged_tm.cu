@@ -2,7 +2,7 @@
 // query head of the group) against tiles of 128 keys on tcgen05, scores and contexts in tensor memory.
 //
 // The mathematics are attn_paged.cu's: an online softmax in f32. f32 activations: q and the probabilities are two f16 parts each, so
-// that a pair of row and key costs 8 D tensor flops instead of 4 D, and nothing else is rounded below 32 bits. f16
+// that a pair of row and key costs 8 D tensor flops instead of 4 D, and nothing else is rounded below 32 bits (small probabilities: see kShift). f16
 // activations (Parts = 1): q as it is, the probabilities as one f16 (half a step of 2^-11, as the result).
 //
 // Bound by the chain scores - softmax - context of each lane. A tile of 128 keys and 256 rows, head_dim 128: 4300 cycles for f16 activations, 7000
@@ -35,7 +35,9 @@ namespace {
 
 constexpr uint32_t kRowsL = 128, kTile = 128;
 constexpr uint32_t kCopyWarp = 8, kTensorWarp = 9, kValueWarp = 10, kThreads = 11 * 32;
-constexpr float kShift = 6.f;   // probabilities are 2^(x - ref), ref = maximum - 6 when it is set and kept while they stay below 2^14
+// Probabilities are 2^(x - ref), ref = maximum - 12 when it is set and kept while they stay below 2^15, which f16 holds. f16 has steps of 2^-24 at
+// its lower end: a probability below 2^-14 of the row's largest is held to 2^-36 of that (half a step for each part), one below 2^-37 is lost.
+constexpr float kShift = 12.f, kLag = 3.f;
 constexpr uint32_t kOCol = 256, kTmemCols = 512;
 
 template <int D, int Parts> struct Tm {
@@ -208,7 +210,7 @@ __device__ __noinline__ void scale_o(uint32_t at, uint32_t columns, float by) {
 }
 // 32 scores to probabilities, in place in tensor memory (at): 2^(s f + m) as f16, hi parts in the first 16 columns and, with two parts,
 // lo parts in the others; sum += them. The hi part is the value cut off after 10 bits of mantissa, so that
-// the lo part needs no conversion back: both together keep 21 bits.
+// the lo part needs no conversion back: both together keep 21 bits (of small ones fewer: see kShift).
 template <int Parts> __device__ __forceinline__ void exp_chunk(const float (&s)[32], F2 f, F2 m, F2 (&sum)[2], uint32_t at) {
     uint32_t ph[16], pl[16];
 #pragma unroll
@@ -991,7 +993,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
                 const float mx = top * f - kShift;   // -inf: no key
                 highest = fmaxf(highest, mx);
                 float rescale = 1.f;
-                if (mx > ref + (step ? 8.f : 0.f)) {   // (-inf + 8 = -inf: the first key of a row sets its reference)
+                if (mx > ref + (step ? kLag : 0.f)) {   // (-inf + 3 = -inf: the first key of a row sets its reference)
                     const float al = ref == -INFINITY ? 1.f : exp2_fast(ref - mx);
                     ref = mx;
                     sum *= al;

@@ -252,8 +252,8 @@ int fl_b200_paged_append(fl_b200_ctx *ctx, const fl_b200_paged_cache *cache, int
  * out that belong to no sequence stay as they are, keys on a page outside the pool count as zero vectors (status 3). What a row does not attend may hold
  * anything; an infinity that it does attend may make it NaN. lse_out
  * (optional): per token and query head (max score, sum of exp(score - max)), (-inf, 0) without a key: what fl_b200_seqpar_combine merges.
- * f32 activations: q and the probabilities go to the tensor cores as two f16 parts each (22 bits), sums in f32; f16
- * activations: as one. out must not overlap q. The first call on a context allocates scratch (65 MB): make it before a capture. */
+ * f32 activations: q and the probabilities go to the tensor cores as two f16 parts each (21 bits; a probability is held to 2^-36 of its row's
+ * largest where that is more), sums in f32; f16 activations: as one. out must not overlap q. The first call on a context allocates scratch (65 MB): make it before a capture. */
 int fl_b200_paged_attn(fl_b200_ctx *ctx, const fl_b200_paged_cache *cache, int act_type, const void *q_dev, uint32_t n_q_head,
                        uint32_t q_stride, const int32_t *table_dev, uint32_t max_blocks, const int32_t *q_start_dev,
                        const int32_t *kv_len_dev, uint32_t n_seq, uint32_t n_tokens, uint32_t max_new, float scale, void *out_dev,

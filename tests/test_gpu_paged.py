@@ -710,3 +710,36 @@ def test_a_row_of_one_key_keeps_its_value(ctx, dim, key):
         assert ((got - want).abs() <= 2.0 ** -20 * want.abs()).all(), ((got - want).abs() / want.abs()).max().item()
         first = c["vs"][s][:, 0].double().repeat_interleave(n_q // n_kv, 0)
         assert ((c["out"].double().view(-1, n_q, dim)[c["start"][s]] - first).abs() <= 2.0 ** -20 * first.abs()).all()
+
+
+@pytest.mark.parametrize("act", ["f32", "f16"])
+@pytest.mark.parametrize("below", [20.3, 30.6, 35.4])
+def test_many_keys_far_below_the_largest(ctx, act, below):
+    """One key, and 20000 at 2^-below of it with values of one sign. A probability is held in two parts to 2^-21 of itself or to 2^-36 of the
+    row's largest (f16: one part, 2^-11 or 2^-37)."""
+    n_q, dim, page, N, new = 128, 64, 64, 20000, 300     # 150 blocks of rows: all keys of most are one CTA's
+    seqs = [(N + new, new)]
+    c = make(int(below), seqs, n_q, 1, dim, page, act)
+    scale = 0.125
+    c["q"].fill_(1.0)
+    c["k"].zero_()
+    c["v"].fill_(1.0)
+    c["ks"][0].zero_()
+    c["vs"][0].fill_(1.0)
+    pg = int(c["table"][0, 0])
+    size = below * math.log(2.0) / (scale * dim)          # the key's dimensions, in f16
+    c["k"][pg, 0, 3], c["ks"][0][0, 3] = size, size
+    c["v"][pg, 0, 3], c["vs"][0][0, 3] = 2.0 ** -12, 2.0 ** -12
+    attn(ctx, c, n_q, 1, dim, page, scale)
+    assert ctx.status() == 0
+    k3 = float(c["ks"][0][0, 3, 0])
+    A = scale * dim * k3
+    for tok in (0, 7, new - 1):
+        keys = N + tok + 1
+        small = math.exp(-A) * (keys - 1)
+        want = (2.0 ** -12 + small) / (1 + small)
+        tol = (A + 1) * 2.0 ** -18 * want + keys * 2.0 ** -36
+        if act == "f16":
+            tol += 2 * 2.0 ** -11 * want + 2.0 ** -25
+        got = c["out"].double().view(-1, n_q, dim)[tok]
+        assert ((got - want).abs() <= tol).all(), ((got - want).abs().max().item(), tol, want)
