@@ -23,7 +23,8 @@
 // The tensor cores truncate their running sum, 3.1e-8 of it per instruction in the mean; with f32 activations half of O's columns are therefore
 // brought out at every tile, in turn, added in f32 to a buffer of the CTA's own that stays in L2, and start from zero: no sum in
 // tensor memory is longer than three tiles (48 instructions). (us with a quarter at every tile, sums of up to eight: 4 x 8 tokens over 4096
-// keys 32.7, now 35.2; 4096 tokens 310, 320; 1000 over 20000 keys 554, 603.)
+// keys 32.7, now 35.2; 4096 tokens 310, 320; 1000 over 20000 keys 554, 603.) f16 activations: at every 128th tile, so that no sum is longer
+// than 129 (1032 instructions, which cut off 2^-13 at most; uncut, rows of a million keys came out 0.7 % too small).
 #include "common.cuh"
 #include "paged.h"
 
@@ -192,8 +193,23 @@ __device__ __noinline__ float move_sums(float4 *mem, uint32_t out, float from, f
     __threadfence();
     return to;
 }
-// (out of line, as load_q and finish are: what they need in registers stays out of the loop over the tiles)
-__device__ __noinline__ void scale_o(uint32_t at, uint32_t columns, float by) {
+// 32 columns of the row's contexts out of tensor memory, where they start from zero, to their sum in memory, times `by`.
+__device__ __forceinline__ void add_out(uint32_t to, float4 *mem, uint32_t c4, float by, bool adds) {
+    float o[32];
+    load32(to + 32 * c4, o);
+    wait_ld(o);
+    const uint32_t zero[16] = {};
+    store16(to + 32 * c4, zero);
+    store16(to + 32 * c4 + 16, zero);
+    float4 *at = mem + 8 * c4 * kRowsL;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float4 v = make_float4(o[4 * j] * by, o[4 * j + 1] * by, o[4 * j + 2] * by, o[4 * j + 3] * by);
+        if (adds) add4(at + j * kRowsL, v);
+        else __stcg(at + j * kRowsL, v);
+    }
+}
+__device__ __forceinline__ void scale_o(uint32_t at, uint32_t columns, float by) {
 #pragma unroll 1
     for (uint32_t c = 0; c < columns; c += 32) {
         float o[32];
@@ -207,6 +223,66 @@ __device__ __noinline__ void scale_o(uint32_t at, uint32_t columns, float by) {
             store16(at + c + 16 * h, w);
         }
     }
+}
+// f16 activations: a half of the contexts goes out at steps n kOutHalf and n kOutHalf + 1, and comes back at the piece's end. What went out
+// follows from the step, and the reference of the sums lies beside them, so that the loop over the tiles holds nothing of it. (us at 4096 tokens with heads of 64, and at 2048 tokens over 30000 keys:
+// without 152, 970; this 157, 990; as a call of its own in the loop, every 64th tile, 167, 1010.)
+constexpr uint32_t kOutHalf = 128;
+__device__ __forceinline__ bool half_goes(uint32_t step) { return step >= kOutHalf && step % kOutHalf < 2; }
+template <int D> __device__ __forceinline__ uint32_t halves_out(uint32_t steps) {   // in front of step `steps`: bit c: columns 32 c ..
+    constexpr uint32_t kHalf = (1u << D / 64) - 1u;
+    return (steps > kOutHalf ? kHalf : 0u) | (steps > kOutHalf + 1 ? kHalf << D / 64 : 0u);
+}
+template <int D> __device__ __forceinline__ float *half_sums(const PagedAttnArgs &a) {   // of the warp's lane: [D / 4][128 rows][4], a row each, references
+    return a.part_tm + ((uint64_t)gridDim.x * 4 + blockIdx.x * 2 + (threadIdx.x >> 7)) * Tm<D, 1>::kRecord;
+}
+// The row's contexts times `by`, where that changes its reference to ref. (Out of line, as load_q and finish are: what they need in registers stays out
+// of the loop over the tiles.)
+template <int D, int Parts> __device__ __noinline__ void change_o(const PagedAttnArgs &a, uint32_t to, float by, uint32_t step, float ref) {
+    if (__any_sync(0xffffffffu, by != 1.f)) scale_o(to, D, by);
+    if (Parts == 2 || !half_goes(step)) return;
+    wait_st();
+    const uint32_t out = halves_out<D>(step), r = threadIdx.x & (kRowsL - 1);
+    float *sums = half_sums<D>(a), *at = sums + (D + 1) * kRowsL + r;
+    float4 *mem = reinterpret_cast<float4 *>(sums) + r;
+    if (out) {
+        const float from = __ldcg(at);
+        if (from != ref) move_sums(mem, out, from, ref);
+    }
+    __stcg(at, ref);
+#pragma unroll 1
+    for (uint32_t c4 = (step & 1u) * (D / 64); c4 < ((step & 1u) + 1) * (D / 64); ++c4) add_out(to, mem, c4, 1.f, out >> c4 & 1u);
+}
+template <int D> __device__ __noinline__ void halves_back(const PagedAttnArgs &a, uint32_t to, uint32_t steps, float ref) {
+    const uint32_t out = halves_out<D>(steps), r = threadIdx.x & (kRowsL - 1);
+    const float *sums = half_sums<D>(a);
+    __threadfence();   // (the additions come before the loads)
+    const float from = __ldcg(sums + (D + 1) * kRowsL + r), by = from == ref ? 1.f : exp2_fast(from - ref);
+#pragma unroll 1
+    for (uint32_t c = 0; c < D / 32; ++c)
+        if (out >> c & 1u) {
+            float4 v[8];
+            float o[32];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = __ldcg(reinterpret_cast<const float4 *>(sums) + (8 * c + j) * kRowsL + r);
+            load32(to + 32 * c, o);
+            wait_ld(o);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t w[16];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float4 x = v[4 * h + j];
+                    const float *y = o + 16 * h + 4 * j;
+                    w[4 * j] = __float_as_uint(fmaf(x.x, by, y[0]));
+                    w[4 * j + 1] = __float_as_uint(fmaf(x.y, by, y[1]));
+                    w[4 * j + 2] = __float_as_uint(fmaf(x.z, by, y[2]));
+                    w[4 * j + 3] = __float_as_uint(fmaf(x.w, by, y[3]));
+                }
+                store16(to + 32 * c + 16 * h, w);
+            }
+        }
+    wait_st();
 }
 // 32 scores to probabilities, in place in tensor memory (at): 2^(s f + m) as f16, hi parts in the first 16 columns and, with two parts,
 // lo parts in the others; sum += them. The hi part is the value cut off after 10 bits of mantissa, so that
@@ -948,21 +1024,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
                     if (ref - acc_ref > 40.f) acc_ref = move_sums(acc_mem, out_of, acc_ref, ref);   // (far below what f32 holds: |O| < 2^47)
                     const float by = ref == acc_ref ? 1.f : exp2_fast(ref - acc_ref);
 #pragma unroll 1
-                    for (uint32_t c4 = (step & 1u) * (D / 64); c4 < ((step & 1u) + 1) * (D / 64); ++c4) {   // 32 columns
-                        float o[32];
-                        load32(to + 32 * c4, o);
-                        wait_ld(o);
-                        const uint32_t zero[16] = {};
-                        store16(to + 32 * c4, zero);
-                        store16(to + 32 * c4 + 16, zero);
-                        float4 *at = acc_mem + 8 * c4 * kRowsL;
-                        const bool adds = out_of >> c4 & 1u;
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const float4 v = make_float4(o[4 * j] * by, o[4 * j + 1] * by, o[4 * j + 2] * by, o[4 * j + 3] * by);
-                            if (adds) add4(at + j * kRowsL, v);
-                            else __stcg(at + j * kRowsL, v);
-                        }
+                    for (uint32_t c4 = (step & 1u) * (D / 64); c4 < ((step & 1u) + 1) * (D / 64); ++c4) {
+                        add_out(to, acc_mem, c4, by, out_of >> c4 & 1u);
                         out_of |= 1u << c4;
                     }
                 }
@@ -999,7 +1062,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
                     sum *= al;
                     rescale = al;
                 }
-                if (step && __any_sync(0xffffffffu, rescale != 1.f)) scale_o(to, D, rescale);
+                if (step && (__any_sync(0xffffffffu, rescale != 1.f) || (Parts == 1 && half_goes(step)))) change_o<D, Parts>(a, to, rescale, step, ref);
                 const float m = ref == -INFINITY ? 0.f : ref;
                 const F2 f2 = pair(f, f), m2 = pair(-m, -m);
                 F2 part[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
@@ -1034,6 +1097,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
                 fence_after();
                 if (Parts == 2) __threadfence();   // (the additions to the sums in memory come before the loads below)
             }
+            if (Parts == 1 && active && steps > kOutHalf && !dead) halves_back<D>(a, to, steps, ref);
             finish<D, Parts>(a, hd, q_s, Sums{ref, sum, highest, acc_ref, out_of}, steps != 0 && !dead, tmem);
             fence_before();
             bar_both();   // both lanes are done with q, O and the notes

@@ -743,3 +743,24 @@ def test_many_keys_far_below_the_largest(ctx, act, below):
             tol += 2 * 2.0 ** -11 * want + 2.0 ** -25
         got = c["out"].double().view(-1, n_q, dim)[tok]
         assert ((got - want).abs() <= tol).all(), ((got - want).abs().max().item(), tol, want)
+
+
+@pytest.mark.parametrize("act", ["f32", "f16"])
+def test_rows_of_a_million_keys(ctx, act):
+    """Long sums, which tensor memory truncates at every instruction, in pieces of thousands of tiles: values of one come back as one. The sums
+    of 2^13 tiles round to f32 at every tile (4 deviations: 4 2^-24 2^6.5 3^-1 for steps of a growing sum, numerator and denominator: 2^-17.1); f16: up to
+    2^-13 cut off sums in tensor memory, the
+    probabilities' roundings, 2^-11 at most and of either sign (over 2^20 keys 4 2^-11 3^-0.5 2^-10: 2^-19.8), and the result's half step."""
+    from fast_llm_b200 import paged
+    n_q, dim, page, N, new = 128, 64, 256, 1 << 20, 300   # 150 blocks of rows: all keys of most are one CTA's
+    g = torch.Generator(device="cuda").manual_seed(20)
+    k, v = torch.zeros((N // page, 1, page, dim), device="cuda", dtype=torch.float16), torch.ones((N // page, 1, page, dim), device="cuda", dtype=torch.float16)
+    k[..., 0] = 8 * torch.rand((N // page, 1, page), generator=g, device="cuda")
+    q = torch.ones((new, n_q * dim), device="cuda", dtype=DT[act])
+    out = torch.full_like(q, CANARY)
+    cache = paged.PagedCache(ctx, k, v, N // page, page, 1, dim)
+    torch.cuda.synchronize()
+    cache.attn(q, torch.arange(N // page, dtype=torch.int32, device="cuda").view(1, -1), ints([0, new]), ints([N]), new, 0.125, out)
+    ctx.sync()
+    assert ctx.status() == 0
+    assert ((out.double() - 1).abs() <= 2.0 ** -17 + (2.0 ** -13 + 2.0 ** -19 + 2.0 ** -11 if act == "f16" else 0)).all(), (out.double() - 1).abs().max().item()
