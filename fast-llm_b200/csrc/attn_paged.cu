@@ -356,7 +356,7 @@ __device__ __forceinline__ void build_q(const PagedAttnArgs &a, FewSmem<D> &sm, 
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     // a power of two brings the row's largest value to [2^11, 2^12)
-    const int e = min(100, max(-100, 138 - (int)(__float_as_uint(top) >> 23)));
+    const int e = min(126, max(-116, 138 - (int)(__float_as_uint(top) >> 23)));   // (-116: the largest f32; 2^-126 is a normal one)
     const float up = __uint_as_float((uint32_t)(e + 127) << 23);
     if (t == 0 && !(g & 1u)) sm.f[row] = fmaxf(a.scale * 1.44269504088896341f * __uint_as_float((uint32_t)(127 - e) << 23), 1e-37f);
     uint2 *to = reinterpret_cast<uint2 *>(sm.o) + n * (D / 16) * 32 + lane;

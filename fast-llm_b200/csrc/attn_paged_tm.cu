@@ -349,7 +349,7 @@ __device__ __noinline__ float load_q(const PagedAttnArgs &a, uint8_t *dst, uint6
                 for (int j = 0; j < V; ++j) top = fmaxf(top, fabsf(x[i][k][j]));
 #pragma unroll
             for (int o = 4; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const int e = min(100, max(-100, 138 - (int)(__float_as_uint(top) >> 23)));
+            const int e = min(126, max(-116, 138 - (int)(__float_as_uint(top) >> 23)));   // (-116: the largest f32; 2^-126 is a normal one)
             const float up = __uint_as_float((uint32_t)(e + 127) << 23);
             const float mine = fmaxf(a.scale * 1.44269504088896341f * __uint_as_float((uint32_t)(127 - e) << 23), 1e-37f);
             const float got = __shfl_sync(0xffffffffu, mine, (lane >> 2 & 3u) * 8);

@@ -764,3 +764,14 @@ def test_rows_of_a_million_keys(ctx, act):
     ctx.sync()
     assert ctx.status() == 0
     assert ((out.double() - 1).abs() <= 2.0 ** -17 + (2.0 ** -13 + 2.0 ** -19 + 2.0 ** -11 if act == "f16" else 0)).all(), (out.double() - 1).abs().max().item()
+
+
+@pytest.mark.parametrize("seqs", [[(200, 3), (77, 1)], [(130, 70)]])
+@pytest.mark.parametrize("q_size,k_size", [(1e35, 1e-4), (3e37, 1e-4), (1e-34, 1.0), (1e-37, 1.0)])
+def test_rows_of_q_at_the_ends_of_f32(ctx, q_size, k_size, seqs):
+    c = make(9, seqs, 8, 2, 128, 16, "f32", kv_scale=k_size)
+    c["q"].mul_(q_size)
+    scale = 1.0 / (q_size * k_size * math.sqrt(128))
+    assert torch.isfinite(c["q"]).all()
+    attn(ctx, c, 8, 2, 128, 16, scale)
+    check(ctx, c, seqs, 8, 2, 128, scale, "f32")
