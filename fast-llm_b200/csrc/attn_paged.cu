@@ -37,32 +37,6 @@ __device__ __forceinline__ uint32_t rows_of(const PagedAttnArgs &a, const PagedS
 __device__ __forceinline__ uint32_t tiles_of(const PagedSeq &q) { return max(1u, ((uint32_t)max(0, q.past + (int32_t)q.n) + kTile - 1) / kTile); }
 __device__ __forceinline__ uint64_t units_of(const PagedAttnArgs &a, const PagedSeq &q) { return rows_of(a, q) ? (uint64_t)tiles_of(q) * a.n_kv : 0u; }
 
-// An end of a share that lies in a sequence's tiles b .. e over one KV head, within kSnap tiles of b or e, moves there: a CTA with a few
-// tiles of another head builds rows of q, leaves a record, is the last to arrive at both and adds the records of both (one sequence over 8000
-// keys 17.0 us, moved 15.1; 4 over 1023 13.0, 10.2; 8 over 2000 17.6, 15.4; 16 over 5500 to 8192, where shares are long, 78.1, 78.6). Up by
-// less than half a share, down by half of one at most, so that none gets empty.
-constexpr uint32_t kSnap = 4;
-// The line over at most `ctas` CTAs: where shares are that small no more of them than keep the largest one, which leaves fewer records. (Longer
-// shares: all of them, for the HBM's sake; 16 x 5500 to 8192 keys 78.5 us, 79.9 with 292 CTAs of 296.)
-__device__ __forceinline__ Shares few_shares(uint32_t units, uint32_t ctas) {
-    const uint32_t most = units / ctas + (units % ctas ? 1u : 0u);
-    return shares_of(units, most == 0 || most > 2 * kSnap ? ctas : units / most + (units % most ? 1u : 0u));
-}
-__device__ __forceinline__ uint32_t snapped(const Shares &sh, uint32_t snap, uint32_t at, uint32_t b, uint32_t e) {
-    const uint32_t down = at - b, up = e - at;
-    const bool may_down = down <= snap && 2 * down <= sh.each, may_up = up <= snap && 2 * up < sh.each;
-    return may_down && (!may_up || down <= up) ? b : may_up ? e : at;
-}
-// The first and the last CTA of tiles b .. e - 1
-__device__ __forceinline__ uint32_t first_of(const Shares &sh, uint32_t snap, uint32_t b, uint32_t e) {
-    const uint32_t c = owner_of(sh, b), hi = share_lo(sh, c + 1);
-    return hi < e && snapped(sh, snap, hi, b, e) == b ? c + 1 : c;
-}
-__device__ __forceinline__ uint32_t last_of(const Shares &sh, uint32_t snap, uint32_t b, uint32_t e) {
-    const uint32_t c = owner_of(sh, e - 1), lo = share_lo(sh, c);
-    return lo > b && snapped(sh, snap, lo, b, e) == e ? c - 1 : c;
-}
-
 // The pieces of a CTA's share: consecutive tiles of one sequence over one KV head.
 struct Piece {
     PagedSeq q;
@@ -160,7 +134,7 @@ template <int D>
 __device__ __forceinline__ void copy_tiles(const PagedAttnArgs &a, FewSmem<D> &sm, Walk &walk, Piece &p) {
     constexpr uint32_t kKV = FewSmem<D>::kHalfStage;
     const uint32_t lane = threadIdx.x & 31u, shift = min(a.page_shift, 6u), boxes = kTile >> shift;
-    const uint32_t page_groups = (1u << a.page_shift) >> 3, in_page = (1u << a.page_shift) - 1u;
+    const uint32_t behind = pool_groups(a.n_pages, a.n_kv, a.page_shift);
     uint32_t issued = 0, stage = 0, parity = 1;
     bool landed = true;
     do {
@@ -168,9 +142,9 @@ __device__ __forceinline__ void copy_tiles(const PagedAttnArgs &a, FewSmem<D> &s
 #pragma unroll 1
         for (uint32_t tile = p.t0; tile < p.t1; ++tile) {
             const uint32_t key = tile * kTile + (lane << shift);
-            uint32_t at = a.n_pages * a.n_kv * page_groups;   // behind the pool: copies from there bring zeros
+            uint32_t at = behind;
             if (lane < boxes && key < (uint32_t)p.keys) {
-                if ((uint32_t)page < a.n_pages) at = ((uint32_t)page * a.n_kv + p.hkv) * page_groups + ((key & in_page) >> 3);
+                if (page_there(page, a.n_pages)) at = page_group((uint32_t)page, a.n_kv, p.hkv, a.page_shift, key);
                 else atomicCAS(a.status, ST_OK, ST_PAGED_PAGE);
             }
             if (tile + 1 < p.t1) page = page_at(a, p, tile + 1);
@@ -435,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
         const uint32_t tiles = max(1u, u / a.n_kv);   // (of the lane's sequence over a KV head)
         auto edge = [&](uint32_t c) {
             const uint32_t at = share_lo(sh, c);
-            if (c == 0 || c == sh.n || sh.each < 2) return at;   // (shares of a tile cannot move: the smallest calls, 9.8 -> 9.4 us)
+            if (!edge_moves(sh, c)) return at;
             const int src = __ffs(__ballot_sync(0xffffffffu, at < x)) - 1;
             const uint32_t n = __shfl_sync(0xffffffffu, tiles, src), b = at - (at - __shfl_sync(0xffffffffu, x - u, src)) % n;
             return snapped(sh, kSnap, at, b, b + n);

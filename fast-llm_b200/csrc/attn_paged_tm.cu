@@ -447,10 +447,9 @@ __device__ __forceinline__ uint64_t head_units(const PagedAttnArgs &a, const Pag
 
 // The tiles of the piece that begins at w.pos, in the block in p; false: there are none.
 __device__ __forceinline__ bool cut_piece(Walk &w, Piece &p) {
-    const uint32_t front = p.base + kStart, shift = tile_units(p.b.rows) - 1u;
-    auto tile = [&](uint32_t unit) { return unit > front ? min(p.b.tiles, (unit - front + shift) >> shift) : 0u; };
-    p.t0 = tile(w.pos);
-    p.t1 = tile(w.hi);
+    const uint32_t front = p.base + kStart, per = tile_units(p.b.rows);
+    p.t0 = tile_at_unit(w.pos, front, p.b.tiles, per);
+    p.t1 = tile_at_unit(w.hi, front, p.b.tiles, per);
     w.pos = min(w.hi, p.base + p.b.units);
     return p.t0 < p.t1;
 }
@@ -647,10 +646,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
     if (tid == 0) a.blocks[blockIdx.x].records = 0;
 
     // ---- this CTA's share of the line: every warp by itself for up to 32 sequences ----
-    auto shares = [](uint32_t units) {   // (two units at least: every CTA between a block's first and last one has a tile of it)
-        const uint32_t n = min(gridDim.x, units / 2);
-        return n ? Shares{n, units / n, units % n} : Shares{0, 0, 0};
-    };
     Shares sh;
     Walk walk;
     Piece p;
@@ -668,7 +663,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
             if (lane >= (uint32_t)o) x += y;
         }
         if (bad && blockIdx.x == 0) atomicCAS(a.status, ST_OK, ST_PAGED_ARGS);
-        sh = shares(__shfl_sync(0xffffffffu, x, 31));
+        sh = tm_shares(__shfl_sync(0xffffffffu, x, 31), gridDim.x);
         walk = Walk{share_lo(sh, blockIdx.x), share_lo(sh, blockIdx.x + 1)};
         const uint32_t at = __ballot_sync(0xffffffffu, walk.pos < x);   // sequences that end behind the share's begin
         const int src = at ? __ffs(at) - 1 : 0;
@@ -691,7 +686,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
         __syncthreads();
         for (uint32_t w = 0; w < kThreads / 32; ++w) total += hd.sum[w];
         if ((bad || total >> 32) && blockIdx.x == 0) atomicCAS(a.status, ST_OK, ST_PAGED_ARGS);
-        sh = shares(total >> 32 ? 0u : (uint32_t)total);
+        sh = tm_shares(total >> 32 ? 0u : (uint32_t)total, gridDim.x);
         walk = Walk{share_lo(sh, blockIdx.x), share_lo(sh, blockIdx.x + 1)};
         uint64_t run = 0;
         for (uint32_t s0 = 0; s0 < a.n_seq && blockIdx.x < sh.n && run <= walk.pos; s0 += kThreads) {
@@ -743,7 +738,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
     if (warp == kCopyWarp) {
         // ---- copies ----
         const uint32_t box = min(1u << a.page_shift, kTile), boxes = kTile / box, bytes = box * D * 2;
-        const uint32_t page_groups = (1u << a.page_shift) >> 3, outside = a.n_pages * a.n_kv * page_groups;
+        const uint32_t outside = pool_groups(a.n_pages, a.n_kv, a.page_shift);
         uint32_t issued = 0;
         for (bool more = some; more && !dead; more = next_piece(a, walk, p)) {
             const int32_t *row = a.table + (uint64_t)p.seq * a.max_blocks;
@@ -760,7 +755,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
                 const uint32_t tile = tile_at(i, v), key = tile * kTile + lane * box, slot = (done + i) % T::kSlots, par = ((done + i) / T::kSlots) & 1u;
                 uint32_t at = outside;   // copies from there bring zeros
                 if (lane < boxes && key < (uint32_t)p.b.keys) {
-                    if ((uint32_t)page < a.n_pages) at = ((uint32_t)page * a.n_kv + p.hkv) * page_groups + ((key & ((1u << a.page_shift) - 1u)) >> 3);
+                    if (page_there(page, a.n_pages)) at = page_group((uint32_t)page, a.n_kv, p.hkv, a.page_shift, key);
                     else atomicCAS(a.status, ST_OK, ST_PAGED_PAGE);
                 }
                 bool v2;

@@ -6,6 +6,7 @@
 #pragma once
 #include "../../include/fl_b200.h"
 #include "kernels.h"
+#include "paged_line.h"
 
 namespace flb {
 
@@ -59,18 +60,6 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedAttnArgs &a, uint32_t s
     bad = b < 0 || e < b || (uint32_t)e > a.n_tokens || (uint32_t)(e - b) > a.max_new || len < 0 || (uint64_t)len > room;
     return bad ? PagedSeq{0, 0, 0} : PagedSeq{(uint32_t)b, (uint32_t)(e - b), len - (e - b)};
 }
-// The line's units over n CTAs, equal shares up to one unit; none is empty (n <= units). 32 bits: a call with 2^32 units or more is refused.
-struct Shares { uint32_t n, each, more; };   // the first `more` CTAs have one unit more than `each`
-__device__ __forceinline__ Shares shares_of(uint32_t units, uint32_t ctas) {
-    const uint32_t n = min(ctas, units);
-    return n ? Shares{n, units / n, units % n} : Shares{0, 0, 0};
-}
-__device__ __forceinline__ uint32_t share_lo(const Shares &s, uint32_t c) { return s.each * c + min(c, s.more); }
-__device__ __forceinline__ uint32_t owner_of(const Shares &s, uint32_t u) {   // the CTA whose share holds unit u
-    const uint32_t front = s.more * (s.each + 1);
-    return u < front ? u / (s.each + 1) : s.more + (u - front) / s.each;
-}
-
 // Values of +inf, -inf and NaN (class 0, 1, 2) among the keys that only part of the rows attend: per class and dimension the
 // first such key. A row that attends keys 0 .. lim is affected by those <= lim.
 __device__ __forceinline__ float unfinite_of(const uint32_t *u, uint32_t dims, uint32_t d, int32_t lim) {
