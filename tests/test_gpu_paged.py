@@ -775,3 +775,63 @@ def test_rows_of_q_at_the_ends_of_f32(ctx, q_size, k_size, seqs):
     assert torch.isfinite(c["q"]).all()
     attn(ctx, c, 8, 2, 128, 16, scale)
     check(ctx, c, seqs, 8, 2, 128, scale, "f32")
+
+
+@pytest.mark.parametrize("act", ["f32", "f16"])
+@pytest.mark.parametrize("n_q,n_kv,dim,seqs", [(8, 2, 128, [(900, 1), (3000, 3), (0, 1), (2, 4)]), (8, 2, 64, [(1500, 90), (700, 1), (3, 40)]), (32, 8, 128, [(1200, 600), (1000, 1000)])])
+@pytest.mark.parametrize("rising", [False, True])
+def test_lse_is_the_maximum_and_the_sum(ctx, n_q, n_kv, dim, seqs, act, rising):
+    """Each of the two for itself, which what merges parts of a sequence needs. rising: the maximum grows by 0.3 exponents per 64 keys, so that references
+    lag it. A score is off by 2^-19 A (see above), the maximum's product by 2^-23 of it, the sum by twice the scores', 2^-21 of the probabilities and 2^-18 for its roundings."""
+    page = 16
+    c = make(len(seqs) + dim, seqs, n_q, n_kv, dim, page, act)
+    scale = 1.0 / math.sqrt(dim)
+    if rising:
+        c["q"].fill_(1.0)
+        for s, (L, _) in enumerate(seqs):
+            j = torch.arange(L, device="cuda")
+            c["ks"][s].zero_()
+            c["ks"][s][:, :, 0] = ((j // 64) * 0.2 / scale * (j % 64 == 17)).half()
+            c["k"][c["table"][s].long()[j // page], :, j % page] = c["ks"][s].transpose(0, 1)
+    attn(ctx, c, n_q, n_kv, dim, page, scale)
+    assert ctx.status() == 0
+    _, _, want = expect(c, seqs, n_q, n_kv, dim, scale, act)
+    q = c["q"].double().abs().view(-1, n_q, dim)
+    for s, (L, m) in enumerate(seqs):
+        if not m:
+            continue
+        a = slice(c["start"][s], c["start"][s] + m)
+        A = torch.zeros((m, n_q), dtype=torch.float64, device="cuda")
+        for h in range(n_q):
+            if L:
+                A[:, h] = (q[a, h] @ c["ks"][s][h * n_kv // n_q].double().abs().t() * scale).amax(-1)
+        got = c["lse"][a].double()
+        none = want[a, :, 0] == -math.inf
+        assert (got[none] == want[a][none]).all()
+        m_off, s_off = (got[..., 0] - want[a, :, 0]).abs(), (got[..., 1] - want[a, :, 1]).abs()
+        assert (m_off <= A * 2.0 ** -19 + 2.0 ** -22 * want[a, :, 0].abs())[~none].all()
+        assert (s_off <= (2 * A * 2.0 ** -19 + 2.0 ** -18 + 2.0 ** -21) * want[a, :, 1])[~none].all()
+
+
+@pytest.mark.parametrize("n_seq,new,kv_len", [(66, 1, 1 << 22), (1, 1, (1 << 22) + 64), (33, 17, 1 << 24), (32, 17, 1 << 24)])
+def test_lines_that_32_bits_do_not_hold(ctx, n_seq, new, kv_len):
+    """Sequences of together 2^32 tiles or more over all KV heads (one: 2^26), which can share their pages: reported, nothing is written."""
+    from fast_llm_b200 import paged
+    n_kv, dim, page = 1024, 64, 256
+    k = torch.zeros((1, n_kv, page, dim), device="cuda", dtype=torch.float16)
+    table = torch.zeros((n_seq, -(-kv_len // page)), dtype=torch.int32, device="cuda")
+    q = torch.ones((n_seq * new, n_kv * dim), device="cuda", dtype=torch.float16)
+    out = torch.full_like(q, CANARY)
+    cache = paged.PagedCache(ctx, k, k, 1, page, n_kv, dim)
+    torch.cuda.synchronize()
+    cache.attn(q, table, ints([i * new for i in range(n_seq + 1)]), ints([kv_len] * n_seq), new, 0.125, out)
+    ctx.sync()
+    assert ctx.status() == 4
+    assert (out == CANARY).all()
+
+
+def test_plan_without_tokens(ctx):
+    """A step in which requests only end or are rewound."""
+    got = run_plan(ctx, [40, 17], [0, 5], [0, 0], [[0, 1, 2], [3, 4, -1]], [-1] * 5, 0, 16, 0)
+    assert ctx.status() == 0
+    assert got == dict(table=[[0, 1, 2], [3, 4, -1]], free=[0, 1, 2, 4, -1], count=4, pos=[], slot=[], start=[0, 0, 0], length=[0, 5])
