@@ -597,9 +597,11 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
             fence_acq_rel_gpu();
             bar_consumers();
             if (tid == 0) {   // (the ticket is the next launch's again whatever became of this one)
-                const bool last = atomicAdd(&a.tickets[c0], 1u) == pieces - 1;
+                const bool gave_up = sm.abort_flag != 0;
+                const uint32_t before = atomicAdd(&a.tickets[c0], ticket_step(gave_up));
+                const bool last = ticket_last(before, pieces);
                 if (last) a.tickets[c0] = 0;
-                if (last && !sm.abort_flag) sm.late[sm.n_late++] = Late{p.q, p.hkv, p.rows, c0, pieces};
+                if (last && ticket_complete(before, gave_up)) sm.late[sm.n_late++] = Late{p.q, p.hkv, p.rows, c0, pieces};
             }
         }
         bar_consumers();   // (also: everybody has read the unfinite values)

@@ -55,6 +55,12 @@ FLB_HD uint32_t last_of(const Shares &sh, uint32_t snap, uint32_t b, uint32_t e)
     return lo > b && snapped(sh, snap, lo, b, e) == e ? c - 1 : c;
 }
 
+// A run's ticket, zero between launches: CTAs that arrived in the low half, those of them that gave up a wait, and left no record, in the high half. The
+// last to arrive resets it, and adds the records where there are all of them.
+FLB_HD uint32_t ticket_step(bool gave_up) { return gave_up ? 0x10001u : 1u; }
+FLB_HD bool ticket_last(uint32_t before, uint32_t pieces) { return (before & 0xFFFFu) == pieces - 1; }
+FLB_HD bool ticket_complete(uint32_t before, bool gave_up) { return before >> 16 == 0 && !gave_up; }
+
 // ---- many rows (attn_paged_tm.cu): a block of rows is `front` units, then tile_units for every tile ----------------------------
 // Two units at least, so that every CTA between a block's first and last one has a tile of it.
 FLB_HD Shares tm_shares(uint32_t units, uint32_t ctas) { return shares_of(units, lesser(ctas, units / 2)); }

@@ -1,5 +1,5 @@
 // Runs the paged attention's own share and page arithmetic (csrc/paged_line.h) over random and extreme lines and checks it against the plain
-// statement of what it stands for. usage: paged_line_model few|tm|large|pages SEED
+// statement of what it stands for. usage: paged_line_model few|tickets|tm|large|pages SEED
 #include "paged_line.h"
 
 #include <cstdio>
@@ -49,6 +49,27 @@ static int few(Rng &g) {
             for (uint32_t c = first + 1; c <= last; ++c) CHECK(edge[c] > b && edge[c] < e);
             if (last > first) CHECK(begins[first]++ == 0);   // (one run at most begins in a CTA and goes on: one ticket, one second record)
         }
+    }
+    return 0;
+}
+// Whoever arrives last, and whoever gave up: the ticket is zero again, one CTA is the last, and it adds records only where all are there.
+static int tickets(Rng &g) {
+    for (int it = 0; it < 20000; ++it) {
+        const uint32_t pieces = pick(g, 1, 296), rare = pick(g, 1, 400);
+        uint32_t ticket = 0, lasts = 0;
+        bool any_gave_up = false, added = false;
+        for (uint32_t i = 0; i < pieces; ++i) {
+            const bool gave_up = pick(g, 1, rare) == 1;
+            any_gave_up |= gave_up;
+            const uint32_t before = ticket;
+            ticket += ticket_step(gave_up);
+            if (ticket_last(before, pieces)) {
+                ++lasts;
+                ticket = 0;
+                added = ticket_complete(before, gave_up);
+            }
+        }
+        CHECK(ticket == 0 && lasts == 1 && added == !any_gave_up);
     }
     return 0;
 }
@@ -116,5 +137,5 @@ int main(int argc, char **argv) {
     if (argc != 3) return 2;
     Rng g((uint32_t)std::atoi(argv[2]));
     const char *w = argv[1];
-    return !std::strcmp(w, "few") ? few(g) : !std::strcmp(w, "tm") ? tm(g) : !std::strcmp(w, "large") ? large(g) : !std::strcmp(w, "pages") ? pages(g) : 2;
+    return !std::strcmp(w, "few") ? few(g) : !std::strcmp(w, "tickets") ? tickets(g) : !std::strcmp(w, "tm") ? tm(g) : !std::strcmp(w, "large") ? large(g) : !std::strcmp(w, "pages") ? pages(g) : 2;
 }

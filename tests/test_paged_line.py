@@ -17,7 +17,7 @@ def model(tmp_path_factory):
 
 
 @pytest.mark.parametrize("seed", [1, 2])
-@pytest.mark.parametrize("what", ["few", "tm", "large", "pages"])
+@pytest.mark.parametrize("what", ["few", "tickets", "tm", "large", "pages"])
 def test_shares_and_pages(model, what, seed):
     r = subprocess.run([model, what, str(seed)], stdout=subprocess.PIPE, text=True, timeout=300)
     assert r.returncode == 0, r.stdout
