@@ -518,6 +518,7 @@ __device__ __forceinline__ bool partly(const PagedAttnArgs &a, const Piece &p, u
 }
 
 __device__ __forceinline__ void bar_both() { asm volatile("bar.sync 1, 256;" ::: "memory"); }   // the softmax warps
+__device__ __forceinline__ bool given_up(const Head &hd) { return *static_cast<const volatile uint32_t *>(&hd.abort_flag) != 0; }
 
 // The rows of q of a piece to L2 (a warp).
 template <int D, int Parts>
@@ -528,6 +529,7 @@ __device__ __noinline__ void prefetch_q(const PagedAttnArgs &a, const Piece p) {
         for (uint32_t c = 0; c < D * 2 * Parts; c += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(from + c));
     }
 }
+__device__ __forceinline__ uint32_t *records_left(const PagedAttnArgs &a) { return reinterpret_cast<uint32_t *>(a.blocks + gridDim.x); }
 struct Sums { float ref, sum, highest, acc_ref; uint32_t out_of; };   // of a row
 // The results of a lane's piece: the rows themselves, or a record. done: the lane has any, and they are in tensor memory.
 template <int D, int Parts>
@@ -562,7 +564,7 @@ __device__ __noinline__ void finish(const PagedAttnArgs &a, Head &hd, uint8_t *q
             ref2 = w[0]; sum2 = w[1]; highest = fmaxf(highest, w[2]); out2 = __float_as_uint(w[3]); acc2_ref = w[4];
         }
     }
-    if (done && active && !(sm && l)) {
+    if (done && active && !(sm && (l || given_up(hd)))) {   // (what the second lane hands over is its own where nobody gave up)
         const bool whole = job.whole, two = sm && job.n > 1;
         const float both = fmaxf(ref, ref2), w1 = ref == -INFINITY ? 0.f : exp2_fast(ref - both), w2 = ref2 == -INFINITY ? 0.f : exp2_fast(ref2 - both);
         const float all = fmaf(sum, w1, sum2 * w2), inv = lim < 0 ? 0.f : 1.f / all;
@@ -643,7 +645,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
         fence_barrier_init();
     }
     griddep_wait();
-    if (tid == 0) a.blocks[blockIdx.x].records = 0;
+    if (tid == 0) {
+        a.blocks[blockIdx.x].records = 0;
+        records_left(a)[2 * blockIdx.x] = records_left(a)[2 * blockIdx.x + 1] = 0;
+    }
 
     // ---- this CTA's share of the line: every warp by itself for up to 32 sequences ----
     Shares sh;
@@ -1096,6 +1101,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
             finish<D, Parts>(a, hd, q_s, Sums{ref, sum, highest, acc_ref, out_of}, steps != 0 && !dead, tmem);
             fence_before();
             bar_both();   // both lanes are done with q, O and the notes
+            if (tid == 0 && !job.whole && !given_up(hd)) records_left(a)[2 * blockIdx.x + job.slot] = 1;
             if (hd.any_unfinite) {
                 for (uint32_t i = tid; i < 3 * D; i += 256) hd.unfinite[i] = 0x7fffffffu;
                 bar_both();
@@ -1128,10 +1134,12 @@ __global__ void __launch_bounds__(kCombineThreads) paged_tm_combine_kernel(const
     const uint32_t rw = threadIdx.x % kCombineRows, c = threadIdx.x / kCombineRows, lane_of = row0 / kRowsL, r = row0 % kRowsL + rw;
     const uint32_t at = b.row0 + row0 + rw, tok = at / a.group, head = b.hkv * a.group + at - tok * a.group;
     const bool there = row0 + rw < b.rows;
-    auto record = [&](uint32_t i) { return a.part_tm + (uint64_t)(((blockIdx.x + i) * 2 + (i ? 0 : b.slot)) * 2 + lane_of) * kRecord; };
+    auto record = [&](uint32_t i) { return a.part_tm + (uint64_t)(record_index(blockIdx.x, i, b.slot) * 2 + lane_of) * kRecord; };
     float from = -INFINITY, high = -INFINITY, sum = 0.f;
+    uint32_t all = 1;   // (a CTA whose wait ran out left no record: nobody writes)
 #pragma unroll 4
     for (uint32_t i = 0; i < b.records; ++i) {
+        all &= __ldcg(records_left(a) + record_index(blockIdx.x, i, b.slot));
         from = fmaxf(from, __ldcg(record(i) + D * kRowsL + r));
         high = fmaxf(high, __ldcg(record(i) + (D + 2) * kRowsL + r));
     }
@@ -1152,8 +1160,9 @@ __global__ void __launch_bounds__(kCombineThreads) paged_tm_combine_kernel(const
     const float inv = b.past + (int32_t)tok < 0 ? 0.f : 1.f / sum;
 #pragma unroll
     for (uint32_t j = 0; j < kPer; ++j) rows_s[rw][c + j * kStep] = make_float4(v[j].x * inv, v[j].y * inv, v[j].z * inv, v[j].w * inv);
-    if (c == 0 && there && a.lse) a.lse[(uint64_t)(b.first + tok) * a.n_kv * a.group + head] = lse_of(high, from, sum);
+    if (c == 0 && there && all && a.lse) a.lse[(uint64_t)(b.first + tok) * a.n_kv * a.group + head] = lse_of(high, from, sum);
     __syncthreads();
+    if (!all) return;
     for (uint32_t i = threadIdx.x; i < kCombineRows * kChunks; i += kCombineThreads) {
         const uint32_t ro = i / kChunks, ch = i % kChunks;
         if (row0 + ro >= b.rows) break;
@@ -1181,7 +1190,7 @@ cudaError_t paged_tm_init(void) {
     return cudaSuccess;
 }
 
-size_t paged_tm_part_bytes(int sms) { return (size_t)6 * sms * Tm<128, 2>::kRecord * sizeof(float) + (size_t)sms * sizeof(PagedTmBlock); }
+size_t paged_tm_part_bytes(int sms) { return (size_t)6 * sms * Tm<128, 2>::kRecord * sizeof(float) + (size_t)sms * (sizeof(PagedTmBlock) + 2 * sizeof(uint32_t)); }
 
 cudaError_t launch_paged_tm(PagedAttnArgs a, const void *k, const void *v, uint32_t head_dim, int sms, cudaStream_t stream) {
     const uint64_t rows = (uint64_t)a.n_pages * a.n_kv << a.page_shift;

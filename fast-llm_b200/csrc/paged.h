@@ -29,7 +29,7 @@ struct PagedAttnArgs {
     float2 *lse;                    // optional
     const int32_t *table, *q_start, *kv_len;
     float *part, *part_tm;          // records
-    PagedTmBlock *blocks;           // one per CTA
+    PagedTmBlock *blocks;           // one per CTA, then two words each: its records that are complete
     uint32_t *tickets;              // zero between launches (attn_paged.cu)
     uint32_t *status;
     uint64_t q_stride, out_stride;  // elements between tokens

@@ -68,6 +68,9 @@ FLB_HD Shares tm_shares(uint32_t units, uint32_t ctas) { return shares_of(units,
 FLB_HD uint32_t tile_at_unit(uint32_t at, uint32_t front, uint32_t tiles, uint32_t tile_units) {
     return at > front ? lesser(tiles, (at - front + tile_units - 1) >> (tile_units - 1)) : 0u;   // (1 or 2)
 }
+// The record of a block's CTA `first + i` is its second (slot 1) where the block begins behind another one's tiles, which only the first CTA's can; every CTA
+// notes which of its two it left: left[2 cta + slot].
+FLB_HD uint32_t record_index(uint32_t first, uint32_t i, uint32_t slot) { return 2 * (first + i) + (i ? 0u : slot); }
 
 // ---- pages ----------------------------------------------------------------------------------------------------------
 // The pool in groups of 8 rows: where the group of row `row` of a page over KV head hkv lies. Pages outside the pool (and keys behind the last):

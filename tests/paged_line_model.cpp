@@ -85,6 +85,7 @@ static int tm(Rng &g) {
         }
         const Shares sh = tm_shares(base.back(), ctas);
         CHECK(base.back() < 2 || (sh.n >= 1 && share_lo(sh, sh.n) == base.back()));
+        std::vector<bool> used(2 * sh.n, false);
         for (uint32_t i = 0; i < n_block && sh.n; ++i) {
             const uint32_t f = base[i] + front, c0 = owner_of(sh, f), c1 = owner_of(sh, f + (tiles[i] - 1) * per[i]);
             uint32_t next = 0;
@@ -96,6 +97,17 @@ static int tm(Rng &g) {
                 if (t0 < t1 && t0) CHECK(share_lo(sh, c) > f);
             }
             CHECK(next == tiles[i]);
+            // its records are each in a place of their own, where the CTA has it: the first of its pieces, or one behind
+            for (uint32_t c = c0; c <= c1 && c1 > c0; ++c) {
+                bool in_front = false;   // tiles of a block in front of this one
+                for (uint32_t j = 0; j < i; ++j) {
+                    const uint32_t fj = base[j] + front;
+                    in_front |= tile_at_unit(share_lo(sh, c), fj, tiles[j], per[j]) < tile_at_unit(share_lo(sh, c + 1), fj, tiles[j], per[j]);
+                }
+                const uint32_t at = record_index(c0, c - c0, c == c0 && in_front);
+                CHECK(at == 2 * c + in_front && (c == c0 || !in_front) && at < 2 * sh.n && !used[at]);
+                used[at] = true;
+            }
         }
     }
     return 0;
