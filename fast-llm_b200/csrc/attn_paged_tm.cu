@@ -518,6 +518,12 @@ __device__ __forceinline__ bool partly(const PagedAttnArgs &a, const Piece &p, u
 }
 
 __device__ __forceinline__ void bar_both() { asm volatile("bar.sync 1, 256;" ::: "memory"); }   // the softmax warps
+// The same, and whether any of their threads says yes: what all of them then go by, whatever another role still writes.
+__device__ __forceinline__ bool bar_both_any(bool yes) {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(r) : "r"((uint32_t)yes) : "memory");
+    return r != 0;
+}
 __device__ __forceinline__ bool given_up(const Head &hd) { return *static_cast<const volatile uint32_t *>(&hd.abort_flag) != 0; }
 
 // The rows of q of a piece to L2 (a warp).
@@ -1100,9 +1106,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
             if (Parts == 1 && active && steps > kOutHalf && !dead) halves_back<D>(a, to, steps, ref);
             finish<D, Parts>(a, hd, q_s, Sums{ref, sum, highest, acc_ref, out_of}, steps != 0 && !dead, tmem);
             fence_before();
-            bar_both();   // both lanes are done with q, O and the notes
+            // both lanes are done with q, O and the notes (once a wait has run out the value warp may still be at them: the flag is read once)
+            const bool notes = bar_both_any(*static_cast<volatile uint32_t *>(&hd.any_unfinite) != 0);
             if (tid == 0 && !job.whole && !given_up(hd)) records_left(a)[2 * blockIdx.x + job.slot] = 1;
-            if (hd.any_unfinite) {
+            if (notes) {
                 for (uint32_t i = tid; i < 3 * D; i += 256) hd.unfinite[i] = 0x7fffffffu;
                 bar_both();
                 if (tid == 0) hd.any_unfinite = 0;
