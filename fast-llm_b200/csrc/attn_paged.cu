@@ -33,9 +33,9 @@ constexpr uint32_t kRowsB = kFewRows, kTile = 64, kStages = 3, kWarps = 4, kThre
 constexpr float kShift = 12.f;   // probabilities are 2^(x - m + 12): their lo parts stay normal f16 numbers down to 2^-14 of the largest, below it are held to 2^-37 of that
 
 // Rows of a sequence over one KV head, 0 where it is the other kernel's; its tiles: at least one, so that somebody writes its rows.
-__device__ __forceinline__ uint32_t rows_of(const PagedAttnArgs &a, const PagedSeq &q) { return q.n * a.group > a.few_rows ? 0u : q.n * a.group; }
+__device__ __forceinline__ uint32_t rows_of(const PagedAttnArgs &a, uint32_t few, const PagedSeq &q) { return q.n * a.group > few ? 0u : q.n * a.group; }
 __device__ __forceinline__ uint32_t tiles_of(const PagedSeq &q) { return max(1u, ((uint32_t)max(0, q.past + (int32_t)q.n) + kTile - 1) / kTile); }
-__device__ __forceinline__ uint64_t units_of(const PagedAttnArgs &a, const PagedSeq &q) { return rows_of(a, q) ? (uint64_t)tiles_of(q) * a.n_kv : 0u; }
+__device__ __forceinline__ uint64_t units_of(const PagedAttnArgs &a, uint32_t few, const PagedSeq &q) { return rows_of(a, few, q) ? (uint64_t)tiles_of(q) * a.n_kv : 0u; }
 
 // The pieces of a CTA's share: consecutive tiles of one sequence over one KV head.
 struct Piece {
@@ -44,7 +44,7 @@ struct Piece {
     int32_t keys;
     uint32_t base;                                 // unit of its tile 0
 };
-struct Walk { uint32_t pos, hi; };                 // the share's units behind the piece
+struct Walk { uint32_t pos, hi, few; };            // the share's units behind the piece; see few_limit
 // Tiles of the piece that begins at w.pos, over KV head p.hkv of the sequence in p.
 __device__ __forceinline__ void cut_piece(Walk &w, Piece &p) {
     p.t0 = w.pos - p.base;
@@ -58,7 +58,7 @@ __device__ __forceinline__ bool next_piece(const PagedAttnArgs &a, Walk &w, Piec
     if (++p.hkv == a.n_kv) {
         bool bad;
         p.hkv = 0;
-        do { p.q = paged_seq(a, ++p.seq, bad); } while ((p.rows = rows_of(a, p.q)) == 0);
+        do { p.q = paged_seq(a, ++p.seq, bad); } while ((p.rows = rows_of(a, w.few, p.q)) == 0);
         p.tiles = tiles_of(p.q);
         p.keys = max(0, p.q.past + (int32_t)p.q.n);
     }
@@ -394,7 +394,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
     if (a.n_seq <= 32) {
         bool bad = false;
         const PagedSeq q = lane < a.n_seq ? paged_seq(a, lane, bad) : PagedSeq{0, 0, 0};
-        const uint64_t mine = units_of(a, q);
+        walk.few = few_limit(a, q);
+        const uint64_t mine = units_of(a, walk.few, q);
         bad |= mine >> 26 != 0;   // (32 of them stay below 2^32; 2^26 tiles are 2^32 keys)
         const uint32_t u = mine >> 26 ? 0u : (uint32_t)mine;
         uint32_t x = u;
@@ -427,7 +428,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
         uint64_t mine = 0;
         bool bad = false, any_bad = false;
         for (uint32_t s = s0; s < s1; ++s) {
-            mine += units_of(a, paged_seq(a, s, bad));
+            mine += units_of(a, kFewRows, paged_seq(a, s, bad));
             any_bad |= bad;
         }
         uint64_t x = mine, total = 0;
@@ -446,11 +447,11 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
         x -= mine;
         sh = few_shares(total >> 32 ? 0u : (uint32_t)total, gridDim.x);
         if (blockIdx.x >= sh.n) return;
-        walk = Walk{share_lo(sh, blockIdx.x), share_lo(sh, blockIdx.x + 1)};
+        walk = Walk{share_lo(sh, blockIdx.x), share_lo(sh, blockIdx.x + 1), kFewRows};
         if (walk.pos >= x && walk.pos < x + mine) {
             uint32_t s = s0;
             for (;; ++s) {
-                const uint64_t u = units_of(a, paged_seq(a, s, bad));
+                const uint64_t u = units_of(a, kFewRows, paged_seq(a, s, bad));
                 if (walk.pos < x + u) break;
                 x += u;
             }
@@ -462,7 +463,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const __grid_con
         p.base = sm.start_off;
         p.q = paged_seq(a, p.seq, bad);
     }
-    p.rows = rows_of(a, p.q);
+    p.rows = rows_of(a, walk.few, p.q);
     p.tiles = tiles_of(p.q);
     p.keys = max(0, p.q.past + (int32_t)p.q.n);
     p.hkv = (walk.pos - p.base) / p.tiles;

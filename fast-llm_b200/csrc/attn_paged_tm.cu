@@ -56,7 +56,7 @@ struct Job {
     uint32_t whole, slot;               // the block is this CTA's alone; its record's
     int32_t past;
 };
-struct Walk { uint32_t pos, hi; };   // the share's units behind the piece
+struct Walk { uint32_t pos, hi, few; };   // the share's units behind the piece; see few_limit
 struct Block { uint32_t rows, tiles, units; int32_t keys; };
 struct Piece {
     PagedSeq q;
@@ -419,13 +419,13 @@ __device__ __forceinline__ Block block_of(const PagedAttnArgs &a, const PagedSeq
     b.units = kStart + b.tiles * tile_units(b.rows);
     return b;
 }
-__device__ __forceinline__ uint32_t blocks_of(const PagedAttnArgs &a, const PagedSeq &q) {   // of this kernel: sequences of more than few_rows rows
+__device__ __forceinline__ uint32_t blocks_of(const PagedAttnArgs &a, uint32_t few, const PagedSeq &q) {   // of this kernel: sequences of more than `few` rows
     const uint32_t rows = q.n * a.group;
-    return rows > a.few_rows ? (rows + 2 * kRowsL - 1) / (2 * kRowsL) : 0u;
+    return rows > few ? (rows + 2 * kRowsL - 1) / (2 * kRowsL) : 0u;
 }
 // Tiles of every lane's sequence over one KV head; long ones are summed by the whole warp.
-__device__ __forceinline__ uint64_t head_units(const PagedAttnArgs &a, const PagedSeq &q, uint32_t lane) {
-    const uint32_t n = blocks_of(a, q);
+__device__ __forceinline__ uint64_t head_units(const PagedAttnArgs &a, uint32_t few, const PagedSeq &q, uint32_t lane) {
+    const uint32_t n = blocks_of(a, few, q);
     uint64_t u = 0;
     if (n <= 4)
         for (uint32_t b = 0; b < n; ++b) u += block_of(a, q, b).units;
@@ -459,7 +459,7 @@ __device__ __forceinline__ uint32_t owner_of_tile(const Shares &sh, const Piece 
 // the share has tiles of it.
 __device__ __forceinline__ bool first_piece(const PagedAttnArgs &a, Walk &w, Piece &p) {
     const uint32_t lane = threadIdx.x & 31u;
-    p.n_blk = blocks_of(a, p.q);
+    p.n_blk = blocks_of(a, w.few, p.q);
     uint32_t per_head = 0;
     for (uint32_t b = lane; b < p.n_blk; b += 32) per_head += block_of(a, p.q, b).units;
     per_head = __reduce_add_sync(0xffffffffu, per_head);
@@ -495,7 +495,7 @@ __device__ __forceinline__ bool next_piece(const PagedAttnArgs &a, Walk &w, Piec
             if (++p.hkv == a.n_kv) {
                 bool bad;
                 p.hkv = 0;
-                do { p.q = paged_seq(a, ++p.seq, bad); } while ((p.n_blk = blocks_of(a, p.q)) == 0);
+                do { p.q = paged_seq(a, ++p.seq, bad); } while ((p.n_blk = blocks_of(a, w.few, p.q)) == 0);
             }
         }
         p.b = block_of(a, p.q, p.blk);
@@ -663,7 +663,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
     bool bad = false;
     if (a.n_seq <= 32) {
         const PagedSeq q = lane < a.n_seq ? paged_seq(a, lane, bad) : PagedSeq{0, 0, 0};
-        const uint64_t mine = head_units(a, q, lane) * a.n_kv;
+        const uint32_t few = few_limit(a, q);
+        const uint64_t mine = head_units(a, few, q, lane) * a.n_kv;
         const bool fits = __reduce_add_sync(0xffffffffu, (uint32_t)min(mine >> 16, (uint64_t)0x10000u) + 1u) <= 0x10000u;   // (then all of them stay below 2^32)
         bad |= !fits;
         const uint32_t u = fits ? (uint32_t)mine : 0u;
@@ -675,7 +676,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
         }
         if (bad && blockIdx.x == 0) atomicCAS(a.status, ST_OK, ST_PAGED_ARGS);
         sh = tm_shares(__shfl_sync(0xffffffffu, x, 31), gridDim.x);
-        walk = Walk{share_lo(sh, blockIdx.x), share_lo(sh, blockIdx.x + 1)};
+        walk = Walk{share_lo(sh, blockIdx.x), share_lo(sh, blockIdx.x + 1), few};
         const uint32_t at = __ballot_sync(0xffffffffu, walk.pos < x);   // sequences that end behind the share's begin
         const int src = at ? __ffs(at) - 1 : 0;
         p.seq = src;
@@ -689,7 +690,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
             bool b = false;
             const PagedSeq q = s0 + tid < a.n_seq ? paged_seq(a, s0 + tid, b) : PagedSeq{0, 0, 0};
             bad |= b;
-            mine += head_units(a, q, lane) * a.n_kv;
+            mine += head_units(a, kFewRows, q, lane) * a.n_kv;   // (more than 32 sequences: each by its rows)
         }
 #pragma unroll
         for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
@@ -698,11 +699,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
         for (uint32_t w = 0; w < kThreads / 32; ++w) total += hd.sum[w];
         if ((bad || total >> 32) && blockIdx.x == 0) atomicCAS(a.status, ST_OK, ST_PAGED_ARGS);
         sh = tm_shares(total >> 32 ? 0u : (uint32_t)total, gridDim.x);
-        walk = Walk{share_lo(sh, blockIdx.x), share_lo(sh, blockIdx.x + 1)};
+        walk = Walk{share_lo(sh, blockIdx.x), share_lo(sh, blockIdx.x + 1), kFewRows};
         uint64_t run = 0;
         for (uint32_t s0 = 0; s0 < a.n_seq && blockIdx.x < sh.n && run <= walk.pos; s0 += kThreads) {
             const PagedSeq q = s0 + tid < a.n_seq ? paged_seq(a, s0 + tid, bad) : PagedSeq{0, 0, 0};
-            const uint64_t u = head_units(a, q, lane) * a.n_kv;
+            const uint64_t u = head_units(a, kFewRows, q, lane) * a.n_kv;
             uint64_t x = u;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {

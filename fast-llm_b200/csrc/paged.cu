@@ -435,11 +435,9 @@ int fl_b200_paged_attn(fl_b200_ctx *c, const fl_b200_paged_cache *cache, int act
     a.scale = scale;
     a.part_tm = c->paged_part + paged_few_part_bytes(c->sms) / sizeof(float);
     const bool many = (uint64_t)max_new * a.group > kFewRows;
-    // Few sequences: the second kernel takes all of them, single tokens too, instead of a launch for each kind. us both ways (8 KV heads unless
-    // said): 6 sequences of up to 100 keys, a quarter of them 16 tokens 33 -> 23; 4 x 8 tokens over 4096 keys 55 -> 52; 8 over 6000 keys, 4 KV
-    // heads, a quarter 777 tokens 155 -> 146; 16 over 4000 keys, a quarter 500 tokens 298 -> 322, since a piece's start and end cost it more.
-    a.few_rows = many && 2ull * n_seq * n_kv <= (uint32_t)c->sms ? 0 : kFewRows;
-    if (a.few_rows)
+    a.spare = !many ? 0 : a.half && dim == 128 ? kSpareHalf128 : kSpare;
+    if (many && n_seq <= 32 && (uint64_t)n_seq * n_kv * (((uint64_t)max_blocks << shift) / 128 + kSpareStart) <= kSpareNoLaunch) a.spare = kSpareAll;
+    if (a.spare != kSpareAll)
         if (int rc = cuda_err(launch_paged_few(a, cache->k_dev, cache->v_dev, dim, c->sms, c->stream), "paged_attn launch")) return rc;
     return many ? cuda_err(launch_paged_tm(a, cache->k_dev, cache->v_dev, dim, c->sms, c->stream), "paged_attn launch") : FL_B200_OK;
 }

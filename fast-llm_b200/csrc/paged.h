@@ -33,16 +33,25 @@ struct PagedAttnArgs {
     uint32_t *tickets;              // zero between launches (attn_paged.cu)
     uint32_t *status;
     uint64_t q_stride, out_stride;  // elements between tokens
+    uint32_t spare;                 // see few_limit; 0: no sequence can have many rows
     uint32_t n_seq, max_blocks, n_tokens, max_new, n_pages, page_shift;
     uint32_t n_kv, group, half;     // half: activations are f16
-    uint32_t few_rows;              // sequences of at most so many rows over a KV head are the first kernel's, the others the second's
     float scale;
 };
 
-// Sequences of few rows over a KV head (mma.sync: attn_paged.cu) and of many (tcgen05: attn_paged_tm.cu). kmap and vmap are filled in there. us of
-// both at 4 x 65000, 32 x 4000 and 1 x 8000 keys, 8 KV heads: 4 rows 150, 76, 15 and 212, 136, 34 (f16: 158, 92, 29); 16 rows 165, 92, 27 and
-// 215, 137, 34 (f16: 158, 92, 29).
+// Sequences of few rows over a KV head (mma.sync: attn_paged.cu) and of many (tcgen05: attn_paged_tm.cu). kmap and vmap are filled in there. 16 is what
+// the first kernel's instances hold. us of both at 4 x 65000, 32 x 4000 and 1 x 8000 keys, 8 KV heads of 128, pages of 16: 4 rows 166, 91, 17 and 243, 197, 40 (f16 166,
+// 89, 16 and 187, 143, 32); 16 rows 200, 150, 29 and 257, 181, 34 (f16 200, 126, 29 and 188, 134, 30).
 constexpr uint32_t kFewRows = 16;
+// Up to 32 sequences, of few rows and of many: the second kernel takes all of them where those of few rows are less work than a launch of their own
+// in front of it, in tiles of 128 keys; a sequence's start and end over a KV head count as 60. us with two launches and with one, 8 KV heads of 128 dimensions, single
+// tokens over so many keys: f32, beside 500 tokens over 4000 keys 8 x 4000 133 and 122, 12 x 4000 144 and 138, 16 x 4000 151 and 149, 1 x 65000 161 and 143, 2 x 65000 196
+// and 202; beside 30 over 1000 12 x 2000 49 and 61; beside 200 over 500 28 x 300 40 and 65. f16, whose tiles take the second kernel half as long: 8 x 4000 100 and 85, 16 x
+// 4000 118 and 107, 2 x 65000 162 and 148, 12 x 2000 44 and 45, 28 x 300 37 and 45; f16 and heads of 64: 8 x 4000 74 and 72, 16 x 4000 87 and 96.
+constexpr uint32_t kSpareStart = 60, kSpare = 6500, kSpareHalf128 = 12000;
+// Where the table's width bounds that work by as much as this the first kernel is not launched (4 x 8 tokens over 4096 keys 39.6 us, 36 without). The price: single
+// tokens in a call that allows more, as a recorded one may, run on the second kernel (1 x 8000 keys 24 us, 31 so; 4 x 1000 18, 24).
+constexpr uint32_t kSpareNoLaunch = 4000, kSpareAll = 0xffffffffu;
 cudaError_t paged_few_init(void);
 size_t paged_few_part_bytes(int sms);
 cudaError_t launch_paged_few(PagedAttnArgs a, const void *k, const void *v, uint32_t head_dim, int sms, cudaStream_t stream);
@@ -60,6 +69,16 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedAttnArgs &a, uint32_t s
     bad = b < 0 || e < b || (uint32_t)e > a.n_tokens || (uint32_t)(e - b) > a.max_new || len < 0 || (uint64_t)len > room;
     return bad ? PagedSeq{0, 0, 0} : PagedSeq{(uint32_t)b, (uint32_t)(e - b), len - (e - b)};
 }
+// The rows that a sequence of the first kernel has at most (lane i holds sequence i, of up to 32): none where the second one has others to work on and
+// takes those too.
+__device__ __forceinline__ uint32_t few_limit(const PagedAttnArgs &a, const PagedSeq &q) {
+    if (a.spare == 0 || a.spare == kSpareAll) return a.spare ? 0u : kFewRows;
+    const uint32_t rows = q.n * a.group, tiles = ((uint32_t)max(0, q.past + (int32_t)q.n) + 127) / 128;
+    const uint32_t cost = rows && rows <= kFewRows ? min(min(tiles + kSpareStart, 1u << 16) * a.n_kv, 1u << 24) : 0u;   // (32 of them below 2^32)
+    const uint32_t all = __reduce_add_sync(0xffffffffu, cost);
+    return __any_sync(0xffffffffu, rows > kFewRows) && all <= a.spare ? 0u : kFewRows;
+}
+
 // Values of +inf, -inf and NaN (class 0, 1, 2) among the keys that only part of the rows attend: per class and dimension the
 // first such key. A row that attends keys 0 .. lim is affected by those <= lim.
 __device__ __forceinline__ float unfinite_of(const uint32_t *u, uint32_t dims, uint32_t d, int32_t lim) {

@@ -835,3 +835,26 @@ def test_plan_without_tokens(ctx):
     got = run_plan(ctx, [40, 17], [0, 5], [0, 0], [[0, 1, 2], [3, 4, -1]], [-1] * 5, 0, 16, 0)
     assert ctx.status() == 0
     assert got == dict(table=[[0, 1, 2], [3, 4, -1]], free=[0, 1, 2, 4, -1], count=4, pos=[], slot=[], start=[0, 0, 0], length=[0, 5])
+
+
+@pytest.mark.parametrize("act,dim", [("f32", 128), ("f16", 128), ("f16", 64)])
+@pytest.mark.parametrize("seqs,wide,max_new", [
+    ([(700, 1)] * 2 + [(500, 30)], 0, None),                     # the table's width bounds the single tokens' work: one kernel takes all
+    ([(700, 1)] * 2 + [(500, 30), (90, 90)], 4000, None),        # it does not, but the lengths are short: the same, after the other one looked at them
+    ([(9000, 1), (8000, 2)] * 6 + [(500, 30)], 0, None),         # each by its rows
+    ([(900, 1)] * 3 + [(900, 4)], 4000, 200),                    # a call that allows chunks and has none
+    ([(900, 1)] * 3 + [(900, 4)], 0, 200),                       # the same under a narrow table
+    ([(700, 1)] * 40 + [(500, 30), (64, 5)], 0, None)])          # more than 32 sequences
+def test_sequences_of_few_rows_beside_chunks(ctx, seqs, wide, max_new, act, dim):
+    n_q, n_kv, page = 16, 4, 16
+    c = make(len(seqs) + wide, seqs, n_q, n_kv, dim, page, act)
+    if wide:
+        c["table"] = torch.cat([c["table"], torch.full((len(seqs), wide), -7, dtype=torch.int32, device="cuda")], 1).contiguous()
+    if max_new:
+        more = max_new + 2 - c["q"].shape[0]                     # (n_tokens bounds max_new)
+        c["q"] = torch.cat([c["q"], c["q"].new_zeros((more, n_q * dim))])
+        c["out_all"] = torch.full((max_new + 2, n_q * dim + 8), CANARY, device="cuda", dtype=DT[act])
+        c["out"] = c["out_all"][:, :n_q * dim]
+        c["lse"] = torch.full((max_new + 2, n_q, 2), CANARY, device="cuda")
+    attn(ctx, c, n_q, n_kv, dim, page, 1.0 / math.sqrt(dim), max_new=max_new)
+    check(ctx, c, seqs, n_q, n_kv, dim, 1.0 / math.sqrt(dim), act)
