@@ -3,6 +3,10 @@
 Per step ``plan`` (block tables, slots and positions from the lengths, on the device), per layer ``PagedCache.append`` and
 ``PagedCache.attn``. Arguments are torch CUDA tensors, checked here for type, shape and device; strides between tokens
 are taken from the tensors, so that q, k and v can be slices of one projection's output.
+
+Calls run on the context's stream (``Context.stream``), as everywhere in this library, whatever torch's current stream is. It waits for
+torch's default stream and the other way round; work on any other torch stream has to be ordered with it by the caller, by running it
+there (``torch.cuda.stream(torch.cuda.ExternalStream(ctx.stream()))``), by events or by ``ctx.sync()``.
 """
 import ctypes as C
 
@@ -45,17 +49,25 @@ def _ints(dev, name, t, n):
     return t.data_ptr()
 
 
+def _fits(name, value):
+    """value, which ctypes would cut to 32 bits."""
+    if not 0 <= value < 1 << 32:
+        raise ValueError("%s: %d is not a 32-bit size" % (name, value))
+    return value
+
+
 def _rows(dev, name, t, dtype, n, width):
     """(pointer, stride) of a 2-D tensor of n tokens whose rows are packed."""
     if t.dtype is not dtype or t.size() != (n, width) or t.get_device() != dev or t.stride(1) != 1:
         raise ValueError("%s: %s activations [%d][%d], packed rows, on device %d are wanted, got %s %s on %s"
                          % (name, dtype, n, width, dev, t.dtype, tuple(t.shape), t.device))
-    return t.data_ptr(), t.stride(0) if n > 1 else width
+    return t.data_ptr(), _fits(name + "'s stride", t.stride(0)) if n > 1 else width
 
 
 def plan(ctx, held, past, new, table, free_list, free_count_in, free_count_out, q_start, kv_len, pos, slot, page_size):
     """fl_b200_paged_plan; table [n_seq][max_blocks], free_list [n_pages], pos and slot [max_tokens]."""
     n_seq, blocks, n_pages, n_tok, dev = held.numel(), table.size(-1), free_list.numel(), pos.numel(), ctx.device
+    _fits("page_size", page_size)
     capi._ck(_entry(ctx.lib, "fl_b200_paged_plan")(
         ctx._h, _ints(dev, "held", held, n_seq), _ints(dev, "past", past, n_seq), _ints(dev, "new", new, n_seq), n_seq, page_size,
         _ints(dev, "table", table, n_seq * blocks), blocks, _ints(dev, "free_list", free_list, n_pages), n_pages,
@@ -72,6 +84,8 @@ class PagedCache:
                     or t.get_device() != ctx.device:
                 raise ValueError("%s: a contiguous pool of %d f16 values on device %d is wanted, got %s %s on %s"
                                  % (name, n_pages * n_kv_head * page_size * head_dim, ctx.device, t.dtype, tuple(t.shape), t.device))
+        for name, value in (("n_pages", n_pages), ("page_size", page_size), ("n_kv_head", n_kv_head), ("head_dim", head_dim)):
+            _fits(name, value)
         self.ctx, self.k, self.v = ctx, k, v
         self.width = n_kv_head * head_dim
         self.cfg = PagedCacheP(k.data_ptr(), v.data_ptr(), n_pages, page_size, n_kv_head, head_dim)
@@ -82,6 +96,8 @@ class PagedCache:
         kp, ks = _rows(dev, "k", k, dtype, n, width)
         vp, vs = _rows(dev, "v", v, dtype, n, width)
         qp, qw, qs, op, os_ = None, 0, 0, None, 0
+        if (q is None) != (q_out is None):
+            raise ValueError("append: q and q_out, or neither")
         if q is not None:
             qw = q.size(-1)
             qp, qs = _rows(dev, "q", q, dtype, n, qw)
@@ -90,7 +106,7 @@ class PagedCache:
             raise ValueError("append: f32 or f16 activations of whole heads, k and v of one stride")
         capi._ck(_entry(ctx.lib, "fl_b200_paged_append")(
             ctx._h, self.cfg, _ACT[dtype], qp, qw // dim, qs, kp, vp, ks, _ints(dev, "pos", pos, n), _ints(dev, "slot", slot, n), n,
-            dim if n_rot is None else n_rot, freq_base, op, os_))
+            dim if n_rot is None else _fits("n_rot", n_rot), freq_base, op, os_))
 
     def attn(self, q, table, q_start, kv_len, max_new, scale, out, lse=None):
         """Causal attention of every sequence's new tokens; q, out [n_tokens][heads * head_dim], lse [n_tokens][heads][2] f32."""
@@ -104,5 +120,5 @@ class PagedCache:
             raise ValueError("lse: f32 [n_tokens][heads][2] on device %d" % dev)
         capi._ck(_entry(ctx.lib, "fl_b200_paged_attn")(
             ctx._h, self.cfg, _ACT[dtype], qp, qw // dim, qs, _ints(dev, "table", table, n_seq * blocks), blocks,
-            _ints(dev, "q_start", q_start, n_seq + 1), _ints(dev, "kv_len", kv_len, n_seq), n_seq, n, max_new, scale, op, os_,
+            _ints(dev, "q_start", q_start, n_seq + 1), _ints(dev, "kv_len", kv_len, n_seq), n_seq, n, _fits("max_new", max_new), scale, op, os_,
             None if lse is None else lse.data_ptr()))

@@ -248,8 +248,8 @@ int fl_b200_paged_append(fl_b200_ctx *ctx, const fl_b200_paged_cache *cache, int
  * the last of them; token i of n attends keys 0 .. kv_len - n + i. A token without a key gets zeros. n_q_head is a multiple of
  * n_kv_head (groups of up to 128), q and out [n_tokens][stride] as above, table [n_seq][max_blocks] (max_blocks * page_size <= 2^31 - 256), scale
  * positive. n_tokens: rows of q and out; max_new: the most new tokens that any sequence has. Sequences whose lengths break these bounds are left
- * out (status 4), and so are lines of together 2^32 or more tiles over all KV heads (a minute's work); rows of
- * out that belong to no sequence stay as they are, keys on a page outside the pool count as zero vectors (status 3). After a wait that ran out (status
+ * out (status 4), and so are lines of together 2^31 or more tiles of 256 rows by 128 keys over all KV heads (a minute's work; of few rows: a sequence of
+ * 2^26 tiles of 64 keys); rows of out that belong to no sequence stay as they are, keys on a page outside the pool count as zero vectors (status 3). After a wait that ran out (status
  * 1) rows may be left as they were, none is written in part. What a row does not attend may hold
  * anything; an infinity that it does attend may make it NaN. lse_out
  * (optional): per token and query head (max score, sum of exp(score - max)), (-inf, 0) without a key: what fl_b200_seqpar_combine merges.

@@ -95,3 +95,29 @@ def test_attn_refuses_tables_whose_last_tile_ends_past_31_bits(lib, page):
     change = dict(cache=cache(page=page), blocks=((1 << 31) - 256) // page + 1)
     assert call(lib, "fl_b200_paged_attn", dict(ATTN, **change).values()) == 1
     assert b"blocks" in lib.fl_b200_last_error()
+
+
+def test_python_sizes_past_32_bits():
+    """ctypes cuts what does not fit: a stride of 2^32 + 128 would become one of 128."""
+    from fast_llm_b200 import paged
+
+    class Ctx:
+        device, lib, _h = -1, None, None          # -1: where tensors without storage are
+    meta = lambda *shape: torch.empty(shape, dtype=torch.float16, device="meta")   # noqa: E731
+    wide = torch.empty_strided((2, 128), ((1 << 32) + 128, 1), dtype=torch.float32, device="meta")
+    with pytest.raises(ValueError, match="stride"):
+        paged._rows(-1, "q", wide, torch.float32, 2, 128)
+    with pytest.raises(ValueError, match="n_pages"):
+        paged.PagedCache(Ctx, meta(64, 128), meta(64, 128), -4, -16, 1, 128)
+    cache = paged.PagedCache(Ctx, meta(64, 128), meta(64, 128), 4, 16, 1, 128)
+    ints = lambda *shape: torch.empty(shape, dtype=torch.int32, device="meta")     # noqa: E731
+    q = meta(2, 128)
+    for most in ((1 << 32) + 1, -1):
+        with pytest.raises(ValueError, match="max_new"):
+            cache.attn(q, ints(1, 4), ints(2), ints(1), most, 0.1, q)
+    with pytest.raises(ValueError, match="n_rot"):
+        cache.append(q, q, q, ints(2), ints(2), q, freq_base=1e4, n_rot=(1 << 32) + 64)
+    with pytest.raises(ValueError, match="page_size"):
+        paged.plan(Ctx, ints(1), ints(1), ints(1), ints(1, 4), ints(4), ints(1), ints(1), ints(2), ints(1), ints(3), ints(3), page_size=(1 << 32) + 16)
+    with pytest.raises(ValueError, match="q_out"):
+        cache.append(q, q, q, ints(2), ints(2), None, freq_base=1e4)
