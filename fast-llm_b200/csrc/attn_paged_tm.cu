@@ -582,29 +582,40 @@ __device__ __noinline__ void finish(const PagedAttnArgs &a, Head &hd, uint8_t *q
         struct Part { uint32_t at; const float4 *mem; uint32_t out; float keep; };
         const Part part1{to, acc_mem, s.out_of, s.acc_ref == ref ? 1.f : exp2_fast(s.acc_ref - ref)};
         const Part part2{to + 128, acc_mem + T::kRecord / 4, out2, acc2_ref == ref2 ? 1.f : exp2_fast(acc2_ref - ref2)};
-        auto add_part = [&](const Part &p, int c, float w, float (&v)[16]) {   // v += w times the contexts of columns 16 c ..
+        // (the sums in memory of the next columns are on their way meanwhile: 4 x 8 tokens over 4096 keys 37.3 us, 35.7 so)
+        auto fetch = [&](const Part &p, int c, float4 (&x)[4]) {
+            const bool acc = Parts == 2 && c < D / 16 && (p.out >> (c / 2) & 1u);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = acc ? __ldcg(p.mem + (4 * c + j) * kRowsL) : make_float4(0.f, 0.f, 0.f, 0.f);
+        };
+        auto add_part = [&](const Part &p, int c, float w, const float4 (&old)[4], float (&v)[16]) {   // v += w times the contexts of columns 16 c ..
             float o[16];
             load16(p.at + 16 * c, o);
-            const bool acc = Parts == 2 && (p.out >> (c / 2) & 1u);
-            float4 old[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) old[j] = acc ? __ldcg(p.mem + (4 * c + j) * kRowsL) : make_float4(0.f, 0.f, 0.f, 0.f);
-            const float keep = w * p.keep;
             wait_ld(o);
 #pragma unroll
             for (int j = 0; j < 16; ++j) v[j] = fmaf(o[j], w, v[j]);
-            if (acc)
+            if (Parts == 2 && (p.out >> (c / 2) & 1u)) {
+                const float keep = w * p.keep;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     v[4 * j] = fmaf(old[j].x, keep, v[4 * j]); v[4 * j + 1] = fmaf(old[j].y, keep, v[4 * j + 1]);
                     v[4 * j + 2] = fmaf(old[j].z, keep, v[4 * j + 2]); v[4 * j + 3] = fmaf(old[j].w, keep, v[4 * j + 3]);
                 }
+            }
         };
+        float4 next1[4], next2[4];
+        fetch(part1, 0, next1);
+        fetch(part2, 0, next2);   // (nothing where there is no second part)
 #pragma unroll 1
         for (int c = 0; c < D / 16; ++c) {
             float v[16] = {};
-            add_part(part1, c, two ? w1 : 1.f, v);
-            if (two) add_part(part2, c, w2, v);
+            float4 old1[4], old2[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { old1[j] = next1[j]; old2[j] = next2[j]; }
+            fetch(part1, c + 1, next1);
+            fetch(part2, c + 1, next2);
+            add_part(part1, c, two ? w1 : 1.f, old1, v);
+            if (two) add_part(part2, c, w2, old2, v);
             if (any_unfinite)
 #pragma unroll 1
                 for (int j = 0; j < 16; ++j) {
@@ -1023,7 +1034,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
             uint32_t out_of = 0;                                               // bit c: columns 32 c .. have a sum in memory
             for (uint32_t step = 0; step < steps; ++step) {
                 const int32_t k0 = (int32_t)((t0 + (sm ? 2 * step + l : step)) * kTile);
-                if (Parts == 2 && active && step >= 2 && (step + 1 < steps || step == 3)) {   // (three tiles of a half at the end: they stay)
+                if (Parts == 2 && active && step >= 2) {
                     // half of O to its sum in memory, while the tensor cores form the scores
                     if (!wait(&hd.o_done[l], (s_seen - 1) & 1u)) break;
                     fence_after();
