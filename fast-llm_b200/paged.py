@@ -50,7 +50,7 @@ def _ints(dev, name, t, n):
 
 
 def _fits(name, value):
-    """value, which ctypes would cut to 32 bits."""
+    """value, which ctypes would cut to 32 bits. (Asked where value >> 32 is not 0.)"""
     if not 0 <= value < 1 << 32:
         raise ValueError("%s: %d is not a 32-bit size" % (name, value))
     return value
@@ -61,13 +61,19 @@ def _rows(dev, name, t, dtype, n, width):
     if t.dtype is not dtype or t.size() != (n, width) or t.get_device() != dev or t.stride(1) != 1:
         raise ValueError("%s: %s activations [%d][%d], packed rows, on device %d are wanted, got %s %s on %s"
                          % (name, dtype, n, width, dev, t.dtype, tuple(t.shape), t.device))
-    return t.data_ptr(), _fits(name + "'s stride", t.stride(0)) if n > 1 else width
+    if n < 2:
+        return t.data_ptr(), width
+    stride = t.stride(0)
+    if stride >> 32:
+        _fits(name + "'s stride", stride)
+    return t.data_ptr(), stride
 
 
 def plan(ctx, held, past, new, table, free_list, free_count_in, free_count_out, q_start, kv_len, pos, slot, page_size):
     """fl_b200_paged_plan; table [n_seq][max_blocks], free_list [n_pages], pos and slot [max_tokens]."""
     n_seq, blocks, n_pages, n_tok, dev = held.numel(), table.size(-1), free_list.numel(), pos.numel(), ctx.device
-    _fits("page_size", page_size)
+    if page_size >> 32:
+        _fits("page_size", page_size)
     capi._ck(_entry(ctx.lib, "fl_b200_paged_plan")(
         ctx._h, _ints(dev, "held", held, n_seq), _ints(dev, "past", past, n_seq), _ints(dev, "new", new, n_seq), n_seq, page_size,
         _ints(dev, "table", table, n_seq * blocks), blocks, _ints(dev, "free_list", free_list, n_pages), n_pages,
@@ -96,9 +102,13 @@ class PagedCache:
         kp, ks = _rows(dev, "k", k, dtype, n, width)
         vp, vs = _rows(dev, "v", v, dtype, n, width)
         qp, qw, qs, op, os_ = None, 0, 0, None, 0
-        if (q is None) != (q_out is None):
-            raise ValueError("append: q and q_out, or neither")
+        if n_rot is None:
+            n_rot = dim
+        elif n_rot >> 32:
+            _fits("n_rot", n_rot)
         if q is not None:
+            if q_out is None:
+                raise ValueError("append: q goes to q_out")
             qw = q.size(-1)
             qp, qs = _rows(dev, "q", q, dtype, n, qw)
             op, os_ = _rows(dev, "q_out", q_out, dtype, n, qw)
@@ -106,12 +116,14 @@ class PagedCache:
             raise ValueError("append: f32 or f16 activations of whole heads, k and v of one stride")
         capi._ck(_entry(ctx.lib, "fl_b200_paged_append")(
             ctx._h, self.cfg, _ACT[dtype], qp, qw // dim, qs, kp, vp, ks, _ints(dev, "pos", pos, n), _ints(dev, "slot", slot, n), n,
-            dim if n_rot is None else _fits("n_rot", n_rot), freq_base, op, os_))
+            n_rot, freq_base, op, os_))
 
     def attn(self, q, table, q_start, kv_len, max_new, scale, out, lse=None):
         """Causal attention of every sequence's new tokens; q, out [n_tokens][heads * head_dim], lse [n_tokens][heads][2] f32."""
         ctx, dim, n, qw, dtype, dev = self.ctx, self.cfg.head_dim, q.size(0), q.size(-1), q.dtype, self.ctx.device
         n_seq, blocks = kv_len.numel(), table.size(-1)
+        if max_new >> 32:
+            _fits("max_new", max_new)
         qp, qs = _rows(dev, "q", q, dtype, n, qw)
         op, os_ = _rows(dev, "out", out, dtype, n, qw)
         if dtype not in _ACT or qw % dim:
@@ -120,5 +132,5 @@ class PagedCache:
             raise ValueError("lse: f32 [n_tokens][heads][2] on device %d" % dev)
         capi._ck(_entry(ctx.lib, "fl_b200_paged_attn")(
             ctx._h, self.cfg, _ACT[dtype], qp, qw // dim, qs, _ints(dev, "table", table, n_seq * blocks), blocks,
-            _ints(dev, "q_start", q_start, n_seq + 1), _ints(dev, "kv_len", kv_len, n_seq), n_seq, n, _fits("max_new", max_new), scale, op, os_,
+            _ints(dev, "q_start", q_start, n_seq + 1), _ints(dev, "kv_len", kv_len, n_seq), n_seq, n, max_new, scale, op, os_,
             None if lse is None else lse.data_ptr()))
