@@ -30,7 +30,8 @@ namespace flb {
 namespace {
 
 constexpr uint32_t kRowsB = kFewRows, kTile = 64, kStages = 3, kWarps = 4, kThreads = (kWarps + 1) * 32;
-constexpr float kShift = 12.f;   // probabilities are 2^(x - m + 12): their lo parts stay normal f16 numbers down to 2^-14 of the largest, below it are held to 2^-37 of that
+// Probabilities are 2^(x - m + 12): their lo parts stay normal f16 numbers down to 2^-14 of the largest, below it are held to 2^-37 of that
+constexpr float kShift = 12.f;
 
 // Rows of a sequence over one KV head, 0 where it is the other kernel's; its tiles: at least one, so that somebody writes its rows.
 __device__ __forceinline__ uint32_t rows_of(const PagedAttnArgs &a, uint32_t few, const PagedSeq &q) { return q.n * a.group > few ? 0u : q.n * a.group; }
@@ -167,10 +168,10 @@ __device__ __forceinline__ void copy_tiles(const PagedAttnArgs &a, FewSmem<D> &s
         for (uint32_t i = issued - min(issued, kStages); i < issued; ++i) mbar_wait_bounded(&sm.full[i % kStages], i / kStages & 1u, a.status);
 }
 
-// The records of a sequence over one KV head, added in order: of CTA c0 the one of the tiles that begin in its share, of the others the one of
-// tiles that began before. This is the launch's tail: its time is round trips to L2, so that as many records as the ring holds, which is free by then, are
-// copied into it at once; then their weights, 8 lanes a row, then the contexts. Run once, so out of line. (16 rows, 42 records: 11 us;
-// loads into registers, 8 at a time, 20.)
+// The records of a sequence over one KV head, added in order: of CTA c0 the one of the tiles that begin in its share, of the others the one
+// of tiles that began before. This is the launch's tail: its time is round trips to L2, so that as many records as the ring holds, which is
+// free by then, are copied into it at once; then their weights, 8 lanes a row, then the contexts. Run once, so out of line. (16 rows, 42
+// records: 11 us; loads into registers, 8 at a time, 20.)
 template <int D, int B>
 __device__ __noinline__ void combine(const PagedAttnArgs &a, FewSmem<D> &sm, const Late late) {
     constexpr uint32_t kRecord = kRowsB * (D + 4), kChunks = D / 4, kThr = kWarps * 32, kItems = 4 * B * kChunks <= kThr ? 1 : 4 * B * kChunks / kThr;

@@ -5,10 +5,11 @@
 // that a pair of row and key costs 8 D tensor flops instead of 4 D, and nothing else is rounded below 32 bits (small probabilities: see kShift). f16
 // activations (Parts = 1): q as it is, the probabilities as one f16 (half a step of 2^-11, as the result).
 //
-// Bound by the chain scores - softmax - context of each lane. A tile of 128 keys and 256 rows, head_dim 128: 4300 cycles for f16 activations, 7000
-// for f32; the tensor pipe is busy for 2350 and 4700 of them (77 cycles an instruction for scores, both operands in shared memory, 70 for
-// contexts), the exponentials take 2048 of the special functions. Measured (32/8 heads): 2048 tokens over 30000 keys, f16, 964 us in a burst (1.08 PFLOP/s), 1122
-// under the power cap; 4096 tokens, f32, 334 us (0.82 PFLOP/s of tensor work); 4 x 8 tokens over 4096 keys 35 us. Roles of a CTA (11 warps, one CTA per SM):
+// Bound by the chain scores - softmax - context of each lane. A tile of 128 keys and 256 rows, head_dim 128: about 3900 cycles for f16
+// activations, 7600 for f32 (ncu's cycles of 2048 tokens over 30000 keys and of 4096 tokens, a block's start and end counted as six tiles); the
+// tensor pipe is busy for 2100 and 4200 of them (53 and 40 % of the launches), the exponentials and conversions for 55 % of the first. Measured
+// (32/8 heads, device times): 2048 tokens over 30000 keys, f16, 990 us in a burst (1.05 PFLOP/s), 1160 under the power cap; 4096 tokens, f32, 343
+// us (0.80 PFLOP/s of tensor work); 4 x 8 tokens over 4096 keys 35.6 us. Roles of a CTA (11 warps, one CTA per SM):
 //   softmax (2 x 4 warps): "lane" l = its 128 rows, thread = row: scores out of tensor memory, maximum, exponentials, probabilities
 //                          back over the scores' columns; at the end of a piece the contexts out
 //   copy    (1 warp)     : K and V tiles into a ring of slots, one TMA box per page (attn_paged.cu)
@@ -225,8 +226,9 @@ __device__ __forceinline__ void scale_o(uint32_t at, uint32_t columns, float by)
     }
 }
 // f16 activations: a half of the contexts goes out at steps n kOutHalf and n kOutHalf + 1, and comes back at the piece's end. What went out
-// follows from the step, and the reference of the sums lies beside them, so that the loop over the tiles holds nothing of it. (us at 4096 tokens with heads of 64, and at 2048 tokens over 30000 keys:
-// without 152, 970; this 157, 990; as a call of its own in the loop, every 64th tile, 167, 1010.)
+// follows from the step, and the reference of the sums lies beside them, so that the loop over the tiles holds nothing of it. (us at 4096
+// tokens with heads of 64, and at 2048 tokens over 30000 keys: without 152, 970; this 157, 990; as a call of its own in the loop, every
+// 64th tile, 167, 1010.)
 constexpr uint32_t kOutHalf = 128;
 __device__ __forceinline__ bool half_goes(uint32_t step) { return step >= kOutHalf && step % kOutHalf < 2; }
 template <int D> __device__ __forceinline__ uint32_t halves_out(uint32_t steps) {   // in front of step `steps`: bit c: columns 32 c ..
@@ -236,8 +238,8 @@ template <int D> __device__ __forceinline__ uint32_t halves_out(uint32_t steps) 
 template <int D> __device__ __forceinline__ float *half_sums(const PagedAttnArgs &a) {   // of the warp's lane: [D / 4][128 rows][4], a row each, references
     return a.part_tm + ((uint64_t)gridDim.x * 4 + blockIdx.x * 2 + (threadIdx.x >> 7)) * Tm<D, 1>::kRecord;
 }
-// The row's contexts times `by`, where that changes its reference to ref. (Out of line, as load_q and finish are: what they need in registers stays out
-// of the loop over the tiles.)
+// The row's contexts times `by`, where that changes its reference to ref. (Out of line, as load_q and finish are: what they need in
+// registers stays out of the loop over the tiles.)
 template <int D, int Parts> __device__ __noinline__ void change_o(const PagedAttnArgs &a, uint32_t to, float by, uint32_t step, float ref) {
     if (__any_sync(0xffffffffu, by != 1.f)) scale_o(to, D, by);
     if (Parts == 2 || !half_goes(step)) return;
@@ -919,9 +921,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tm_kernel(const __grid_cons
             const int32_t lim_first = p.q.past + (int32_t)(p.blk * 2 * kRowsL / a.group);
             for (uint32_t t = 0; t < n; ++t, ++v_seen) {
                 const uint32_t i = done + v_index(sm, t, n), slot = i % T::kSlots;
-                // (a slot is not filled again before its V tile has been reported; at most five reports are ahead of the tensor warp, the V tiles of a full ring)
-                // (first that the slot was free: a copy before it that has not landed yet would leave the barrier one phase behind, where this
-                // phase's parity reads as complete)
+                // (a slot is not filled again before its V tile has been reported; at most five reports are ahead of the tensor warp, the V
+                // tiles of a full ring; first that the slot was free: a copy before it that has not landed yet would leave the barrier one
+                // phase behind, where this phase's parity reads as complete)
                 if (!wait(&hd.empty[slot], ((i / T::kSlots) & 1u) ^ 1u) || !wait(&hd.full[slot], (i / T::kSlots) & 1u)) break;
                 if (!partly(a, p, p.t0 + t)) {
                     if (lane == 0) arrive(&hd.v_ready[v_seen & 7u]);

@@ -155,9 +155,9 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs
 }
 
 // ---- append ---------------------------------------------------------------------------------------------------------
-// Bound by HBM bytes. A CTA has one token (8192 tokens, 8B shape, f32: 66 us, four of them 69, eight 73), few tokens several CTAs each: the angles'
-// sines and cosines once in shared memory, then every thread 16 bytes of one head at a time, the next ones' load in flight. The angle pos * base^(-2i/n) is formed in turns in 64 bits and reduced before it is rounded: in
-// 32 bits a position of 120000 is 0.004 radians off.
+// Bound by HBM bytes. A CTA has one token (8192 tokens, 8B shape, f32: 66 us, four of them 69, eight 73), few tokens several CTAs each: the angles' sines and
+// cosines once in shared memory, then every thread 16 bytes of one head at a time, the next ones' load in flight. The angle pos *
+// base^(-2i/n) is formed in turns in 64 bits and reduced before it is rounded: in 32 bits a position of 120000 is 0.004 radians off.
 constexpr uint32_t kAppThreads = 256;
 
 struct AppendArgs {

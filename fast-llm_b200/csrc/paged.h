@@ -39,18 +39,21 @@ struct PagedAttnArgs {
     float scale;
 };
 
-// Sequences of few rows over a KV head (mma.sync: attn_paged.cu) and of many (tcgen05: attn_paged_tm.cu). kmap and vmap are filled in there. 16 is what
-// the first kernel's instances hold. us of both at 4 x 65000, 32 x 4000 and 1 x 8000 keys, 8 KV heads of 128, pages of 16: 4 rows 166, 91, 17 and 243, 197, 40 (f16 166,
-// 89, 16 and 187, 143, 32); 16 rows 200, 150, 29 and 257, 181, 34 (f16 200, 126, 29 and 188, 134, 30).
+// Sequences of few rows over a KV head (mma.sync: attn_paged.cu) and of many (tcgen05: attn_paged_tm.cu). kmap and vmap are filled in
+// there. 16 is what the first kernel's instances hold. us of both at 4 x 65000, 32 x 4000 and 1 x 8000 keys, 8 KV heads of 128, pages of
+// 16: 4 rows 166, 91, 17 and 243, 197, 40 (f16 166, 89, 16 and 187, 143, 32); 16 rows 200, 150, 29 and 257, 181, 34 (f16 200, 126, 29 and
+// 188, 134, 30).
 constexpr uint32_t kFewRows = 16;
-// Up to 32 sequences, of few rows and of many: the second kernel takes all of them where those of few rows are less work than a launch of their own
-// in front of it, in tiles of 128 keys; a sequence's start and end over a KV head count as 60. us with two launches and with one, 8 KV heads of 128 dimensions, single
-// tokens over so many keys: f32, beside 500 tokens over 4000 keys 8 x 4000 133 and 122, 12 x 4000 144 and 138, 16 x 4000 151 and 149, 1 x 65000 161 and 143, 2 x 65000 196
-// and 202; beside 30 over 1000 12 x 2000 49 and 61; beside 200 over 500 28 x 300 40 and 65. f16, whose tiles take the second kernel half as long: 8 x 4000 100 and 85, 16 x
-// 4000 118 and 107, 2 x 65000 162 and 148, 12 x 2000 44 and 45, 28 x 300 37 and 45; f16 and heads of 64: 8 x 4000 74 and 72, 16 x 4000 87 and 96.
+// Up to 32 sequences, of few rows and of many: the second kernel takes all of them where those of few rows are less work than a launch of
+// their own in front of it, in tiles of 128 keys; a sequence's start and end over a KV head count as 60. us with two launches and with one,
+// 8 KV heads of 128 dimensions, single tokens over so many keys: f32, beside 500 tokens over 4000 keys 8 x 4000 133 and 122, 12 x 4000 144
+// and 138, 16 x 4000 151 and 149, 1 x 65000 161 and 143, 2 x 65000 196 and 202; beside 30 over 1000 12 x 2000 49 and 61; beside 200 over
+// 500 28 x 300 40 and 65. f16, whose tiles take the second kernel half as long: 8 x 4000 100 and 85, 16 x 4000 118 and 107, 2 x 65000 162
+// and 148, 12 x 2000 44 and 45, 28 x 300 37 and 45; f16 and heads of 64: 8 x 4000 74 and 72, 16 x 4000 87 and 96.
 constexpr uint32_t kSpareStart = 60, kSpare = 6500, kSpareHalf128 = 12000;
-// Where the table's width bounds that work by as much as this the first kernel is not launched (4 x 8 tokens over 4096 keys 39.6 us, 36 without). The price: single
-// tokens in a call that allows more, as a recorded one may, run on the second kernel (1 x 8000 keys 24 us, 31 so; 4 x 1000 18, 24).
+// Where the table's width bounds that work by as much as this the first kernel is not launched (4 x 8 tokens over 4096 keys 39.6 us, 36
+// without). The price: single tokens in a call that allows more, as a recorded one may, run on the second kernel (1 x 8000 keys 24 us, 31
+// so; 4 x 1000 18, 24).
 constexpr uint32_t kSpareNoLaunch = 4000, kSpareAll = 0xffffffffu;
 cudaError_t paged_few_init(void);
 size_t paged_few_part_bytes(int sms);
@@ -69,8 +72,8 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedAttnArgs &a, uint32_t s
     bad = b < 0 || e < b || (uint32_t)e > a.n_tokens || (uint32_t)(e - b) > a.max_new || len < 0 || (uint64_t)len > room;
     return bad ? PagedSeq{0, 0, 0} : PagedSeq{(uint32_t)b, (uint32_t)(e - b), len - (e - b)};
 }
-// The rows that a sequence of the first kernel has at most (lane i holds sequence i, of up to 32): none where the second one has others to work on and
-// takes those too.
+// The rows that a sequence of the first kernel has at most (lane i holds sequence i, of up to 32): none where the second one has others to
+// work on and takes those too.
 __device__ __forceinline__ uint32_t few_limit(const PagedAttnArgs &a, const PagedSeq &q) {
     if (a.spare == 0 || a.spare == kSpareAll) return a.spare ? 0u : kFewRows;
     const uint32_t rows = q.n * a.group, tiles = ((uint32_t)max(0, q.past + (int32_t)q.n) + 127) / 128;

@@ -55,8 +55,8 @@ FLB_HD uint32_t last_of(const Shares &sh, uint32_t snap, uint32_t b, uint32_t e)
     return lo > b && snapped(sh, snap, lo, b, e) == e ? c - 1 : c;
 }
 
-// A run's ticket, zero between launches: CTAs that arrived in the low half, those of them that gave up a wait, and left no record, in the high half. The
-// last to arrive resets it, and adds the records where there are all of them.
+// A run's ticket, zero between launches: CTAs that arrived in the low half, those of them that gave up a wait, and left no record, in the
+// high half. The last to arrive resets it, and adds the records where there are all of them.
 FLB_HD uint32_t ticket_step(bool gave_up) { return gave_up ? 0x10001u : 1u; }
 FLB_HD bool ticket_last(uint32_t before, uint32_t pieces) { return (before & 0xFFFFu) == pieces - 1; }
 FLB_HD bool ticket_complete(uint32_t before, bool gave_up) { return before >> 16 == 0 && !gave_up; }
@@ -68,8 +68,8 @@ FLB_HD Shares tm_shares(uint32_t units, uint32_t ctas) { return shares_of(units,
 FLB_HD uint32_t tile_at_unit(uint32_t at, uint32_t front, uint32_t tiles, uint32_t tile_units) {
     return at > front ? lesser(tiles, (at - front + tile_units - 1) >> (tile_units - 1)) : 0u;   // (1 or 2)
 }
-// The record of a block's CTA `first + i` is its second (slot 1) where the block begins behind another one's tiles, which only the first CTA's can; every CTA
-// notes which of its two it left: left[2 cta + slot].
+// The record of a block's CTA `first + i` is its second (slot 1) where the block begins behind another one's tiles, which only the first
+// CTA's can; every CTA notes which of its two it left: left[2 cta + slot].
 FLB_HD uint32_t record_index(uint32_t first, uint32_t i, uint32_t slot) { return 2 * (first + i) + (i ? 0u : slot); }
 
 // ---- pages ----------------------------------------------------------------------------------------------------------

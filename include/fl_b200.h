@@ -219,16 +219,16 @@ typedef struct {
 } fl_b200_paged_cache;
 /* Activations of the paged calls: f32 as everywhere else in this library, or f16. */
 enum { FL_B200_ACT_F32 = 0, FL_B200_ACT_F16 = 1 };
-/* The plan of a step, from the sequences' lengths: sequence s (of n_seq <= 4096) holds the pages of held[s] tokens, keeps the
- * first past[s] <= held[s] of them and gets fresh[s] more (a prompt: held = past = 0; a rewound draft: past < held; an ended
- * request: past = fresh = 0). Row s of the block table ([n_seq][max_blocks]) names its pages in order, and the first
- * free_count entries of free_list ([n_pages]) the unused ones, the last of them the next to go. Pages that past + fresh tokens do not
- * need go onto the list in order of (s, block); then the missing ones are taken from its end in the same order and written into
- * the table behind the ones held. Other entries of table and list stay as they are. Outputs: *free_count_out (may be
- * free_count_in itself), q_start[n_seq + 1] = first token of each sequence in the step's batch, kv_len[s] = past + fresh (may be held,
- * past or fresh itself), and per token of the batch its position and its slot; the rest of pos and slot (max_tokens
- * each) is -1. Where pages or max_tokens do not suffice (status 5) or lengths are impossible (status 4) the plan is empty: q_start 0, every
- * pos and slot -1, all else unchanged. A token on a page that no pool has (negative, or past 2^31 rows) gets slot -1 (status 3). No page may be listed twice. Other buffers must not overlap. */
+/* The plan of a step, from the sequences' lengths: sequence s (of n_seq <= 4096) holds the pages of held[s] tokens, keeps the first
+ * past[s] <= held[s] of them and gets fresh[s] more (a prompt: held = past = 0; a rewound draft: past < held; an ended request: past =
+ * fresh = 0). Row s of the block table ([n_seq][max_blocks]) names its pages in order, and the first free_count entries of free_list
+ * ([n_pages]) the unused ones, the last of them the next to go. Pages that past + fresh tokens do not need go onto the list in order
+ * of (s, block); then the missing ones are taken from its end in the same order and written into the table behind the ones held. Other
+ * entries of table and list stay as they are. Outputs: *free_count_out (may be free_count_in itself), q_start[n_seq + 1] = first token
+ * of each sequence in the step's batch, kv_len[s] = past + fresh (may be held, past or fresh itself), and per token of the batch its
+ * position and its slot; the rest of pos and slot (max_tokens each) is -1. Where pages or max_tokens do not suffice (status 5) or
+ * lengths are impossible (status 4) the plan is empty: q_start 0, every pos and slot -1, all else unchanged. A token on a page that no
+ * pool has (negative, or past 2^31 rows) gets slot -1 (status 3). No page may be listed twice. Other buffers must not overlap. */
 int fl_b200_paged_plan(fl_b200_ctx *ctx, const int32_t *held_dev, const int32_t *past_dev, const int32_t *fresh_dev,
                        uint32_t n_seq, uint32_t page_size, int32_t *table_dev, uint32_t max_blocks, int32_t *free_list_dev,
                        uint32_t n_pages, const int32_t *free_count_in_dev, int32_t *free_count_out_dev, int32_t *q_start_dev,
@@ -243,22 +243,22 @@ int fl_b200_paged_append(fl_b200_ctx *ctx, const fl_b200_paged_cache *cache, int
                          uint32_t q_stride, const void *k_dev, const void *v_dev, uint32_t kv_stride, const int32_t *pos_dev,
                          const int32_t *slot_dev, uint32_t n_tokens, uint32_t n_rot, float freq_base, void *q_out_dev,
                          uint32_t q_out_stride);
-/* Causal grouped-query attention of every sequence's new tokens over its pages: fl_b200_attn_decode, fl_b200_attn_verify and prompt chunks in
- * one call. Sequence s has tokens q_start[s] .. q_start[s + 1] - 1 of the batch and kv_len[s] keys, its new tokens' own
- * the last of them; token i of n attends keys 0 .. kv_len - n + i. A token without a key gets zeros. n_q_head is a multiple of
- * n_kv_head (groups of up to 128), q and out [n_tokens][stride] as above, table [n_seq][max_blocks] (max_blocks * page_size <= 2^31 - 256), scale
- * positive. n_tokens: rows of q and out; max_new: the most new tokens that any sequence has. Sequences whose lengths break these bounds are left
- * out (status 4), and so are lines of together 2^31 or more tiles of 256 rows by 128 keys over all KV heads (a minute's work; of few rows: a sequence of
- * 2^26 tiles of 64 keys); rows of out that belong to no sequence stay as they are, keys on a page outside the pool count as zero vectors (status 3). After a wait that ran out (status
- * 1) rows may be left as they were, none is written in part. What a row does not attend may hold
- * anything; an infinity that it does attend may make it NaN. lse_out
- * (optional): per token and query head (max score, sum of exp(score - max)), (-inf, 0) without a key: what fl_b200_seqpar_combine merges.
- * Where max_new * n_q_head / n_kv_head is above 16 the call prepares for chunks: one whose sequences then all have a token is 8 to 25 us slower than
- * with max_new 1, so that graphs of decode steps are best recorded with their own max_new.
- * f32 activations: q and the probabilities go to the tensor cores as two f16 parts each (21 bits; a probability is held to 2^-36 of its row's
- * largest where that is more), sums in f32. f16 activations: q as it is; the probabilities of sequences of up to 16 rows (tokens * n_q_head / n_kv_head) as two
- * parts, of others, and of short ones that a call takes along with a chunk, as one f16 (half a step of 2^-11, as the result's own; sums in f32 but for
- * 2^-13 at most): a request's last bit may depend on its batch.
+/* Causal grouped-query attention of every sequence's new tokens over its pages: fl_b200_attn_decode, fl_b200_attn_verify and prompt
+ * chunks in one call. Sequence s has tokens q_start[s] .. q_start[s + 1] - 1 of the batch and kv_len[s] keys, its new tokens' own the
+ * last of them; token i of n attends keys 0 .. kv_len - n + i. A token without a key gets zeros. n_q_head is a multiple of n_kv_head
+ * (groups of up to 128), q and out [n_tokens][stride] as above, table [n_seq][max_blocks] (max_blocks * page_size <= 2^31 - 256),
+ * scale positive. n_tokens: rows of q and out; max_new: the most new tokens that any sequence has. Sequences whose lengths break these
+ * bounds are left out (status 4), and so are lines of together 2^31 or more tiles of 256 rows by 128 keys over all KV heads (a
+ * minute's work; of few rows: a sequence of 2^26 tiles of 64 keys); rows of out that belong to no sequence stay as they are, keys on a
+ * page outside the pool count as zero vectors (status 3). After a wait that ran out (status 1) rows may be left as they were, none is
+ * written in part. What a row does not attend may hold anything; an infinity that it does attend may make it NaN. lse_out (optional):
+ * per token and query head (max score, sum of exp(score - max)), (-inf, 0) without a key: what fl_b200_seqpar_combine merges.
+ * Where max_new * n_q_head / n_kv_head is above 16 the call prepares for chunks: one whose sequences then all have a token is 8 to 25
+ * us slower than with max_new 1, so that graphs of decode steps are best recorded with their own max_new.
+ * f32 activations: q and the probabilities go to the tensor cores as two f16 parts each (21 bits; a probability is held to 2^-36 of
+ * its row's largest where that is more), sums in f32. f16 activations: q as it is; the probabilities of sequences of up to 16 rows
+ * (tokens * n_q_head / n_kv_head) as two parts, of others, and of short ones that a call takes along with a chunk, as one f16 (half a
+ * step of 2^-11, as the result's own; sums in f32 but for 2^-13 at most): a request's last bit may depend on its batch.
  * out must not overlap q. The first call on a context allocates scratch (65 MB): make it before a capture. */
 int fl_b200_paged_attn(fl_b200_ctx *ctx, const fl_b200_paged_cache *cache, int act_type, const void *q_dev, uint32_t n_q_head,
                        uint32_t q_stride, const int32_t *table_dev, uint32_t max_blocks, const int32_t *q_start_dev,
