@@ -247,12 +247,13 @@ int fl_b200_paged_append(fl_b200_ctx *ctx, const fl_b200_paged_cache *cache, int
  * chunks in one call. Sequence s has tokens q_start[s] .. q_start[s + 1] - 1 of the batch and kv_len[s] keys, its new tokens' own the
  * last of them; token i of n attends keys 0 .. kv_len - n + i. A token without a key gets zeros. n_q_head is a multiple of n_kv_head
  * (groups of up to 128), q and out [n_tokens][stride] as above, table [n_seq][max_blocks] (max_blocks * page_size <= 2^31 - 256),
- * scale positive. n_tokens: rows of q and out; max_new: the most new tokens that any sequence has. Sequences whose lengths break these
- * bounds are left out (status 4), and so are lines of together 2^31 or more tiles of 256 rows by 128 keys over all KV heads (a
- * minute's work; of few rows: a sequence of 2^26 tiles of 64 keys); rows of out that belong to no sequence stay as they are, keys on a
- * page outside the pool count as zero vectors (status 3). After a wait that ran out (status 1) rows may be left as they were, none is
- * written in part. What a row does not attend may hold anything; an infinity that it does attend may make it NaN. lse_out (optional):
- * per token and query head (max score, sum of exp(score - max)), (-inf, 0) without a key: what fl_b200_seqpar_combine merges.
+ * scale positive, |scale * q.k| below 2^24 (f32 tells keys apart no further; a row beyond may become NaN). n_tokens: rows of q and
+ * out; max_new: the most new tokens that any sequence has. Sequences whose lengths break these bounds are left out (status 4), and so
+ * are lines of together 2^31 or more tiles of 256 rows by 128 keys over all KV heads (a minute's work; of few rows: a sequence of 2^26
+ * tiles of 64 keys); rows of out that belong to no sequence stay as they are, keys on a page outside the pool count as zero vectors
+ * (status 3). After a wait that ran out (status 1) rows may be left as they were, none is written in part. What a row does not attend
+ * may hold anything; an infinity that it does attend may make it NaN. lse_out (optional): per token and query head (max score, sum of
+ * exp(score - max)), (-inf, 0) without a key: what fl_b200_seqpar_combine merges.
  * Where max_new * n_q_head / n_kv_head is above 16 the call prepares for chunks: one whose sequences then all have a token is 8 to 25
  * us slower than with max_new 1, so that graphs of decode steps are best recorded with their own max_new.
  * f32 activations: q and the probabilities go to the tensor cores as two f16 parts each (21 bits; a probability is held to 2^-36 of

@@ -858,3 +858,25 @@ def test_sequences_of_few_rows_beside_chunks(ctx, seqs, wide, max_new, act, dim)
         c["lse"] = torch.full((max_new + 2, n_q, 2), CANARY, device="cuda")
     attn(ctx, c, n_q, n_kv, dim, page, 1.0 / math.sqrt(dim), max_new=max_new)
     check(ctx, c, seqs, n_q, n_kv, dim, 1.0 / math.sqrt(dim), act)
+
+
+@pytest.mark.parametrize("act", ["f32", "f16"])
+@pytest.mark.parametrize("seqs", [[(300, 1), (70, 2)], [(300, 100)]])
+def test_scores_of_millions(ctx, seqs, act):
+    """Rows whose scores reach 2^23: the largest takes all (the next one is 1000 below at least), its value comes back."""
+    n_q, n_kv, dim, page = 8, 2, 128, 16
+    c = make(41, seqs, n_q, n_kv, dim, page, act)
+    c["q"].fill_(16.0)
+    for s, (L, _) in enumerate(seqs):
+        j = torch.arange(L, device="cuda")
+        c["ks"][s].zero_()
+        c["ks"][s][:, :, 1] = 32 * ((j * 37) % L).half()       # whole numbers below 2^14, all different
+        c["k"][c["table"][s].long()[j // page], :, j % page] = c["ks"][s].transpose(0, 1)
+    attn(ctx, c, n_q, n_kv, dim, page, 50.0)                    # 16 * 32 * 50 = 25600 a step, up to 7.7e6
+    assert ctx.status() == 0
+    got = c["out"].double().view(-1, n_q, dim)
+    for s, (L, m) in enumerate(seqs):
+        for i in range(m):
+            best = int(((torch.arange(L - m + i + 1) * 37) % L).argmax())
+            want = c["vs"][s][:, best].double().repeat_interleave(n_q // n_kv, 0)
+            assert ((got[c["start"][s] + i] - want).abs() <= (2.0 ** -20 + (2.0 ** -10 if act == "f16" else 0)) * want.abs()).all()
